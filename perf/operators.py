@@ -24,7 +24,7 @@ DEV = "cuda"
 BF = torch.bfloat16
 IGNORE = -100
 HEADS = ((4, 2, 64), (14, 2, 64), (32, 8, 64), (24, 24, 64), (12, 2, 128), (28, 4, 128))
-SECTIONS = {64: "8,12,12", 128: "16,24,24"}
+SECTIONS = {(64, False): (8, 12, 12), (128, False): (16, 24, 24), (64, True): (12, 10, 10), (128, True): (24, 20, 20)}
 
 
 def listed():
@@ -164,7 +164,7 @@ def prepare(case, seed):
         inv = 1.0 / 1e6 ** (torch.arange(0, case["d"], 2, dtype=torch.float64, device=DEV) / case["d"])
         ang = torch.arange(n, dtype=torch.float64, device=DEV)[:, None] * inv
         s["cos"], s["sin"] = ang.cos().float(), ang.sin().float()
-        s["sections"] = tuple(int(x) for x in SECTIONS[case["d"]].split(","))
+        s["sections"] = SECTIONS[case["d"], case["cyclic"]]
     else:
         T, V = case["T"], case["V"]
         s["idx"], s["lg"], s["labels"] = _teacher(g, T, V, case["K"])
