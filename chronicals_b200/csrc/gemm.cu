@@ -49,7 +49,8 @@ struct GemmArgs {
   const bf16* addend;
   long long ld_add;
   // cut-cross-entropy
-  const long long* labels;  // [M], global vocab ids, ignore_index allowed
+  const long long* labels;  // [M], global vocab ids, ignore_index allowed; null: no row has a label
+  float e2_scale;           // log2(e) over the temperature: a logit v stands for 2^(v e2_scale)
   float* part_m;            // [n_splits, M]
   float* part_s;            // [n_splits, M]
   float* part_sum;          // [n_splits, M] or null (only for label smoothing)
@@ -282,8 +283,9 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       float run_m = -INFINITY, run_s = 0.f, run_sum = 0.f;
       int lab = -1;
       float lse_r = 0.f, gs = 0.f, coef = 1.f;
+      const float e2 = g.e2_scale;
       if (EPI != EPI_STORE && row_ok) {
-        const long long l = g.labels[row];
+        const long long l = g.labels != nullptr ? g.labels[row] : -1;
         const long long rel = l - g.col_offset;
         lab = (l >= 0 && rel >= 0 && rel < g.N) ? static_cast<int>(rel) : -1;
         if (EPI == EPI_DLOGITS) {
@@ -337,7 +339,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 // run one per scheduler, so every instruction in this loop is paid at its full latency)
                 const float cg = coef * gs, smg = sm * gs;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = fmaf(ex2_approx(fmaf(v[j], 1.4426950408889634f, -l2)), cg, -smg);
+                for (int j = 0; j < 32; ++j) v[j] = fmaf(ex2_approx(fmaf(v[j], e2, -l2)), cg, -smg);
                 if (rel >= 0 && rel < 32) {
                   const float hit = (1.f - g.smoothing) * gs;
 #pragma unroll
@@ -461,17 +463,17 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 if (full_chunk || col0 + j < g.N) cmax = fmaxf(cmax, v);
               }
               const float nm = fmaxf(run_m, cmax);
-              const float nm2 = nm * 1.4426950408889634f;
+              const float nm2 = nm * e2;
               float acc_s = 0.f, acc_l = 0.f;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const float v = __uint_as_float(r[j]);
                 if (full_chunk || col0 + j < g.N) {
-                  acc_s += exp2f(fmaf(v, 1.4426950408889634f, -nm2));
+                  acc_s += exp2f(fmaf(v, e2, -nm2));
                   acc_l += v;
                 }
               }
-              run_s = run_s * exp2f((run_m - nm) * 1.4426950408889634f) + acc_s;
+              run_s = run_s * exp2f((run_m - nm) * e2) + acc_s;
               run_m = nm;
               run_sum += acc_l;
               const int rel = lab - col0;
@@ -497,7 +499,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 // run one per scheduler, so every instruction in this loop is paid at its full latency)
                 const float cg = coef * gs, smg = sm * gs;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = fmaf(ex2_approx(fmaf(v[j], 1.4426950408889634f, -l2)), cg, -smg);
+                for (int j = 0; j < 32; ++j) v[j] = fmaf(ex2_approx(fmaf(v[j], e2, -l2)), cg, -smg);
                 if (rel >= 0 && rel < 32) {
                   const float hit = (1.f - g.smoothing) * gs;
 #pragma unroll
@@ -1042,10 +1044,11 @@ int cb_cce_num_splits(int M, int V) {
   return ((V + 255) / 256 + per - 1) / per;
 }
 
-// Forward: per-row log-sum-exp partials of hidden[M,K] * weight[V,K]^T, target logit.
-int cb_cce_forward(const void* hidden, const void* weight, const long long* labels, int M, int V, int K,
-                   long long ldh, long long ldw, int col_offset, float* part_m, float* part_s, float* part_sum,
-                   float* tgt, int* status, void* stream) {
+// Forward: per-row log-sum-exp partials of hidden[M,K] * weight[V,K]^T over the temperature (part_m: the maximum of the
+// logits themselves), target logit where there are labels (else labels and tgt are null).
+int cb_cce_forward_t(const void* hidden, const void* weight, const long long* labels, int M, int V, int K,
+                     long long ldh, long long ldw, int col_offset, float e2_scale, float* part_m, float* part_s, float* part_sum,
+                     float* tgt, int* status, void* stream) {
   const int bn = 256;
   CUtensorMap ta, tb;
   int e = build_maps(&ta, &tb, hidden, weight, M, V, K, ldh, ldw, 0, 0, bn);
@@ -1058,12 +1061,20 @@ int cb_cce_forward(const void* hidden, const void* weight, const long long* labe
   const int n_splits = (g.num_n_tiles + g.tiles_per_item - 1) / g.tiles_per_item;
   g.num_items = g.num_m_blocks * n_splits;
   g.labels = labels;
+  g.e2_scale = e2_scale;
   g.part_m = part_m; g.part_s = part_s; g.part_sum = part_sum; g.tgt = tgt;
   g.col_offset = col_offset;
   g.status = status;
   CUtensorMap tc;
   memset(&tc, 0, sizeof(tc));
   return dispatch<cb::EPI_LSE>(bn, 0, 0, ta, tb, tc, g, static_cast<cudaStream_t>(stream));
+}
+
+int cb_cce_forward(const void* hidden, const void* weight, const long long* labels, int M, int V, int K,
+                   long long ldh, long long ldw, int col_offset, float* part_m, float* part_s, float* part_sum,
+                   float* tgt, int* status, void* stream) {
+  return cb_cce_forward_t(hidden, weight, labels, M, V, K, ldh, ldw, col_offset, 1.4426950408889634f, part_m, part_s, part_sum,
+                          tgt, status, stream);
 }
 
 int cb_cce_combine(const float* part_m, const float* part_s, const float* part_sum, const float* tgt,
@@ -1079,11 +1090,11 @@ int cb_cce_combine(const float* part_m, const float* part_s, const float* part_s
 }
 
 // Backward, step 1: G[M, Vc] = d(loss)/d(logits) for the vocab columns [col_offset, col_offset + Vc)
-// of `weight_chunk` (= weight + col_offset * ldw), written as bf16 with row pitch ldg.
-int cb_cce_dlogits(const void* hidden, const void* weight_chunk, const long long* labels, const float* lse,
-                   const float* gscale, const float* gout, void* G, int M, int Vc, int K, long long ldh,
-                   long long ldw, long long ldg, int col_offset, int V_total, float smoothing, float z_weight,
-                   int* status, void* stream) {
+// of `weight_chunk` (= weight + col_offset * ldw), written as bf16 with row pitch ldg.  lse: of the logits over the temperature.
+int cb_cce_dlogits_t(const void* hidden, const void* weight_chunk, const long long* labels, const float* lse,
+                     const float* gscale, const float* gout, void* G, int M, int Vc, int K, long long ldh,
+                     long long ldw, long long ldg, int col_offset, int V_total, float smoothing, float z_weight,
+                     float e2_scale, int* status, void* stream) {
   const int bn = pick_block_n(M, Vc, 0);
   CUtensorMap ta, tb;
   int e = build_maps(&ta, &tb, hidden, weight_chunk, M, Vc, K, ldh, ldw, 0, 0, bn);
@@ -1096,12 +1107,21 @@ int cb_cce_dlogits(const void* hidden, const void* weight_chunk, const long long
   g.num_items = g.num_m_blocks * g.num_n_tiles;
   g.C = G; g.ldc = ldg; g.out_fp32 = 0; g.accumulate = 0;
   g.labels = labels; g.lse = lse; g.gscale = gscale; g.gout = gout;
+  g.e2_scale = e2_scale;
   g.z_weight = z_weight; g.smoothing = smoothing; g.V_total = V_total; g.col_offset = col_offset;
   g.status = status;
   CUtensorMap tc;
   e = build_out_map(&tc, &g.tma_store, G, M, Vc, ldg, 0);
   if (e) return e;
   return dispatch<cb::EPI_DLOGITS>(bn, 0, 0, ta, tb, tc, g, static_cast<cudaStream_t>(stream));
+}
+
+int cb_cce_dlogits(const void* hidden, const void* weight_chunk, const long long* labels, const float* lse,
+                   const float* gscale, const float* gout, void* G, int M, int Vc, int K, long long ldh,
+                   long long ldw, long long ldg, int col_offset, int V_total, float smoothing, float z_weight,
+                   int* status, void* stream) {
+  return cb_cce_dlogits_t(hidden, weight_chunk, labels, lse, gscale, gout, G, M, Vc, K, ldh, ldw, ldg, col_offset, V_total,
+                          smoothing, z_weight, 1.4426950408889634f, status, stream);
 }
 
 }  // extern "C"

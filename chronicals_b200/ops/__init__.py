@@ -9,10 +9,12 @@ On a CUDA device the kernel library is mandatory; a missing library raises.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 import os
 import weakref
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -20,8 +22,10 @@ from . import ref
 from . import _ext
 
 __all__ = [
-    "linear", "gemm", "gemm_dual", "gemm_splitk", "colsum", "rmsnorm", "rmsnorm_residual", "add_rmsnorm", "swiglu", "geglu", "qk_rope_", "embedding",
-    "attention_varlen", "attention_qkv_packed", "linear_cross_entropy", "cross_entropy_logits", "kernels_active",
+    "linear", "gemm", "gemm_dual", "gemm_splitk", "colsum", "rmsnorm", "rmsnorm_residual", "add_rmsnorm", "swiglu", "geglu", "qk_rope_", "qk_rope_axes_",
+    "embedding",
+    "attention_varlen", "attention_qkv_packed", "linear_cross_entropy", "cross_entropy_logits",
+    "distillation_logits", "linear_distillation", "kernels_active",
 ]
 
 
@@ -624,6 +628,93 @@ def qk_rope_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, position_i
     return torch.cat((q.reshape(T, nq), k.reshape(T, nk), qkv[:, nq + nk:]), dim=-1)
 
 
+def _same_device(op: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Kernels run on the current device's stream: refuses tensors of several devices, or of one that is not current."""
+    devs = {t.device for t in tensors if t is not None}
+    if len(devs) > 1:
+        raise ValueError(f"{op}: tensors on several devices: {sorted(map(str, devs))}")
+    for d in devs:
+        if d.type == "cuda" and d.index != torch.cuda.current_device():
+            raise ValueError(f"{op}: tensors on {d}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_axis_words(sections: Tuple[int, ...], cyclic: bool):
+    """The axis map of a head for the kernel: two bits a frequency, 16 frequencies a word."""
+    ax = ref.rope_axis_map(sections, cyclic)
+    words = (ctypes.c_uint32 * (-(-len(ax) // 16)))()
+    for f, a in enumerate(ax):
+        words[f // 16] |= a << 2 * (f % 16)
+    return words
+
+
+def _rope_axes_launch(src, dst, cos, sin, pos, hq, hk, d, sections, cyclic, interleaved, inverse):
+    words = _rope_axis_words(sections, cyclic)
+    code = _ext.lib().cb_qk_rope_axes(src.data_ptr(), dst.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), pos.stride(0),
+                                      pos.shape[0], src.shape[0], hq + hk, 0 if dst is src else hk, d, src.stride(0), dst.stride(0),
+                                      ctypes.addressof(words), int(interleaved), int(inverse), cos.shape[0], _ext.stream_ptr())
+    _ext.check(code, "qk_rope_axes")
+    return dst
+
+
+class _QKRopeAxesFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, cos, sin, pos, cfg):
+        _rope_axes_launch(qkv, qkv, cos, sin, pos, *cfg)
+        ctx.mark_dirty(qkv)
+        ctx.save_for_backward(cos, sin, pos)
+        ctx.cfg = cfg
+        return qkv
+
+    @staticmethod
+    def backward(ctx, dqkv):
+        cos, sin, pos = ctx.saved_tensors
+        # the gradient that comes in may be another node's too: the rotated one goes to a buffer of its own
+        g = dqkv if _rope_axes_rows(dqkv) else dqkv.contiguous()
+        return _rope_axes_launch(g, torch.empty_like(g, memory_format=torch.contiguous_format), cos, sin, pos, *ctx.cfg[:-1],
+                                 not ctx.cfg[-1]), None, None, None, None
+
+
+def _rope_axes_rows(t: torch.Tensor) -> bool:
+    return t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 and (t.shape[0] < 2 or t.stride(0) >= t.shape[1])
+
+
+def qk_rope_axes_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, position_ids: torch.Tensor, num_q_heads: int,
+                  num_kv_heads: int, head_dim: int, sections: Sequence[int], *, cyclic: bool = False, interleaved: bool = False,
+                  inverse: bool = False) -> torch.Tensor:
+    """:func:`qk_rope_` for tokens with one position per axis, such as the time, height and width of images and video.
+
+    ``position_ids [axes, T]`` (one to four axes); ``sections`` says how many of the ``head_dim / 2`` frequencies turn by which
+    axis: blocks one behind the other, or (``cyclic``) dealt to the axes in turn, axis 0 taking what is left over.  ``cos`` and
+    ``sin`` are the tables of :func:`ref.rope_cache`, one row a position; positions outside them use the first or last row.
+    ``inverse`` turns back.  In place on CUDA; returns the rotated buffer.  The backward pass turns the gradient back into a
+    buffer of its own."""
+    sections = tuple(int(n) for n in sections)
+    if qkv.dim() != 2 or qkv.shape[1] != (num_q_heads + 2 * num_kv_heads) * head_dim:
+        raise ValueError(f"qk_rope_axes_: qkv {tuple(qkv.shape)} is not [T, (hq + 2 hk) * d] for hq, hk, d = "
+                         f"{num_q_heads}, {num_kv_heads}, {head_dim}")
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or 2 * sum(sections) != head_dim:
+        raise ValueError(f"qk_rope_axes_: sections {sections} must be one to four counts that sum up to head_dim / 2 = {head_dim / 2:g}")
+    if position_ids.shape != (len(sections), qkv.shape[0]) or position_ids.dtype.is_floating_point or position_ids.dtype == torch.bool:
+        raise ValueError(f"qk_rope_axes_: position_ids {tuple(position_ids.shape)} {position_ids.dtype}, wanted whole numbers of shape "
+                         f"{(len(sections), qkv.shape[0])}")
+    if cyclic and any(n and a + len(sections) * (n - 1) >= head_dim // 2 for a, n in enumerate(sections) if a):
+        raise ValueError(f"qk_rope_axes_: sections {sections} cannot be dealt in turn: an axis other than the first has more than its share")
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] * 2 != head_dim or cos.shape[0] == 0:
+        raise ValueError(f"qk_rope_axes_: tables {tuple(cos.shape)} and {tuple(sin.shape)}, wanted [positions, head_dim / 2]")
+    _same_device("qk_rope_axes_", qkv, cos, sin, position_ids)
+    if _fast(qkv) and head_dim % 16 == 0 and head_dim <= 512 and _rope_axes_rows(qkv):
+        pos = position_ids.long()
+        if pos.stride(1) != 1:
+            pos = pos.contiguous()
+        return _QKRopeAxesFn.apply(qkv, cos.float().contiguous(), sin.float().contiguous(), pos,
+                                   (num_q_heads, num_kv_heads, head_dim, sections, bool(cyclic), bool(interleaved), bool(inverse)))
+    T, nqk = qkv.shape[0], (num_q_heads + num_kv_heads) * head_dim
+    c, s = ref.rope_axes_tables(cos, sin, position_ids, ref.rope_axis_map(sections, cyclic))
+    y = ref.apply_rope(qkv[:, :nqk].reshape(T, -1, head_dim), c, s, None, interleaved, inverse)
+    return torch.cat((y.reshape(T, nqk), qkv[:, nqk:]), dim=-1)
+
+
 # ============================================================================ embedding
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
@@ -928,3 +1019,187 @@ def cross_entropy_logits(logits: torch.Tensor, labels: torch.Tensor, ignore_inde
             return rows.sum()
         return rows.sum() / (y != ignore_index).sum().clamp_min(1)
     return ref.cross_entropy_logits(lg, y, ignore_index, label_smoothing, z_loss_weight, reduction)
+
+
+# ============================================================================ distillation from a teacher's top logits
+def _distill_args(op, lead, V, idx, lg, temperature, labels, reduction, *others):
+    """Checks, and the teacher's entries as the kernels read them: ``(idx [rows, K], logits [rows, K], labels or None)``."""
+    K = idx.shape[-1] if idx.dim() else 0
+    if idx.shape != (*lead, K) or lg.shape != idx.shape or K < 1:
+        raise ValueError(f"{op}: teacher_indices {tuple(idx.shape)} and teacher_logits {tuple(lg.shape)}, wanted {(*lead, 'K')} with K >= 1")
+    if idx.dtype.is_floating_point or idx.dtype.is_complex or idx.dtype == torch.bool:
+        raise ValueError(f"{op}: teacher_indices are {idx.dtype}, wanted whole numbers")
+    if not lg.dtype.is_floating_point:
+        raise ValueError(f"{op}: teacher_logits are {lg.dtype}, wanted floating-point numbers")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"{op}: temperature {temperature} must be positive and finite")
+    if labels is not None and (labels.shape != lead or labels.dtype.is_floating_point):
+        raise ValueError(f"{op}: labels {tuple(labels.shape)} {labels.dtype}, wanted whole numbers of shape {tuple(lead)}")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"{op}: reduction {reduction!r} is not 'mean', 'sum' or 'none'")
+    if V < 1:
+        raise ValueError(f"{op}: the vocabulary is empty")
+    _same_device(op, idx, lg, labels, *others)
+    idx, lg = idx.reshape(-1, K), lg.detach().reshape(-1, K)
+    if idx.dtype not in (torch.int64, torch.int32):
+        idx = idx.long()
+    if lg.dtype not in (torch.float32, torch.bfloat16, torch.float64):
+        lg = lg.float()
+    idx, lg = (t if t.stride(1) == 1 else t.contiguous() for t in (idx, lg))
+    return idx, lg, None if labels is None else labels.reshape(-1).long().contiguous()
+
+
+def _teacher_ptrs(idx, lg):
+    return (idx.data_ptr(), idx.stride(0), int(idx.dtype == torch.int64), lg.data_ptr(), lg.stride(0), int(lg.dtype == torch.bfloat16),
+            idx.shape[1])
+
+
+class _DistillLogitsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, idx, lg, labels, ignore_index, tau, mean):
+        rows, V = logits.shape
+        f32 = dict(dtype=torch.float32, device=logits.device)
+        stats, q = torch.empty(rows, 2, **f32), torch.empty(rows, idx.shape[1], **f32)
+        loss_rows, out = torch.empty(rows, **f32), torch.empty(2, **f32)
+        code = _ext.lib().cb_kd_logits(logits.data_ptr(), rows, logits.stride(0), V, int(logits.dtype == torch.bfloat16),
+                                       *_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau, int(mean), stats.data_ptr(),
+                                       q.data_ptr(), loss_rows.data_ptr(), out.data_ptr(), _ext.stream_ptr())
+        _ext.check(code, "kd_logits")
+        ctx.save_for_backward(logits, idx, lg, labels, stats, q, out)
+        ctx.cfg = (ignore_index, tau, mean)
+        ctx.set_materialize_grads(False)
+        return out[0], loss_rows
+
+    @staticmethod
+    def backward(ctx, gout, grows):
+        logits, idx, lg, labels, stats, q, out = ctx.saved_tensors
+        ignore_index, tau, mean = ctx.cfg
+        rows, V = logits.shape
+        ld = logits.stride(0)
+        # rows as far apart as the logits', so that both start at the same distance from a 16-byte boundary
+        dl = torch.empty_strided((rows, V), (ld, 1) if V <= ld < 2 * V else (V, 1), dtype=logits.dtype, device=logits.device)
+        gout = None if gout is None else gout.float()
+        grows = None if grows is None else grows.float().contiguous()
+        code = _ext.lib().cb_kd_logits_grad(logits.data_ptr(), dl.data_ptr(), rows, ld, dl.stride(0), V,
+                                            int(logits.dtype == torch.bfloat16), *_teacher_ptrs(idx, lg), _ext.ptr(labels),
+                                            ignore_index, tau, stats.data_ptr(), q.data_ptr(), _ext.ptr(gout),
+                                            out[1].data_ptr() if mean else None, _ext.ptr(grows), _ext.stream_ptr())
+        _ext.check(code, "kd_logits_grad")
+        return dl, None, None, None, None, None, None
+
+
+def distillation_logits(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor, temperature: float = 1.0,
+                        labels: Optional[torch.Tensor] = None, ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """Distillation loss of ``logits [..., V]`` against a teacher's top logits ``[..., K]`` and their vocabulary indices:
+    ``temperature**2 * KL(teacher || student)``, the teacher's distribution the softmax of its K logits over ``temperature``, the
+    student's the softmax over the whole vocabulary.
+
+    Entries with an index outside the vocabulary (-1, say) or a logit of -inf are absent; entries of one index add up.  Rows
+    without an entry, and rows whose label is ``ignore_index`` where ``labels [...]`` are given, take no part: loss and gradient
+    are zero, and the mean is over the others.  No gradient goes to the teacher.  bf16 and fp32 logits run on the kernels."""
+    V = logits.shape[-1]
+    idx, lg, y = _distill_args("distillation_logits", logits.shape[:-1], V, teacher_indices, teacher_logits, temperature, labels,
+                               reduction, logits)
+    z = logits.reshape(-1, V)
+    if (z.is_cuda and not _ext.reference_forced() and z.dtype in (torch.bfloat16, torch.float32) and z.stride(1) == 1 and z.shape[0]
+            and idx.shape[1] <= _ext.lib().cb_kd_max_entries()):
+        lg = lg.float() if lg.dtype == torch.float64 else lg
+        loss, rows = _DistillLogitsFn.apply(z, idx, lg, y, ignore_index, float(temperature), reduction == "mean")
+        return rows.view(logits.shape[:-1]) if reduction == "none" else loss
+    rows, valid = ref.distillation_rows(z, idx, lg, float(temperature), y, ignore_index)
+    return ref.reduce_rows(rows.view(logits.shape[:-1]), valid, reduction)
+
+
+class _LinearDistillFn(torch.autograd.Function):
+    """``_LinearCEFn`` with a teacher's distribution in the place of the label: the log-sum-exp of the logits over the temperature
+    from the product's epilogue, the teacher's words as gathered dot products; d(logits) chunk by chunk, the softmax's part from
+    the product's epilogue and the teacher's words over it."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, idx, lg, labels, ignore_index, tau, mean):
+        L = _ext.lib()
+        M, K = hidden.shape
+        V = weight.shape[0]
+        dev = hidden.device
+        f32 = dict(dtype=torch.float32, device=dev)
+        n_splits = L.cb_cce_num_splits(M, V)
+        part = torch.empty(2, n_splits, M, **f32)
+        code = L.cb_cce_forward_t(hidden.data_ptr(), weight.data_ptr(), None, M, V, K, hidden.stride(0), weight.stride(0), 0,
+                                  math.log2(math.e) / tau, part[0].data_ptr(), part[1].data_ptr(), None, None,
+                                  _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr())
+        _ext.check(code, "cce_forward_t")
+        lse, loss_rows, gscale = torch.empty(3, M, **f32)
+        stats, coef, out = torch.empty(M, 2, **f32), torch.empty(M, idx.shape[1], **f32), torch.empty(2, **f32)
+        code = L.cb_kd_linear_rows(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), K, V, M,
+                                   part[0].data_ptr(), part[1].data_ptr(), n_splits, *_teacher_ptrs(idx, lg), _ext.ptr(labels),
+                                   ignore_index, tau, int(mean), lse.data_ptr(), stats.data_ptr(), coef.data_ptr(),
+                                   loss_rows.data_ptr(), out.data_ptr(), gscale.data_ptr(), _ext.stream_ptr())
+        _ext.check(code, "kd_linear_rows")
+        ctx.save_for_backward(hidden, weight, idx, lg, lse, coef, gscale, stats)
+        ctx.tau = tau
+        ctx.set_materialize_grads(False)
+        return out[0], loss_rows
+
+    @staticmethod
+    def backward(ctx, gout, grows):
+        hidden, weight, idx, lg, lse, coef, gscale, stats = ctx.saved_tensors
+        L = _ext.lib()
+        M, K = hidden.shape
+        V = weight.shape[0]
+        dev = hidden.device
+        status = _ext.status_buffer(dev)
+        if grows is None and gout is not None:
+            g1 = gout.float().reshape(1).contiguous()
+        else:                                          # gradient arriving through the rows' losses
+            scale = gscale * gout.float() if gout is not None else torch.zeros_like(gscale)
+            if grows is not None:
+                scale = scale + grows.float() * ctx.tau * (stats[:, 1] != -1.0)
+            gscale = scale.contiguous()
+            g1 = torch.ones(1, dtype=torch.float32, device=dev)
+        need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        Vc = _cce_chunk(M, K, V, _sm_count(dev))
+        G = torch.empty(M, Vc, dtype=torch.bfloat16, device=dev)
+        # sums over several chunks stay in fp32; one chunk is rounded where it is computed
+        dh = torch.empty(M, K, dtype=torch.float32 if Vc < V else hidden.dtype, device=dev) if need_dh else None
+        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_dw else None
+        for c0 in range(0, V, Vc):
+            vc = min(Vc, V - c0)
+            wc = weight[c0:c0 + vc]
+            code = L.cb_cce_dlogits_t(hidden.data_ptr(), wc.data_ptr(), None, lse.data_ptr(), gscale.data_ptr(), g1.data_ptr(),
+                                      G.data_ptr(), M, vc, K, hidden.stride(0), weight.stride(0), G.stride(0), c0, V, 0.0, 0.0,
+                                      math.log2(math.e) / ctx.tau, status.data_ptr(), _ext.stream_ptr())
+            _ext.check(code, "cce_dlogits_t")
+            code = L.cb_kd_place(G.data_ptr(), G.stride(0), c0, vc, V, M, *_teacher_ptrs(idx, lg), ctx.tau, coef.data_ptr(),
+                                 gscale.data_ptr(), g1.data_ptr(), _ext.stream_ptr())
+            _ext.check(code, "kd_place")
+            Gc = G[:, :vc]
+            if need_dh:   # dH += G_c @ W_c
+                gemm(Gc, wc, b_mn=True, out=dh, accumulate=c0 > 0)
+            if need_dw:   # dW_c = G_c^T @ H
+                gemm(Gc, hidden, a_mn=True, b_mn=True, out=dw[c0:c0 + vc])
+        return dh.to(hidden.dtype) if need_dh else None, dw, None, None, None, None, None, None
+
+
+def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor,
+                        temperature: float = 1.0, labels: Optional[torch.Tensor] = None, ignore_index: int = -100,
+                        reduction: str = "mean") -> torch.Tensor:
+    """:func:`distillation_logits` of ``hidden @ weight.T`` without ever holding the ``[tokens, vocab]`` logits, as
+    :func:`linear_cross_entropy` is :func:`cross_entropy_logits`.  bf16 on CUDA runs on the kernels; the hidden states of rows that
+    take no part have to be finite."""
+    lead = hidden.shape[:-1]
+    if weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
+        raise ValueError(f"linear_distillation: weight {tuple(weight.shape)} does not fit hidden states {tuple(hidden.shape)}")
+    idx, lg, y = _distill_args("linear_distillation", lead, weight.shape[0], teacher_indices, teacher_logits, temperature, labels,
+                               reduction, hidden, weight)
+    h = hidden.reshape(-1, hidden.shape[-1])
+    if (_fast(h, weight) and h.shape[1] % 8 == 0 and h.shape[0] and _gemm_ok(weight)
+            and weight.stride(0) >= weight.shape[1] and h.shape[1] * 2 + idx.shape[1] * 12 <= 200 * 1024
+            and idx.shape[1] <= _ext.lib().cb_kd_max_entries()):
+        if not _gemm_ok(h) or h.stride(0) < h.shape[1]:
+            h = h.clone(memory_format=torch.contiguous_format)
+        lg = lg.float() if lg.dtype == torch.float64 else lg
+        loss, rows = _LinearDistillFn.apply(h, weight, idx, lg, y, ignore_index, float(temperature), reduction == "mean")
+        return rows.view(lead) if reduction == "none" else loss
+    wide = torch.float64 if h.dtype == torch.float64 else torch.float32
+    rows, valid = ref.distillation_rows(h.to(wide) @ weight.to(wide).t(), idx, lg, float(temperature), y, ignore_index)
+    return ref.reduce_rows(rows.view(lead), valid, reduction)

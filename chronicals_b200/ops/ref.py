@@ -142,6 +142,25 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, position_i
     return out.to(x.dtype)
 
 
+def rope_axis_map(sections: Sequence[int], cyclic: bool = False) -> Tuple[int, ...]:
+    """The axis of every frequency of a head: ``sections[i]`` frequencies for axis ``i``, one axis's behind the other's, or
+    (``cyclic``) dealt to the axes in turn, where what an axis with no frequencies left would get goes to axis 0."""
+    n = len(sections)
+    if not cyclic:
+        return tuple(a for a, k in enumerate(sections) for _ in range(k))
+    return tuple(f % n if f // n < sections[f % n] else 0 for f in range(sum(sections)))
+
+
+def rope_axes_tables(cos: torch.Tensor, sin: torch.Tensor, position_ids: torch.Tensor, axis_map: Sequence[int]
+                     ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``cos, sin`` rows ``[T, D/2]`` of tokens with one position per axis (``position_ids [axes, T]``); positions outside the
+    tables use their first or last row."""
+    ax = torch.as_tensor(axis_map, device=position_ids.device)
+    rows = position_ids.long().clamp(0, cos.shape[0] - 1)[ax].t()
+    f = torch.arange(ax.numel(), device=rows.device)
+    return cos[rows, f], sin[rows, f]
+
+
 # --------------------------------------------------------------------------- attention
 def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      max_seqlen: Optional[int] = None, causal: bool = True,
@@ -305,6 +324,34 @@ def cross_entropy_logits(logits: torch.Tensor, labels: torch.Tensor, ignore_inde
     if reduction == "sum":
         return loss.sum()
     return loss.sum() / (y != ignore_index).sum().clamp_min(1)
+
+
+# --------------------------------------------------------------------------- distillation
+def distillation_rows(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor, temperature: float = 1.0,
+                      labels: Optional[torch.Tensor] = None, ignore_index: int = -100) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(loss of every row, rows that take part)`` of ``logits [rows, V]`` against a teacher's top logits ``[rows, K]``:
+    ``temperature**2 * KL(softmax(teacher / temperature) || softmax(logits / temperature))``, the teacher's distribution over the
+    row's entries (those of one index add up), the student's over the vocabulary.  An entry whose index is outside the vocabulary or
+    whose logit is -inf is absent; a row without an entry, or with the ignored label, takes no part."""
+    z = (logits if logits.dtype == torch.float64 else logits.float()) / temperature
+    t = teacher_logits.detach().to(z.dtype) / temperature
+    on = (teacher_indices >= 0) & (teacher_indices < z.shape[1]) & (t != -math.inf)
+    valid = on.any(1)
+    if labels is not None:
+        valid = valid & (labels != ignore_index)
+    q = torch.softmax(torch.where(valid[:, None], torch.where(on, t, -math.inf), 0.0), 1)
+    at = torch.where(on, teacher_indices, 0).long()
+    word = torch.zeros_like(z, requires_grad=False).scatter_add_(1, at, torch.where(on, q, 0.0)).gather(1, at)
+    logp = z.gather(1, at) - torch.logsumexp(z, 1, keepdim=True)
+    part = valid[:, None] & on & (q != 0)
+    terms = torch.where(part, q * (torch.where(part, word, 1.0).log() - torch.where(part, logp, 0.0)), 0.0)
+    return temperature * temperature * terms.sum(1), valid
+
+
+def reduce_rows(rows: torch.Tensor, valid: torch.Tensor, reduction: str) -> torch.Tensor:
+    if reduction == "none":
+        return rows
+    return rows.sum() if reduction == "sum" else rows.sum() / valid.sum().clamp_min(1)
 
 
 # --------------------------------------------------------------------------- optimizer math
