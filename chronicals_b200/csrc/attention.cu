@@ -52,6 +52,9 @@ struct AttnArgs {
   float* dv_part;
   int* status;
   int o_tma;            // forward: a tensor map over O exists, whole blocks may leave by TMA store
+  // windowed forms: a query sees the last `window` keys of its document, its own among them, and the document's first `sinks`
+  int window, sinks;
+  int sink_run;         // backward: query blocks per CTA of a key block that holds sinks
 };
 
 // Phase timers (compiled in with -DCB_ATTN_PHASE_TIMERS only): two threads of every CTA - the MMA-issuing thread
@@ -124,6 +127,65 @@ __device__ __forceinline__ void zero_padding_rows(const AttnArgs& a, int beyond,
     const long long t = row0 + i / CH;
     if (t < a.T) reinterpret_cast<uint4*>(a.O + t * a.ldo + static_cast<long long>(h) * D)[i % CH] = make_uint4(0u, 0u, 0u, 0u);
   }
+}
+
+// The tile of a windowed kernel: CTA b's, document by document, the weights being all but equal (a window's worth of blocks).
+// Forward, one tile per query block, the last block of a document first.  Backward, one per key block; a key block that holds sinks
+// is seen by every later query of its document, and its query blocks are shared out over CTAs in runs of a.sink_run, which come
+// first in their document.  blk: the block of the tile, run: of which run (-1: a key block without sinks).
+template <bool BWD>
+__device__ __forceinline__ bool locate_window_tile(const AttnArgs& a, int b, int& start, int& len, int& nblk, int& blk, int& run,
+                                                   int* beyond = nullptr) {
+  const int lane = threadIdx.x & 31;
+  const int with_sinks = BWD ? (a.sinks + 127) >> 7 : 0;
+  for (int d0 = 0; d0 < a.n_docs; d0 += 32) {
+    const int d = d0 + lane;
+    int st = 0, ln = 0;
+    if (d < a.n_docs) {
+      st = a.cu[d];
+      ln = a.cu[d + 1] - st;
+    }
+    const int nb = (ln + 127) >> 7, ns = min(nb, with_sinks);
+    const int runs = BWD ? (nb + a.sink_run - 1) / a.sink_run : 0;
+    const int mine = nb - ns + ns * runs;
+    int upto = mine;                                   // tiles of the documents up to mine
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned m = __ballot_sync(0xffffffffu, b < upto);
+    if (m != 0) {
+      const int src = __ffs(m) - 1;
+      const int at = b - __shfl_sync(0xffffffffu, upto - mine, src);
+      start = __shfl_sync(0xffffffffu, st, src);
+      len = __shfl_sync(0xffffffffu, ln, src);
+      nblk = __shfl_sync(0xffffffffu, nb, src);
+      const int n_s = __shfl_sync(0xffffffffu, ns, src), n_r = __shfl_sync(0xffffffffu, runs, src);
+      if (!BWD) {
+        blk = nblk - 1 - at;
+        run = -1;
+      } else if (at < n_s * n_r) {
+        blk = at % n_s;
+        run = at / n_s;
+      } else {
+        blk = at - n_s * n_r + n_s;
+        run = -1;
+      }
+      return true;
+    }
+    b -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (beyond != nullptr) *beyond = b;                  // index among the CTAs past the last tile
+  return false;
+}
+
+// The query blocks [first, first + count) that key block `jb` of a document of nblk blocks meets, or those of its run
+__device__ __forceinline__ void window_query_blocks(const AttnArgs& a, int jb, int run, int nblk, int& first, int& count) {
+  const int lo = run < 0 ? jb : max(jb, run * a.sink_run);
+  const int hi = run < 0 ? min(nblk, ((jb * 128 + 127 + a.window - 1) >> 7) + 1) : min(nblk, (run + 1) * a.sink_run);
+  first = lo;
+  count = hi - lo;
 }
 
 // store 32 consecutive values of thread-row r as bf16 into a [128 x 128] operand image made of two
@@ -697,7 +759,7 @@ struct Fwd3Smem {
   static constexpr int TOTAL = OFF_BAR + 256 + 1024;
 };
 
-template <int D>
+template <int D, bool WIN>
 __global__ void __launch_bounds__(FWD3_THREADS, 2)
 attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const AttnArgs a) {
@@ -716,14 +778,25 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   int start, len, qb, nblk;
   int beyond = 0;
-  if (!locate_tile(a.cu, a.n_docs, blockIdx.y, start, len, qb, nblk, &beyond)) {
+  int run = 0;
+  if (!(WIN ? locate_window_tile<false>(a, blockIdx.y, start, len, nblk, qb, run, &beyond)
+            : locate_tile(a.cu, a.n_docs, blockIdx.y, start, len, qb, nblk, &beyond))) {
     zero_padding_rows<D>(a, beyond, blockIdx.x);
     return;
   }
-  qb -= 1;
+  if (!WIN) qb -= 1;                                   // weight = kv blocks up to the diagonal = qb + 1
   const int h = blockIdx.x;
   const int hkv = h / (a.hq / a.hk);
-  const int n_kv = min(2 * qb + 2, (len + 63) >> 6);   // 64-row kv blocks up to and including the diagonal
+  int n_kv = min(2 * qb + 2, (len + 63) >> 6);         // 64-row kv blocks up to and including the diagonal
+  // windowed: the blocks of the sinks, then those from the first row's first key on; `skip` blocks between them are left out
+  int n_snk = 0, skip = 0;
+  if (WIN) {
+    const int lo = max(0, qb * 128 - a.window + 1) >> 6;
+    n_snk = min((a.sinks + 63) >> 6, lo);
+    skip = lo - n_snk;
+    n_kv -= skip;
+  }
+  const auto block_of = [&](int j, int s_, int k_) { return WIN && j >= s_ ? j + k_ : j; };
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -771,13 +844,14 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int u_start = __shfl_sync(0xffffffffu, start, 0);
     const int u_qb = __shfl_sync(0xffffffffu, qb, 0);
     const int u_nkv = __shfl_sync(0xffffffffu, n_kv, 0);
+    const int u_snk = __shfl_sync(0xffffffffu, n_snk, 0), u_skip = __shfl_sync(0xffffffffu, skip, 0);
     if (elect_one()) {
       mbar_expect_tx(bar_q, L::QT);
 #pragma unroll
       for (int p = 0; p < PANELS; ++p) tma_load_2d(sQ + p * 16384, &tmQ, bar_q, h * D + p * 64, u_start + u_qb * 128);
     }
     for (int j = 0; j < u_nkv && ok; ++j) {
-      const int st = j % NS;
+      const int st = j % NS, kv_row = u_start + block_of(j, u_snk, u_skip) * 64;
       if (j >= NS) {                                    // the stage's previous block: S(j - NS) complete
         ok = __all_sync(0xffffffffu, mbar_wait(k_empty + st, ((j / NS) - 1) & 1, abort_flag, a.status, CB_ERR_WAIT_EMPTY) && ok);
         if (!ok) break;
@@ -786,7 +860,7 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         mbar_expect_tx(k_full + st, L::KT);
 #pragma unroll
         for (int p = 0; p < PANELS; ++p)
-          tma_load_2d(sK + st * L::KT + p * 8192, &tmK, k_full + st, hkv * D + p * 64, u_start + j * 64);
+          tma_load_2d(sK + st * L::KT + p * 8192, &tmK, k_full + st, hkv * D + p * 64, kv_row);
       }
       if (j >= NS) {                                    // P V of block j - NS complete
         ok = __all_sync(0xffffffffu, mbar_wait(v_empty + st, ((j / NS) - 1) & 1, abort_flag, a.status, CB_ERR_WAIT_EMPTY) && ok);
@@ -796,7 +870,7 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         mbar_expect_tx(v_full + st, L::KT);
 #pragma unroll
         for (int p = 0; p < PANELS; ++p)
-          tma_load_2d(sV + st * L::KT + p * 8192, &tmV, v_full + st, hkv * D + p * 64, u_start + j * 64);
+          tma_load_2d(sV + st * L::KT + p * 8192, &tmV, v_full + st, hkv * D + p * 64, kv_row);
       }
     }
     __syncwarp();
@@ -884,8 +958,17 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       CB_PHASE(2);
       // columns j*64 + c <= qb*128 + r are visible; only the blocks that touch the diagonal need the test
-      const int lim = qb * 128 + r - j * 64;
-      if (j >= 2 * qb) {
+      const int kb = block_of(j, n_snk, skip);
+      const int lim = qb * 128 + r - kb * 64;
+      if (WIN && kb * 64 + a.window <= qb * 128 + 127) {   // some row's window begins after the block's first key
+        const int lo = lim - a.window + 1, snk = a.sinks - kb * 64;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          if (c < lo && c >= snk) s0[c] = 0xff800000u;
+          if (c + 32 < lo && c + 32 >= snk) s1[c] = 0xff800000u;
+        }
+      }
+      if (kb >= 2 * qb) {
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
           if (c > lim) s0[c] = 0xff800000u;             // -inf
@@ -933,7 +1016,8 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (up) m_ref = mx;
       }
       CB_PHASE(4);
-      const float mb = m_ref * sl2;
+      // a row of a windowed tile may have seen no key yet: its scores are all -inf and stand for zeros against any reference
+      const float mb = WIN && m_ref == -INFINITY ? 0.f : m_ref * sl2;
       uint32_t pk[32];
       float rs0 = 0.f, rs1 = 0.f;
 #pragma unroll
@@ -1081,7 +1165,7 @@ __device__ __forceinline__ void load_row_chunk32(const uint8_t* base, int r, int
   }
 }
 
-template <int D>
+template <int D, bool WIN>
 __global__ void __launch_bounds__(BWD2_THREADS, 2)
 attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -1096,8 +1180,17 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   constexpr uint32_t IDESC_DQ = umma_idesc_bf16(128, D, 0, 1);           // dS K
 
   int start, len, jb, nblk;
-  if (!locate_tile(a.cu, a.n_docs, blockIdx.y, start, len, jb, nblk)) return;
-  jb = nblk - jb;                                      // weight = query blocks from the diagonal on = nblk - jb
+  int ib, n_it;                                        // the first query block and how many
+  if (WIN) {
+    int run;
+    if (!locate_window_tile<true>(a, blockIdx.y, start, len, nblk, jb, run)) return;
+    window_query_blocks(a, jb, run, nblk, ib, n_it);
+    if (n_it <= 0) return;                             // a run that ends before the key block begins
+  } else {
+    if (!locate_tile(a.cu, a.n_docs, blockIdx.y, start, len, jb, nblk)) return;
+    ib = jb = nblk - jb;                               // weight = query blocks from the diagonal on = nblk - jb
+    n_it = nblk - jb;
+  }
   const int h = blockIdx.x;
   const int hkv = h / (a.hq / a.hk);
 
@@ -1136,16 +1229,15 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const uint32_t tmem = *tmem_slot;
   const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
 
-  const int n_it = nblk - jb;
   // Warp 0 issues every TMA load and MMA: the whole warp follows the issuing path with warp-uniform control flow
   // and one elected lane issues, with the values that feed coordinates and descriptors broadcast from lane 0, so
   // that the compiler can keep them in uniform registers.
   const bool w0 = __shfl_sync(0xffffffffu, warp, 0) == 0;
   const int u_start = __shfl_sync(0xffffffffu, start, 0);
-  const int u_jb = __shfl_sync(0xffffffffu, jb, 0);
+  const int u_jb = __shfl_sync(0xffffffffu, jb, 0), u_ib = __shfl_sync(0xffffffffu, ib, 0);
   const int kv_row0 = u_start + u_jb * 128;
-  auto load_q = [&](int it) {                          // Q / dO of query block jb + it
-    const int row0 = u_start + (u_jb + it) * 128;
+  auto load_q = [&](int it) {                          // Q / dO of query block ib + it
+    const int row0 = u_start + (u_ib + it) * 128;
     mbar_expect_tx(q_full, 2 * L::TILE);
 #pragma unroll
     for (int p = 0; p < PANELS; ++p) {
@@ -1175,7 +1267,7 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   // lse and delta of my query row: fetched one iteration ahead, the loads fly while this iteration works
   // (the loaded values are not touched before the next iteration, so nothing waits for the loads here)
   auto row_stats = [&](int it, float& lse_o, float& dlt_o) {
-    const int rg_ = (jb + it) * 128 + r;
+    const int rg_ = (ib + it) * 128 + r;
     const long long at = static_cast<long long>(h) * a.T + start + rg_;
     lse_o = 0.f;
     dlt_o = 0.f;
@@ -1189,7 +1281,7 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   CB_PHASE_DECL;
   for (int it = 0; it < n_it; ++it) {
-    const int i = jb + it;
+    const int i = ib + it;
     CB_PHASE(0);
     if (w0) {
       ok = __all_sync(0xffffffffu, mbar_wait(q_full, it & 1, abort_flag, a.status, CB_ERR_WAIT_FULL) && ok);
@@ -1211,7 +1303,9 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const bool row_ok = rg < len;
     const float lse2 = row_ok ? lse_n * LOG2E : INFINITY, dlt = dlt_n;
     row_stats(it + 1, lse_n, dlt_n);
-    const bool diag = (it == 0);
+    const bool diag = WIN ? i == jb : it == 0;
+    const bool edge = WIN && (i - jb) * 128 + 127 >= a.window;         // some query's window begins after the block's first key
+    const int lo = rg - a.window + 1 - jb * 128, snk = a.sinks - jb * 128;
     CB_PHASE(1);
     // ---- phase 1: P = exp(S - lse), masked, to shared memory
     ok &= mbar_wait(bar_s, it & 1, abort_flag, a.status, CB_ERR_WAIT_TMEM_FULL);
@@ -1227,6 +1321,11 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       uint32_t s[32];
       tmem_ld_32x32(t_row + C_S + c * 32, s);
       tmem_ld_wait();
+      if (WIN && edge) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (c * 32 + k < lo && c * 32 + k >= snk) s[k] = 0xff800000u;                  // -inf
+      }
       if (diag) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -1334,7 +1433,7 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
           tma_reduce_add_2d(&tmdQ, sP + c * 16384, h * D + c * 32,
-                            u_start + (u_jb + it) * 128);
+                            u_start + (u_ib + it) * 128);
         tma_store_commit();
       }
     }
@@ -1428,7 +1527,7 @@ __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <int D>
+template <int D, bool WIN>
 __global__ void __launch_bounds__(BWD3_THREADS, 1)
 attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
@@ -1445,8 +1544,17 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   constexpr uint32_t IDESC_DQ = umma_idesc_bf16(128, D, 1, 1);           // dS K
 
   int start, len, jb, nblk;
-  if (!locate_tile(a.cu, a.n_docs, blockIdx.y, start, len, jb, nblk)) return;
-  jb = nblk - jb;                                      // weight = query blocks from the diagonal on = nblk - jb
+  int ib, n_it;                                        // the first query block and how many
+  if (WIN) {
+    int run;
+    if (!locate_window_tile<true>(a, blockIdx.y, start, len, nblk, jb, run)) return;
+    window_query_blocks(a, jb, run, nblk, ib, n_it);
+    if (n_it <= 0) return;                             // a run that ends before the key block begins
+  } else {
+    if (!locate_tile(a.cu, a.n_docs, blockIdx.y, start, len, jb, nblk)) return;
+    ib = jb = nblk - jb;                               // weight = query blocks from the diagonal on = nblk - jb
+    n_it = nblk - jb;
+  }
   const int h = blockIdx.x;
   const int hkv = h / (a.hq / a.hk);
 
@@ -1496,7 +1604,6 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int n_it = nblk - jb;
   const int lane = tid & 31;
   bool ok = true;
   // one arrival for a warp: what its lanes did before is ordered by the warp barrier
@@ -1516,13 +1623,13 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (warp == 13) {
       // ------------------------------------------------------------------ loads
       const int u_start = __shfl_sync(0xffffffffu, start, 0);
-      const int u_jb = __shfl_sync(0xffffffffu, jb, 0);
+      const int u_jb = __shfl_sync(0xffffffffu, jb, 0), u_ib = __shfl_sync(0xffffffffu, ib, 0);
       const int u_n = __shfl_sync(0xffffffffu, n_it, 0);
       float lse_n[4], dlt_n[4];                          // statistics of the next block: the loads fly an iteration ahead
       auto fetch_stats = [&](int it) {
   #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int rg = (u_jb + it) * 128 + lane + 32 * k;
+          const int rg = (u_ib + it) * 128 + lane + 32 * k;
           const long long at = static_cast<long long>(h) * a.T + u_start + rg;
           const bool in = it < u_n && rg < len;
           lse_n[k] = in ? __ldg(a.lse + at) : 0.f;
@@ -1537,7 +1644,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       for (int it = 0; it < u_n; ++it) {
         const int st = it & 1;
-        const int row0 = u_start + (u_jb + it) * 128;
+        const int row0 = u_start + (u_ib + it) * 128;
         if (it >= 2 && !wait_w(q_empty + st, (it >> 1) - 1, CB_ERR_WAIT_EMPTY)) break;
         if (elect_one()) {
           mbar_expect_tx(q_full + st, L::TILE);
@@ -1546,13 +1653,13 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (it == 0) {
             mbar_expect_tx(v_full, L::TILE);
   #pragma unroll
-            for (int p = 0; p < PANELS; ++p) tma_load_2d(sV + p * 16384, &tmV, v_full, hkv * D + p * 64, row0);
+            for (int p = 0; p < PANELS; ++p) tma_load_2d(sV + p * 16384, &tmV, v_full, hkv * D + p * 64, u_start + u_jb * 128);
           }
         }
         // rows past the end of the document get lse = +inf: finite scores give probabilities of exactly zero
   #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const bool in = (u_jb + it) * 128 + lane + 32 * k < len;
+          const bool in = (u_ib + it) * 128 + lane + 32 * k < len;
           sStat[st * 256 + lane + 32 * k] = in ? lse_n[k] * LOG2E : INFINITY;
           sStat[st * 256 + 128 + lane + 32 * k] = dlt_n[k];
         }
@@ -1656,7 +1763,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       tmem_ld_wait();
       tc_fence_before();
       arrive_w(dq_free);
-      if ((jb + it) * 128 + q4 * 32 + lane >= len) {   // rows of the next document: nothing, whatever either holds
+      if ((ib + it) * 128 + q4 * 32 + lane >= len) {   // rows of the next document: nothing, whatever either holds
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
 #pragma unroll
@@ -1674,9 +1781,9 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         fence_async_smem();
         __syncwarp();
         if (elect_one()) {
-          CB_DEBUG_CHECK_ST(a.status, start + (jb + it) * 128 >= 0, CB_DBG_TMA_COORD, start + (jb + it) * 128);
-          if ((jb + it) * 128 + q4 * 32 < len)
-            tma_reduce_add_2d(&tmdQ, box + (c & 1) * 4096, h * D + c * 32, start + (jb + it) * 128 + q4 * 32);
+          CB_DEBUG_CHECK_ST(a.status, start + (ib + it) * 128 >= 0, CB_DBG_TMA_COORD, start + (ib + it) * 128);
+          if ((ib + it) * 128 + q4 * 32 < len)
+            tma_reduce_add_2d(&tmdQ, box + (c & 1) * 4096, h * D + c * 32, start + (ib + it) * 128 + q4 * 32);
           tma_store_commit();
         }
       }
@@ -1706,7 +1813,15 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tmem_ld_32x32(t_s, s[0]);
         tmem_ld_32x32(t_s + 32, s[1]);
         tmem_ld_wait();
-        if (it == 0) {                                 // the diagonal block: queries before my key see nothing of it
+        if (WIN && (ib + it - jb) * 128 + 127 >= a.window && jb * 128 + r >= a.sinks) {
+          const int hi = (jb - ib - it) * 128 + r + a.window - half * 64;                // my key is behind these queries' windows
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            if (c >= hi) s[0][c] = 0xff800000u;                                          // -inf
+            if (c + 32 >= hi) s[1][c] = 0xff800000u;
+          }
+        }
+        if (WIN ? ib + it == jb : it == 0) {           // the diagonal block: queries before my key see nothing of it
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             if (half * 64 + c < r) s[0][c] = 0xff800000u;                // -inf
@@ -1908,12 +2023,12 @@ int cb_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse
     if (!a.o_tma) mo = mq;                              // O is not TMA-addressable: every block stores row by row
     if (D == 64) {
       static bool cfg = false;
-      if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<64>, cb::Fwd3Smem<64>::TOTAL); if (e) return e; cfg = true; }
-      cb::attn_fwd3_kernel<64><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<64>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
+      if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<64, false>, cb::Fwd3Smem<64>::TOTAL); if (e) return e; cfg = true; }
+      cb::attn_fwd3_kernel<64, false><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<64>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
     } else {
       static bool cfg = false;
-      if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<128>, cb::Fwd3Smem<128>::TOTAL); if (e) return e; cfg = true; }
-      cb::attn_fwd3_kernel<128><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<128>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
+      if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<128, false>, cb::Fwd3Smem<128>::TOTAL); if (e) return e; cfg = true; }
+      cb::attn_fwd3_kernel<128, false><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<128>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
     }
     return static_cast<int>(cudaGetLastError());
   }
@@ -1942,12 +2057,64 @@ int cb_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse
   return static_cast<int>(cudaGetLastError());
 }
 
-// Backward.  scratch: delta [hq*T] fp32, dq_acc [T*hq*D] fp32, dk_part / dv_part [T*hk*D] fp32 (all three
-// accumulators are zeroed here).  dqkv: bf16 [T, (hq + 2 hk) * D] with row pitch ld_dqkv receives dQ | dK | dV.
-int cb_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+// Forward over the last `window` (>= 1) keys and the first `sinks` (>= 0) of each document; the rest as cb_attn_fwd.
+int cb_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu, int n_docs, int T,
+                       int hq, int hk, int D, long long ldq, long long ldk, long long ldv, long long ldo, float scale, int window,
+                       int sinks, int* status, void* stream) {
+  if ((D != 64 && D != 128) || hk <= 0 || hq % hk != 0 || T <= 0 || n_docs <= 0 || window < 1 || sinks < 0) return -1;
+  CUtensorMap mq, mk64, mv64, mo;
+  int e = cbhost::make_tmap(&mq, q, static_cast<unsigned long long>(hq) * D, T, ldq, 64, 128);
+  if (!e) e = cbhost::make_tmap(&mk64, k, static_cast<unsigned long long>(hk) * D, T, ldk, 64, 64);
+  if (!e) e = cbhost::make_tmap(&mv64, v, static_cast<unsigned long long>(hk) * D, T, ldv, 64, 64);
+  if (e) return e;
+  cb::AttnArgs a = {};
+  a.T = T; a.hq = hq; a.hk = hk; a.n_docs = n_docs; a.cu = cu; a.scale = scale;
+  a.O = static_cast<cb::bf16*>(o); a.ldo = ldo; a.lse = lse; a.status = status;
+  a.window = std::min(window, T); a.sinks = std::min(sinks, T);
+  a.o_tma = cbhost::make_tmap(&mo, o, static_cast<unsigned long long>(hq) * D, T, ldo, 64, 128) == 0 ? 1 : 0;
+  if (!a.o_tma) mo = mq;
+  const long long tiles = (T + 127LL) / 128 + n_docs;
+  if (tiles > 65535) return -1;
+  const dim3 grid(hq, static_cast<unsigned>(tiles));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (D == 64) {
+    static bool cfg = false;
+    if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<64, true>, cb::Fwd3Smem<64>::TOTAL); if (e) return e; cfg = true; }
+    cb::attn_fwd3_kernel<64, true><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<64>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
+  } else {
+    static bool cfg = false;
+    if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<128, true>, cb::Fwd3Smem<128>::TOTAL); if (e) return e; cfg = true; }
+    cb::attn_fwd3_kernel<128, true><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<128>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
+  }
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // extern "C"
+
+namespace {
+
+template <int D, bool WIN>
+int launch_bwd2(dim3 grid, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo,
+                const CUtensorMap& mdq, const cb::AttnArgs& a) {
+  static bool cfg = false;
+  if (!cfg) { const int e = set_smem(cb::attn_bwd2_kernel<D, WIN>, cb::Bwd2Smem<D>::TOTAL); if (e) return e; cfg = true; }
+  cb::attn_bwd2_kernel<D, WIN><<<grid, cb::BWD2_THREADS, cb::Bwd2Smem<D>::TOTAL, s>>>(mq, mk, mv, mdo, mdq, a);
+  return 0;
+}
+template <int D, bool WIN>
+int launch_bwd3(dim3 grid, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo,
+                const CUtensorMap& mdq, const CUtensorMap& mdk, const CUtensorMap& mdv, const cb::AttnArgs& a) {
+  static bool cfg = false;
+  if (!cfg) { const int e = set_smem(cb::attn_bwd3_kernel<D, WIN>, cb::Bwd3Smem<D>::TOTAL); if (e) return e; cfg = true; }
+  cb::attn_bwd3_kernel<D, WIN><<<grid, cb::BWD3_THREADS, cb::Bwd3Smem<D>::TOTAL, s>>>(mq, mk, mv, mdo, mdq, mdk, mdv, a);
+  return 0;
+}
+
+// Both backward entry points; window = 0: none.
+int attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
                 const int* cu, int n_docs, int T, int hq, int hk, int D, long long ldq, long long ldk, long long ldv,
                 long long ldo, long long ld_do, float scale, float* delta, float* dq_acc, float* dk_part,
-                float* dv_part, void* dqkv, long long ld_dqkv, int* status, void* stream, int scratch_is_zero) {
+                float* dv_part, void* dqkv, long long ld_dqkv, int* status, void* stream, int scratch_is_zero, int window, int sinks) {
   if ((D != 64 && D != 128) || hq % hk != 0 || T <= 0 || n_docs <= 0) return -1;
   if ((reinterpret_cast<uintptr_t>(dqkv) & 7) != 0 || ld_dqkv % 4 != 0) return -1;       // the gradient is written 8 bytes at a time
   const bool wide = (reinterpret_cast<uintptr_t>(dqkv) & 15) == 0 && ld_dqkv % 8 == 0;   // or 16
@@ -1991,15 +2158,25 @@ int cb_attn_bwd(const void* q, const void* k, const void* v, const void* o, cons
   a.lse = const_cast<float*>(lse); a.delta = delta; a.dq_acc = dq_acc; a.dk_part = dk_part; a.dv_part = dv_part;
   a.status = status;
   dim3 grid(hq, (T + 127) / 128 + n_docs);            // x: query head (fastest, the heads of a group share K/V in L2); y: tile by descending weight
+  if (window > 0) {
+    a.window = std::min(window, T);
+    a.sinks = std::min(sinks, T);
+    // runs as long as the loop of a key block without sinks, and no shorter than 8: a CTA of less is mostly set-up
+    a.sink_run = std::max(8, (a.window + 127) / 128 + 1);
+    const long long tiles = (T + 127LL) / 128 + n_docs;
+    const long long all = tiles + (a.sinks + 127LL) / 128 * (tiles / a.sink_run + n_docs);
+    if (all > 65535) return -1;
+    grid.y = static_cast<unsigned>(all);
+  }
   // D = 64 runs two CTAs of the phase-by-phase kernel on an SM where one of the pipelined kernel fits, so the pipelined one
   // wins where the grid does not fill the SMs twice over (1 x 2048 tokens, 14 heads: 44 against 80 us; 4 x 512: 23 / 26)
   // or its loops are long (2 x 4096: 276 / 290; 4 x 2048, 32 heads: 403 / 350, so no earlier than 4096), unless the
   // documents are so short that a CTA is mostly set-up (20 x 100: 19 / 15).  Lengths as the average over the documents.
   const bool few = static_cast<long long>(hq) * ((T + 127) / 128) <= 2LL * cbhost::num_sms() && T >= 512LL * n_docs;
-  if (D == 64 && !few && T < 4096LL * n_docs) {
-    static bool cfg = false;
-    if (!cfg) { e = set_smem(cb::attn_bwd2_kernel<64>, cb::Bwd2Smem<64>::TOTAL); if (e) return e; cfg = true; }
-    cb::attn_bwd2_kernel<64><<<grid, cb::BWD2_THREADS, cb::Bwd2Smem<64>::TOTAL, s>>>(mq, mk, mv, mdo, mdq, a);
+  const bool short_loops = window > 0 ? std::min<long long>(2LL * window, T / n_docs) < 4096 : T < 4096LL * n_docs;
+  if (D == 64 && !few && short_loops) {
+    e = window > 0 ? launch_bwd2<64, true>(grid, s, mq, mk, mv, mdo, mdq, a) : launch_bwd2<64, false>(grid, s, mq, mk, mv, mdo, mdq, a);
+    if (e) return e;
   } else {
     CUtensorMap mdq32;                                  // the accumulator in boxes of 32 rows, one warp's share
     e = cbhost::make_tmap(&mdq32, dq_acc, static_cast<unsigned long long>(hq) * D, T, static_cast<unsigned long long>(hq) * D,
@@ -2010,21 +2187,43 @@ int cb_attn_bwd(const void* q, const void* k, const void* v, const void* o, cons
     if (e) return e;
     e = cbhost::make_tmap(&mdv, dv_part, static_cast<unsigned long long>(hk) * D, T, static_cast<unsigned long long>(hk) * D, 32, 32, 4);
     if (e) return e;
-    if (D == 64) {
-      static bool cfg = false;
-      if (!cfg) { e = set_smem(cb::attn_bwd3_kernel<64>, cb::Bwd3Smem<64>::TOTAL); if (e) return e; cfg = true; }
-      cb::attn_bwd3_kernel<64><<<grid, cb::BWD3_THREADS, cb::Bwd3Smem<64>::TOTAL, s>>>(mq, mk, mv, mdo, mdq32, mdk, mdv, a);
-    } else {
-      static bool cfg = false;
-      if (!cfg) { e = set_smem(cb::attn_bwd3_kernel<128>, cb::Bwd3Smem<128>::TOTAL); if (e) return e; cfg = true; }
-      cb::attn_bwd3_kernel<128><<<grid, cb::BWD3_THREADS, cb::Bwd3Smem<128>::TOTAL, s>>>(mq, mk, mv, mdo, mdq32, mdk, mdv, a);
-    }
+    if (D == 64)
+      e = window > 0 ? launch_bwd3<64, true>(grid, s, mq, mk, mv, mdo, mdq32, mdk, mdv, a)
+                     : launch_bwd3<64, false>(grid, s, mq, mk, mv, mdo, mdq32, mdk, mdv, a);
+    else
+      e = window > 0 ? launch_bwd3<128, true>(grid, s, mq, mk, mv, mdo, mdq32, mdk, mdv, a)
+                     : launch_bwd3<128, false>(grid, s, mq, mk, mv, mdo, mdq32, mdk, mdv, a);
+    if (e) return e;
   }
   const int vecs = (hq + 2 * hk) * D / 8;
   cb::attn_bwd_finalize_kernel<<<T, std::min(256, (vecs + cb::ATT_FIN_BATCH * 32 - 1) / (cb::ATT_FIN_BATCH * 32) * 32), 0, s>>>(
       dq_acc, dk_part, dv_part, static_cast<cb::bf16*>(dqkv), ld_dqkv, hq * D, hk * D, scale, cu, n_docs, scratch_is_zero ? 1 : 0,
       wide);
   return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace
+
+extern "C" {
+
+// Backward.  scratch: delta [hq*T] fp32, dq_acc [T*hq*D] fp32, dk_part / dv_part [T*hk*D] fp32 (all three
+// accumulators are zeroed here).  dqkv: bf16 [T, (hq + 2 hk) * D] with row pitch ld_dqkv receives dQ | dK | dV.
+int cb_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+                const int* cu, int n_docs, int T, int hq, int hk, int D, long long ldq, long long ldk, long long ldv,
+                long long ldo, long long ld_do, float scale, float* delta, float* dq_acc, float* dk_part,
+                float* dv_part, void* dqkv, long long ld_dqkv, int* status, void* stream, int scratch_is_zero) {
+  return attn_bwd(q, k, v, o, d_o, lse, cu, n_docs, T, hq, hk, D, ldq, ldk, ldv, ldo, ld_do, scale, delta, dq_acc, dk_part, dv_part,
+                  dqkv, ld_dqkv, status, stream, scratch_is_zero, 0, 0);
+}
+
+// The same for cb_attn_window_fwd, with its window and sinks; the accumulators are zeroed here.
+int cb_attn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+                       const int* cu, int n_docs, int T, int hq, int hk, int D, long long ldq, long long ldk, long long ldv,
+                       long long ldo, long long ld_do, float scale, int window, int sinks, float* delta, float* dq_acc, float* dk_part,
+                       float* dv_part, void* dqkv, long long ld_dqkv, int* status, void* stream) {
+  if (window < 1 || sinks < 0 || hk <= 0) return -1;
+  return attn_bwd(q, k, v, o, d_o, lse, cu, n_docs, T, hq, hk, D, ldq, ldk, ldv, ldo, ld_do, scale, delta, dq_acc, dk_part, dv_part,
+                  dqkv, ld_dqkv, status, stream, 0, window, sinks);
 }
 
 #ifdef CB_ATTN_PHASE_TIMERS

@@ -765,17 +765,39 @@ def embedding(ids: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
 # ============================================================================ attention
 def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      max_seqlen: Optional[int] = None, causal: bool = True,
-                     softmax_scale: Optional[float] = None, seqlens_host=None) -> torch.Tensor:
-    """Causal GQA attention over packed documents (``q [T,Hq,D]``, ``k/v [T,Hk,D]``)."""
+                     softmax_scale: Optional[float] = None, seqlens_host=None, window: Optional[int] = None,
+                     sinks: int = 0) -> torch.Tensor:
+    """Causal GQA attention over packed documents (``q [T,Hq,D]``, ``k/v [T,Hk,D]``).  With a ``window`` a query sees the last
+    ``window`` tokens of its document, its own among them, and the document's first ``sinks`` tokens."""
     from . import attention as _attn
-    return _attn.attention_varlen(q, k, v, cu_seqlens, max_seqlen, causal, softmax_scale, seqlens_host)
+    return _attn.attention_varlen(q, k, v, cu_seqlens, max_seqlen, causal, softmax_scale, seqlens_host, window, sinks)
 
 
 def attention_qkv_packed(qkv: torch.Tensor, cu_seqlens: torch.Tensor, num_q_heads: int, num_kv_heads: int,
-                         head_dim: int, max_seqlen: Optional[int] = None, seqlens_host=None) -> torch.Tensor:
+                         head_dim: int, max_seqlen: Optional[int] = None, seqlens_host=None, window: Optional[int] = None,
+                         sinks: int = 0) -> torch.Tensor:
     """Causal GQA attention reading Q, K, V straight out of the fused ``[T, (hq + 2 hk) * D]``
-    projection output; returns ``[T, hq * D]``."""
+    projection output; returns ``[T, hq * D]``.
+
+    With a ``window`` a query sees the last ``window`` tokens of its document, its own among them, and the document's first
+    ``sinks`` tokens; time and gradients then grow with the window instead of with the document.  Masked scores are dropped
+    whatever they hold, but a masked key's V row is multiplied by an exact zero, so V (and in the backward pass the output's
+    gradient) has to be finite."""
     from . import attention_cuda as _ac
+    if window is not None or sinks:
+        from .attention import window_band
+        band = window_band("attention_qkv_packed", window, sinks)
+        if num_kv_heads < 1 or num_q_heads % num_kv_heads or qkv.dim() != 2 or qkv.shape[1] != (num_q_heads + 2 * num_kv_heads) * head_dim:
+            raise ValueError(f"attention_qkv_packed: qkv {tuple(qkv.shape)} is not [T, (hq + 2 hk) * d] for hq, hk, d = "
+                             f"{num_q_heads}, {num_kv_heads}, {head_dim}")
+        _same_device("attention_qkv_packed", qkv, cu_seqlens)
+        if _ac.kernel_supports(qkv, head_dim) and qkv.shape[0] and cu_seqlens.numel() > 1:
+            if not _gemm_ok(qkv) or qkv.stride(0) < qkv.shape[1]:
+                qkv = qkv.clone(memory_format=torch.contiguous_format)
+            return _ac.attention_qkv_packed(qkv, cu_seqlens, num_q_heads, num_kv_heads, head_dim, None, band)
+        heads = (num_q_heads, num_kv_heads, num_kv_heads)
+        q, k, v = (t.reshape(qkv.shape[0], n, head_dim) for t, n in zip(qkv.split([n * head_dim for n in heads], dim=1), heads))
+        return ref.attention_window(q, k, v, cu_seqlens, *band, 1.0 / math.sqrt(head_dim)).reshape(qkv.shape[0], num_q_heads * head_dim)
     if qkv.dim() == 2 and _ac.kernel_supports(qkv, head_dim):
         return _ac.attention_qkv_packed(qkv, cu_seqlens, num_q_heads, num_kv_heads, head_dim)
     T = qkv.shape[0]

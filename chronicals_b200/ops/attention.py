@@ -47,11 +47,45 @@ def _sdpa_docs(q, k, v, bounds: Sequence[int], causal: bool, scale: float) -> to
     return out
 
 
+def window_band(op: str, window: Optional[int], sinks: int, causal: bool = True) -> tuple:
+    """``()`` without a window, else the checked ``(window, sinks)``."""
+    if isinstance(window, bool) or not (window is None or isinstance(window, int)) or isinstance(sinks, bool) or not isinstance(sinks, int):
+        raise ValueError(f"{op}: window {window!r} and sinks {sinks!r} must be whole numbers")
+    if sinks < 0:
+        raise ValueError(f"{op}: sinks {sinks} must not be negative")
+    if window is None:
+        if sinks:
+            raise ValueError(f"{op}: {sinks} sinks without a window: every earlier token is visible then")
+        return ()
+    if window < 1:
+        raise ValueError(f"{op}: window {window} must be at least 1, the token itself")
+    if not causal:
+        raise ValueError(f"{op}: a window needs causal attention")
+    return min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1)
+
+
+def _windowed(q, k, v, cu_seqlens, max_seqlen, scale, band):
+    T, hq, d = q.shape
+    if k.shape != v.shape or k.dim() != 3 or k.shape[0] != T or k.shape[2] != d or k.shape[1] == 0 or hq % k.shape[1]:
+        raise ValueError(f"attention_varlen: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"attention_varlen: softmax_scale {scale} must be positive and finite")
+    from . import _same_device
+    _same_device("attention_varlen", q, k, v, cu_seqlens)
+    from .attention_cuda import attention_varlen_cuda, kernel_supports
+    if T and cu_seqlens.numel() > 1 and all(kernel_supports(t, d) for t in (q, k, v)):
+        return attention_varlen_cuda(q, k, v, cu_seqlens, max_seqlen, scale, band)
+    return ref.attention_window(q, k, v, cu_seqlens, *band, scale)
+
+
 def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
                      max_seqlen: Optional[int] = None, causal: bool = True, softmax_scale: Optional[float] = None,
-                     seqlens_host: Optional[Sequence[int]] = None) -> torch.Tensor:
+                     seqlens_host: Optional[Sequence[int]] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     d = q.shape[-1]
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d)
+    band = window_band("attention_varlen", window, sinks, causal)
+    if band:
+        return _windowed(q, k, v, cu_seqlens, max_seqlen, scale, band)
     if q.is_cuda and not _ext.reference_forced() and q.dtype == torch.bfloat16 and _ext.available() and _ext.has_symbol("cb_attn_fwd") \
             and d in (64, 128) and causal:
         from .attention_cuda import attention_varlen_cuda

@@ -190,6 +190,28 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     return out
 
 
+def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, window: int, sinks: int,
+                     scale: float) -> torch.Tensor:
+    """:func:`attention_varlen` in which a query sees the last ``window`` tokens of its document, its own among them, and the
+    document's first ``sinks`` tokens.  A stretch of queries at a time, so that a long document never needs a square of scores."""
+    T, hq, d = q.shape
+    rep = hq // k.shape[1]
+    qf, kf, vf = ((t if t.dtype == torch.float64 else t.float()).transpose(0, 1) for t in (q, k, v))
+    out, bounds, stretch = [], cu_seqlens.tolist(), 512
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        for r0 in range(a, b, stretch):
+            r1 = min(b, r0 + stretch)
+            i = torch.arange(r0, r1, device=q.device)[:, None]
+            lo = max(a, r0 - window + 1)
+            j = torch.cat((torch.arange(a, max(a, min(a + sinks, lo)), device=q.device), torch.arange(lo, r1, device=q.device)))
+            see = (j <= i) & ((i - j < window) | (j < a + sinks))
+            ki, vi = (t[:, j].repeat_interleave(rep, dim=0) for t in (kf, vf))
+            s = (torch.matmul(qf[:, r0:r1], ki.transpose(-1, -2)) * scale).masked_fill(~see, float("-inf"))
+            out.append(torch.matmul(torch.softmax(s, dim=-1), vi).transpose(0, 1).to(q.dtype))
+    out.append(q.new_zeros(T - bounds[-1], hq, d))
+    return torch.cat(out)
+
+
 # --------------------------------------------------------------------------- cross-entropy
 def linear_cross_entropy_dense(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                                bias: Optional[torch.Tensor] = None, ignore_index: int = -100,
