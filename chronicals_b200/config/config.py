@@ -121,6 +121,14 @@ class ChronicalsConfig:
     rope_theta: float = 1e6
     attention_bias: bool = True
     rope_scaling: Optional[Dict[str, Any]] = None
+    # attention over the last `sliding_window` tokens of a document and its first `attention_sinks` (None: over all of them).
+    # Published configurations name windows that only some layers use: :meth:`from_hf_config` reads back what
+    # :meth:`to_hf_config` wrote, and takes no other key for it
+    sliding_window: Optional[int] = None
+    attention_sinks: int = 0
+    # frequencies of each axis where tokens have one position per axis (ops.qk_rope_axes_), dealt in turn if rope_cyclic
+    rope_sections: Optional[List[int]] = None
+    rope_cyclic: bool = False
     model_type: str = "qwen2"
     training_overrides: Dict[str, Any] = field(default_factory=dict)
 
@@ -195,13 +203,15 @@ class ChronicalsConfig:
                    tie_word_embeddings=bool(get("tie_word_embeddings", False)),
                    rope_theta=float(rope_theta),
                    attention_bias=bool(get("attention_bias", mt == "qwen2")),
-                   rope_scaling=get("rope_scaling"), model_type=mt)
+                   rope_scaling=get("rope_scaling"), model_type=mt, **(get("chronicals") or {}))
 
     def to_hf_config(self) -> Dict[str, Any]:
         """``config.json`` content in the layout transformers expects."""
         arch = {"qwen2": "Qwen2ForCausalLM", "llama": "LlamaForCausalLM",
                 "mistral": "MistralForCausalLM", "gemma": "GemmaForCausalLM"}.get(self.model_type, "Qwen2ForCausalLM")
+        own = {k: getattr(self, k) for k in ("sliding_window", "attention_sinks", "rope_sections", "rope_cyclic") if getattr(self, k)}
         return {
+            **({"chronicals": own} if own else {}),
             "architectures": [arch], "model_type": self.model_type,
             "hidden_size": self.hidden_size, "intermediate_size": self.intermediate_size,
             "num_hidden_layers": self.num_hidden_layers, "num_attention_heads": self.num_attention_heads,
@@ -330,6 +340,10 @@ class TrainingConfig:
     # loss
     label_smoothing: float = 0.0
     z_loss_weight: float = 1e-4
+    # batches that carry a teacher's top logits (teacher_indices, teacher_logits [B, S, K]):
+    # (1 - distill_weight) * cross-entropy + distill_weight * distillation loss
+    distill_weight: float = 0.5
+    distill_temperature: float = 1.0
     # logging / saving
     logging_steps: int = 10
     save_steps: int = 500

@@ -162,13 +162,31 @@ class Attention(nn.Module):
         self.o_proj = FusedLinear(self.hq * self.d, OrderedDict(o_proj=cfg.hidden_size), bias=False, dtype=dtype,
                                   device=device)
         self.interleaved_rope = False
+        self.window, self.sinks = cfg.sliding_window, cfg.attention_sinks
+        self.rope_sections, self.rope_cyclic = cfg.rope_sections, cfg.rope_cyclic
 
     def forward(self, x, residual, cos, sin, position_ids, cu_seqlens, max_seqlen, seqlens_host):
         T = x.shape[0]
         qkv = self.qkv_proj(x)
-        qkv = ops.qk_rope_(qkv, cos, sin, position_ids, self.hq, self.hk, self.d, self.interleaved_rope)
-        o = ops.attention_qkv_packed(qkv, cu_seqlens, self.hq, self.hk, self.d, max_seqlen, seqlens_host)
+        qkv = rotate(qkv, cos, sin, position_ids, self.hq, self.hk, self.d, self.interleaved_rope, self.rope_sections, self.rope_cyclic)
+        o = ops.attention_qkv_packed(qkv, cu_seqlens, self.hq, self.hk, self.d, max_seqlen, seqlens_host, self.window, self.sinks)
         return self.o_proj(o, residual)
+
+
+def rotate(qkv, cos, sin, pos, hq, hk, d, interleaved, sections, cyclic):
+    """Rotary positions of a packed QKV buffer: one position a token (``pos [T]``), or one per axis (``[axes, T]``)."""
+    if pos.dim() == 2:
+        return ops.qk_rope_axes_(qkv, cos, sin, pos, hq, hk, d, sections, cyclic=cyclic, interleaved=interleaved)
+    return ops.qk_rope_(qkv, cos, sin, pos, hq, hk, d, interleaved)
+
+
+def token_positions(position_ids: torch.Tensor, input_ids: torch.Tensor, sections) -> torch.Tensor:
+    """``[T]``, or ``[axes, T]`` where the positions have one leading dimension more than the tokens and the model has axes."""
+    if sections is not None and position_ids.dim() == input_ids.dim() + 1:
+        if position_ids.shape[0] != len(sections):
+            raise ValueError(f"position_ids {tuple(position_ids.shape)}: the model's rope_sections {tuple(sections)} have {len(sections)} axes")
+        return position_ids.reshape(len(sections), input_ids.numel())
+    return position_ids.reshape(input_ids.numel())
 
 
 def _is_one_product(m: nn.Module) -> bool:
@@ -250,6 +268,16 @@ class CausalLM(nn.Module):
     ``cu_seqlens``/``position_ids`` say otherwise) or already flat ``[T]`` ids.
     ``labels`` follow the HuggingFace convention (unshifted) when
     ``shift_labels=True``; pass ``shift_labels=False`` for pre-shifted labels.
+
+    With ``rope_sections`` in the configuration, ``position_ids`` may carry one
+    position per axis, ``[axes, B, S]`` (``[axes, T]`` for flat ids); documents
+    are then the rows, or what ``cu_seqlens`` says.
+
+    ``teacher_indices`` and ``teacher_logits [B, S, K]`` (a teacher's top logits
+    for the token that follows each position) add a distillation loss:
+    ``(1 - distill_weight) * cross-entropy + distill_weight * distillation``,
+    over the positions whose label is not ignored; without ``labels`` the loss is
+    the distillation's alone.
     """
 
     def __init__(self, cfg: ChronicalsConfig, dtype: Optional[torch.dtype] = None, device=None):
@@ -266,6 +294,8 @@ class CausalLM(nn.Module):
         self.register_buffer("rope_sin", torch.empty(0), persistent=False)
         self.label_smoothing = 0.0
         self.z_loss_weight = 0.0
+        self.distill_weight = 0.5
+        self.distill_temperature = 1.0
         self.reset_parameters()
 
     # -- init -----------------------------------------------------------------------------------------------
@@ -335,8 +365,11 @@ class CausalLM(nn.Module):
                 cu_seqlens: Optional[torch.Tensor] = None, max_seqlen: Optional[int] = None,
                 seqlens_host: Optional[Sequence[int]] = None, shift_labels: bool = True,
                 output_hidden_states: bool = False, return_logits: bool = False, return_dict: bool = True,
+                teacher_indices: Optional[torch.Tensor] = None, teacher_logits: Optional[torch.Tensor] = None,
                 **_) -> CausalLMOutput:
         dev = input_ids.device
+        if (teacher_indices is None) != (teacher_logits is None):
+            raise ValueError("teacher_indices and teacher_logits come together")
         if input_ids.dim() == 2:
             B, S = input_ids.shape
         else:
@@ -345,7 +378,7 @@ class CausalLM(nn.Module):
         ids = input_ids.reshape(T)
         derived = False
         if cu_seqlens is None:
-            if position_ids is not None and B == 1:
+            if position_ids is not None and B == 1 and token_positions(position_ids, input_ids, self.config.rope_sections).dim() == 1:
                 from ..data.sequence_packer import create_cu_seqlens_from_position_ids
                 cu_seqlens, max_seqlen = create_cu_seqlens_from_position_ids(position_ids.reshape(T))
             else:
@@ -356,7 +389,7 @@ class CausalLM(nn.Module):
                     seqlens_host = [S] * B
         if position_ids is None:
             position_ids = torch.arange(S, device=dev).repeat(B) if derived else _positions_from_cu(cu_seqlens, T)
-        pos = position_ids.reshape(T)
+        pos = token_positions(position_ids, input_ids, self.config.rope_sections)
         if max_seqlen is None:
             max_seqlen = S
         cos, sin = self._rope(max(int(max_seqlen), 1), dev)
@@ -371,12 +404,21 @@ class CausalLM(nn.Module):
         out = CausalLMOutput()
         if output_hidden_states:
             out.hidden_states = h.view(B, S, -1)
+        y = None
         if labels is not None:
             y = labels.reshape(B, S)
             if shift_labels:
                 y = torch.cat((y[:, 1:], torch.full((B, 1), -100, dtype=y.dtype, device=y.device)), dim=1)
-            out.loss = ops.linear_cross_entropy(h, self.output_weight, y.reshape(T), None, -100,
+            y = y.reshape(T)
+        share = 0.0 if teacher_indices is None else 1.0 if labels is None else float(self.distill_weight)
+        if labels is not None and share != 1.0:
+            out.loss = ops.linear_cross_entropy(h, self.output_weight, y, None, -100,
                                                 self.label_smoothing, self.z_loss_weight, "mean")
+        if teacher_indices is not None and share != 0.0:
+            K = teacher_indices.shape[-1]
+            kd = ops.linear_distillation(h, self.output_weight, teacher_indices.reshape(T, K), teacher_logits.reshape(T, K),
+                                         float(self.distill_temperature), y)
+            out.loss = kd if out.loss is None else (1.0 - share) * out.loss + share * kd
         if return_logits or (labels is None and not output_hidden_states):
             out.logits = torch.nn.functional.linear(h, self.output_weight).view(B, S, -1)
         return out

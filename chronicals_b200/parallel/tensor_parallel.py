@@ -34,6 +34,7 @@ import torch.distributed as dist
 import torch.nn as nn
 
 from .. import ops
+from ..models.decoder import rotate, token_positions
 from ..ops import _ext, ref
 
 
@@ -259,6 +260,8 @@ class TPDecoderLayer(nn.Module):
         self.input_norm_weight = nn.Parameter(full_layer.input_layernorm.weight.detach().clone())
         self.post_norm_weight = nn.Parameter(full_layer.post_attention_layernorm.weight.detach().clone())
         self.interleaved_rope = a.interleaved_rope
+        self.window, self.sinks = cfg.sliding_window, cfg.attention_sinks
+        self.rope_sections, self.rope_cyclic = cfg.rope_sections, cfg.rope_cyclic
 
     def _column(self, x, norm_w, weight, bias):
         """RMSNorm on my tokens → all-gather → column-parallel GEMM."""
@@ -278,8 +281,8 @@ class TPDecoderLayer(nn.Module):
 
     def forward(self, x, cos, sin, position_ids, cu_seqlens, max_seqlen, seqlens_host=None):
         qkv = self._column(x, self.input_norm_weight, self.qkv_weight, self.qkv_bias)
-        qkv = ops.qk_rope_(qkv, cos, sin, position_ids, self.hq, self.hk, self.d, self.interleaved_rope)
-        o = ops.attention_qkv_packed(qkv, cu_seqlens, self.hq, self.hk, self.d, max_seqlen, seqlens_host)
+        qkv = rotate(qkv, cos, sin, position_ids, self.hq, self.hk, self.d, self.interleaved_rope, self.rope_sections, self.rope_cyclic)
+        o = ops.attention_qkv_packed(qkv, cu_seqlens, self.hq, self.hk, self.d, max_seqlen, seqlens_host, self.window, self.sinks)
         x = self._row(o, self.o_weight, x)
         gu = self._column(x, self.post_norm_weight, self.gate_up_weight, None)
         act = ops.geglu(gu) if self.gelu else ops.swiglu(gu)
@@ -375,6 +378,8 @@ class TensorParallelCausalLM(nn.Module):
                 position_ids: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
                 max_seqlen: Optional[int] = None, seqlens_host: Optional[Sequence[int]] = None, shift_labels: bool = True, **_):
         from ..models.decoder import CausalLMOutput, _positions_from_cu
+        if _.get("teacher_indices") is not None or _.get("teacher_logits") is not None:
+            raise ValueError("the tensor-parallel model has no distillation loss: its vocabulary is split over the ranks")
         tp = self.tp
         dev = input_ids.device
         B, S = input_ids.shape if input_ids.dim() == 2 else (1, input_ids.shape[0])
@@ -389,7 +394,7 @@ class TensorParallelCausalLM(nn.Module):
             seqlens_host = seqlens_host or [S] * B
         if position_ids is None:
             position_ids = torch.arange(S, device=dev).repeat(B) if derived else _positions_from_cu(cu_seqlens, T)
-        pos = position_ids.reshape(T)
+        pos = token_positions(position_ids, input_ids, self.config.rope_sections)
         cos, sin = self._rope(max(int(max_seqlen or S), 1), dev)
         Tl = T // tp.world
         mine = slice(tp.rank * Tl, (tp.rank + 1) * Tl)

@@ -64,6 +64,9 @@ def print_chronicals_banner(num_gpus: int = 1, model_name: str = "", extra: Opti
     print(line)
 
 
+_TEACHER = ("teacher_indices", "teacher_logits")      # a teacher's top logits [B, S, K], where a batch carries them
+
+
 def _batch_fields(batch: Any) -> Dict[str, Any]:
     """Normalise a batch (PackedBatch | dict | tuple) to a dict of model inputs."""
     if isinstance(batch, PackedBatch):
@@ -145,6 +148,8 @@ class ChronicalsTrainer:
         if self.is_native_model:
             self.model.z_loss_weight = float(a.z_loss_weight or 0.0)
             self.model.label_smoothing = float(a.label_smoothing or 0.0)
+            self.model.distill_weight = float(self._get("distill_weight", 0.5))
+            self.model.distill_temperature = float(self._get("distill_temperature", 1.0))
         self._active_optimizations["fused_kernels"] = on_gpu and self.is_native_model
         self._active_optimizations["cut_cross_entropy"] = self.is_native_model
         self._active_optimizations["varlen_attention"] = bool(a.use_flash_varlen)
@@ -338,7 +343,7 @@ class ChronicalsTrainer:
         f = _batch_fields(batch)
         nb = bool(self.args.non_blocking_transfers)
         out: Dict[str, Any] = {}
-        for k in ("input_ids", "labels", "position_ids", "cu_seqlens", "attention_mask"):
+        for k in ("input_ids", "labels", "position_ids", "cu_seqlens", "attention_mask", *_TEACHER):
             v = f.get(k)
             if isinstance(v, torch.Tensor):
                 out[k] = v.to(self.device, non_blocking=nb)
@@ -353,8 +358,11 @@ class ChronicalsTrainer:
         if self.is_native_model:
             o = self.model(inp["input_ids"], position_ids=inp.get("position_ids"), labels=inp["labels"],
                            cu_seqlens=inp.get("cu_seqlens"), max_seqlen=inp.get("max_seqlen"),
-                           seqlens_host=inp.get("seqlens_host"), shift_labels=bool(self._get("shift_labels", True)))
+                           seqlens_host=inp.get("seqlens_host"), shift_labels=bool(self._get("shift_labels", True)),
+                           **{k: inp[k] for k in _TEACHER if k in inp})
             return o.loss
+        if any(k in inp for k in _TEACHER):
+            raise ValueError("a teacher's top logits in the batch: only this framework's own models have a distillation loss")
         kw = {"input_ids": inp["input_ids"], "labels": inp["labels"]}
         if inp.get("attention_mask") is not None and not self.args.use_sequence_packing:
             kw["attention_mask"] = inp["attention_mask"]
@@ -402,7 +410,8 @@ class ChronicalsTrainer:
             loss = self.zero3.forward_backward(inp["input_ids"], labels=inp["labels"], position_ids=inp.get("position_ids"),
                                                cu_seqlens=inp.get("cu_seqlens"), max_seqlen=inp.get("max_seqlen"),
                                                seqlens_host=inp.get("seqlens_host"),
-                                               shift_labels=bool(self._get("shift_labels", True)))
+                                               shift_labels=bool(self._get("shift_labels", True)),
+                                               **{k: inp[k] for k in _TEACHER if k in inp})
             self.optimizer.step()
             return loss
         if self._nvtx:
@@ -441,7 +450,8 @@ class ChronicalsTrainer:
             f["seqlens_host"] = None
         key = (tuple(ids.shape), tuple(f["cu_seqlens"].shape) if isinstance(f.get("cu_seqlens"), torch.Tensor) else None,
                f.get("max_seqlen"), tuple(f["seqlens_host"]) if f.get("seqlens_host") is not None and
-               not isinstance(f.get("cu_seqlens"), torch.Tensor) else None)
+               not isinstance(f.get("cu_seqlens"), torch.Tensor) else None,
+               tuple(tuple(f[k].shape) for k in ("position_ids", *_TEACHER) if isinstance(f.get(k), torch.Tensor)))
         if self._graph is None or self._graph["key"] != key:
             self._capture_graph(f, key)
         g = self._graph
@@ -462,7 +472,7 @@ class ChronicalsTrainer:
         forward + backward + optimizer kernels of one micro-step into a CUDA graph."""
         a = self.args
         static: Dict[str, torch.Tensor] = {}
-        for k in ("input_ids", "labels", "position_ids", "cu_seqlens"):
+        for k in ("input_ids", "labels", "position_ids", "cu_seqlens", *_TEACHER):
             v = f.get(k) if k != "labels" else f.get("labels", f["input_ids"])
             if isinstance(v, torch.Tensor):
                 static[k] = v.to(self.device).clone()
@@ -751,7 +761,8 @@ class ChronicalsTrainer:
                     tot += self.zero3.forward_only(inp["input_ids"], labels=inp["labels"],
                                                    position_ids=inp.get("position_ids"), cu_seqlens=inp.get("cu_seqlens"),
                                                    max_seqlen=inp.get("max_seqlen"),
-                                                   shift_labels=bool(self._get("shift_labels", True))).loss.float()
+                                                   shift_labels=bool(self._get("shift_labels", True)),
+                                                   **{k: inp[k] for k in _TEACHER if k in inp}).loss.float()
             else:
                 tot += self._forward_loss(inp).float()
             n += 1

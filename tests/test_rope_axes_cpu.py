@@ -12,12 +12,12 @@ def turned(x, cos, sin, pos, axes, heads, d, pairs, inverse=False):
     rows = pos.clamp(0, cos.shape[0] - 1)
     turn = torch.stack([torch.complex(cos[rows[a], f].double(), sin[rows[a], f].double()) for f, a in enumerate(axes)], 1)[:, None]
     turn = turn.conj() if inverse else turn
-    y = x.double().reshape(T, -1, d).clone()
+    y = x.double().reshape(T, -1, d)
     h = y[:, :heads]
     z = torch.complex(h[..., 0::2], h[..., 1::2]) if pairs else torch.complex(h[..., : d // 2], h[..., d // 2:])
     z = z * turn
-    y[:, :heads] = torch.stack((z.real, z.imag), -1).flatten(-2) if pairs else torch.cat((z.real, z.imag), -1)
-    return y.reshape(T, -1)
+    h = torch.stack((z.real, z.imag), -1).flatten(-2) if pairs else torch.cat((z.real, z.imag), -1)
+    return torch.cat((h, y[:, heads:]), 1).reshape(T, -1)
 
 
 AXES = {((2, 3, 3), False): (0, 0, 1, 1, 1, 2, 2, 2), ((4, 2, 2), True): (0, 1, 2, 0, 1, 2, 0, 0), ((8,), False): (0,) * 8,
