@@ -746,6 +746,9 @@ __global__ void attn_delta_generic_kernel(const bf16* __restrict__ dO, const bf1
 // the exp2 unit (16 results per clock and SM) is the bound: 1024 cycles per [128 x 128] of scores.
 constexpr int FWD3_THREADS = 192;                      // 4 softmax warps + the MMA-issuing warp + the TMA warp
 constexpr float FWD3_RAISE_LOG2 = 8.f;                 // raise the reference maximum only beyond 2^8
+#ifndef FWD3_FMA_OF_8
+#define FWD3_FMA_OF_8 3
+#endif
 
 template <int D>
 struct Fwd3Smem {
@@ -960,7 +963,9 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       // columns j*64 + c <= qb*128 + r are visible; only the blocks that touch the diagonal need the test
       const int kb = block_of(j, n_snk, skip);
       const int lim = qb * 128 + r - kb * 64;
-      if (WIN && kb * 64 + a.window <= qb * 128 + 127) {   // some row's window begins after the block's first key
+      const bool edge = WIN && kb * 64 + a.window <= qb * 128 + 127;   // some row's window begins after the block's first key
+      const bool masked = edge || kb >= 2 * qb;
+      if (edge) {
         const int lo = lim - a.window + 1, snk = a.sinks - kb * 64;
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
@@ -1020,6 +1025,40 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const float mb = WIN && m_ref == -INFINITY ? 0.f : m_ref * sl2;
       uint32_t pk[32];
       float rs0 = 0.f, rs1 = 0.f;
+      if (WIN) {
+        // two scores an instruction; FWD3_FMA_OF_8 pairs in eight exponentiate on the FMA pipe where nothing is masked
+        const uint64_t sc = f2_pack(sl2, sl2), nb = f2_pack(-mb, -mb);
+        uint64_t sum = f2_pack(0.f, 0.f), sum1 = sum;
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float e0, e1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(i < 16 ? s0[2 * i] : s1[2 * i - 32]),
+                                     __uint_as_float(i < 16 ? s0[2 * i + 1] : s1[2 * i - 31])), sc, nb), e0, e1);
+            e0 = ex2_approx(e0);
+            e1 = ex2_approx(e1);
+            if (i & 1) sum1 = f2_add(sum1, f2_pack(e0, e1)); else sum = f2_add(sum, f2_pack(e0, e1));
+            pk[i] = pack_bf16x2(e0, e1);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const uint64_t x = f2_fma(f2_pack(__uint_as_float(i < 16 ? s0[2 * i] : s1[2 * i - 32]),
+                                              __uint_as_float(i < 16 ? s0[2 * i + 1] : s1[2 * i - 31])), sc, nb);
+            float e0, e1;
+            if ((i * FWD3_FMA_OF_8) % 8 < FWD3_FMA_OF_8) {
+              ex2_fma2(x, e0, e1);
+            } else {
+              f2_unpack(x, e0, e1);
+              e0 = ex2_approx(e0);
+              e1 = ex2_approx(e1);
+            }
+            if (i & 1) sum1 = f2_add(sum1, f2_pack(e0, e1)); else sum = f2_add(sum, f2_pack(e0, e1));
+            pk[i] = pack_bf16x2(e0, e1);
+          }
+        }
+        f2_unpack(f2_add(sum, sum1), rs0, rs1);
+      } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float e0 = ex2_approx(fmaf(__uint_as_float(s0[2 * i]), sl2, -mb));
@@ -1032,6 +1071,7 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         rs1 += e2 + e3;
         pk[i] = pack_bf16x2(e0, e1);
         pk[16 + i] = pack_bf16x2(e2, e3);
+      }
       }
       l_run += rs0 + rs1;
       CB_PHASE(5);
