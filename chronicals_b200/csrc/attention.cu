@@ -30,33 +30,12 @@
 // (:2460-3209); the reference has no attention backward of its own.
 #include <algorithm>
 #include <cstdlib>
-#include "common.cuh"
+#include "attention.cuh"
 
 namespace cb {
 
 constexpr int ATT_THREADS = 128;
 constexpr int BWD2_THREADS = 256;   // backward variant with two threads per score row
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct AttnArgs {
-  int T, hq, hk, n_docs;
-  const int* cu;        // [n_docs + 1]
-  float scale;
-  bf16* O;              // [T, hq, D], row pitch ldo
-  long long ldo;
-  float* lse;           // [hq, T]
-  // backward
-  const float* delta;   // [hq, T]  rowsum(dO * O)
-  float* dq_acc;        // [T, hq, D] fp32, zero-initialised; accumulated with red.add
-  float* dk_part;       // [T, hk, D] fp32, zero-initialised; accumulated with red.add over the group's query heads
-  float* dv_part;
-  int* status;
-  int o_tma;            // forward: a tensor map over O exists, whole blocks may leave by TMA store
-  // windowed forms: a query sees the last `window` keys of its document, its own among them, and the document's first `sinks`
-  int window, sinks;
-  int sink_run;         // backward: query blocks per CTA of a key block that holds sinks
-};
-
 // Phase timers (compiled in with -DCB_ATTN_PHASE_TIMERS only): two threads of every CTA - the MMA-issuing thread
 // and one thread of another warp - add the SM clock cycles they spend between consecutive marks to a global
 // table, which cb_attn_phase_read() copies out.  The default build contains none of this.
@@ -113,115 +92,6 @@ __device__ __forceinline__ bool locate_tile(const int* cu, int n_docs, int b, in
   }
   if (beyond != nullptr) *beyond = b;                  // index among the CTAs past the last tile
   return false;
-}
-
-// The grid holds at least ceil((T - cu[n_docs]) / 128) CTAs past the last tile (per head).  In the forward
-// kernels they write the zeros of the padding rows at or after cu[n_docs], 128 rows x D columns each, so the
-// caller need not clear the output first.
-template <int D>
-__device__ __forceinline__ void zero_padding_rows(const AttnArgs& a, int beyond, int h) {
-  const int valid = a.cu[a.n_docs];
-  const long long row0 = static_cast<long long>(valid) + static_cast<long long>(beyond) * 128;
-  constexpr int CH = D / 8;                            // 16-byte chunks per row of one head
-  for (int i = threadIdx.x; i < 128 * CH; i += blockDim.x) {
-    const long long t = row0 + i / CH;
-    if (t < a.T) reinterpret_cast<uint4*>(a.O + t * a.ldo + static_cast<long long>(h) * D)[i % CH] = make_uint4(0u, 0u, 0u, 0u);
-  }
-}
-
-// The tile of a windowed kernel: CTA b's, document by document, the weights being all but equal (a window's worth of blocks).
-// Forward, one tile per query block, the last block of a document first.  Backward, one per key block; a key block that holds sinks
-// is seen by every later query of its document, and its query blocks are shared out over CTAs in runs of a.sink_run, which come
-// first in their document.  blk: the block of the tile, run: of which run (-1: a key block without sinks).
-template <bool BWD>
-__device__ __forceinline__ bool locate_window_tile(const AttnArgs& a, int b, int& start, int& len, int& nblk, int& blk, int& run,
-                                                   int* beyond = nullptr) {
-  const int lane = threadIdx.x & 31;
-  const int with_sinks = BWD ? (a.sinks + 127) >> 7 : 0;
-  for (int d0 = 0; d0 < a.n_docs; d0 += 32) {
-    const int d = d0 + lane;
-    int st = 0, ln = 0;
-    if (d < a.n_docs) {
-      st = a.cu[d];
-      ln = a.cu[d + 1] - st;
-    }
-    const int nb = (ln + 127) >> 7, ns = min(nb, with_sinks);
-    const int runs = BWD ? (nb + a.sink_run - 1) / a.sink_run : 0;
-    const int mine = nb - ns + ns * runs;
-    int upto = mine;                                   // tiles of the documents up to mine
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    const unsigned m = __ballot_sync(0xffffffffu, b < upto);
-    if (m != 0) {
-      const int src = __ffs(m) - 1;
-      const int at = b - __shfl_sync(0xffffffffu, upto - mine, src);
-      start = __shfl_sync(0xffffffffu, st, src);
-      len = __shfl_sync(0xffffffffu, ln, src);
-      nblk = __shfl_sync(0xffffffffu, nb, src);
-      const int n_s = __shfl_sync(0xffffffffu, ns, src), n_r = __shfl_sync(0xffffffffu, runs, src);
-      if (!BWD) {
-        blk = nblk - 1 - at;
-        run = -1;
-      } else if (at < n_s * n_r) {
-        blk = at % n_s;
-        run = at / n_s;
-      } else {
-        blk = at - n_s * n_r + n_s;
-        run = -1;
-      }
-      return true;
-    }
-    b -= __shfl_sync(0xffffffffu, upto, 31);
-  }
-  if (beyond != nullptr) *beyond = b;                  // index among the CTAs past the last tile
-  return false;
-}
-
-// The query blocks [first, first + count) that key block `jb` of a document of nblk blocks meets, or those of its run
-__device__ __forceinline__ void window_query_blocks(const AttnArgs& a, int jb, int run, int nblk, int& first, int& count) {
-  const int lo = run < 0 ? jb : max(jb, run * a.sink_run);
-  const int hi = run < 0 ? min(nblk, ((jb * 128 + 127 + a.window - 1) >> 7) + 1) : min(nblk, (run + 1) * a.sink_run);
-  first = lo;
-  count = hi - lo;
-}
-
-// store 32 consecutive values of thread-row r as bf16 into a [128 x 128] operand image made of two
-// 64-column panels of 16 KB, 128-byte rows, 16-byte chunks XOR-swizzled by (row & 7)
-__device__ __forceinline__ void store_row_chunk32(uint8_t* base, int r, int c32, const float (&v)[32]) {
-  const int panel = c32 >> 1;                 // chunks 0,1 -> panel 0 ; 2,3 -> panel 1
-  uint8_t* row = base + panel * 16384 + r * 128;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int cc = (c32 & 1) * 4 + q;         // 16-byte chunk index within the 128-byte row
-    uint4 u;
-    u.x = pack_bf16x2(v[8 * q + 0], v[8 * q + 1]);
-    u.y = pack_bf16x2(v[8 * q + 2], v[8 * q + 3]);
-    u.z = pack_bf16x2(v[8 * q + 4], v[8 * q + 5]);
-    u.w = pack_bf16x2(v[8 * q + 6], v[8 * q + 7]);
-    *reinterpret_cast<uint4*>(row + ((cc ^ (r & 7)) << 4)) = u;
-  }
-}
-
-// the same for 32 values already packed as bf16 pairs
-__device__ __forceinline__ void store_row_chunk32_packed(uint8_t* base, int r, int c32, const uint32_t (&v)[16]) {
-  const int panel = c32 >> 1;
-  uint8_t* row = base + panel * 16384 + r * 128;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int cc = (c32 & 1) * 4 + q;
-    *reinterpret_cast<uint4*>(row + ((cc ^ (r & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-  }
-}
-
-// descriptors over a [128 rows x D] bf16 tile stored as D/64 panels of 16 KB
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t base, int kk) {      // K = columns, k-step of 16 columns
-  return umma_smem_desc(base + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t base, int kk) {     // K = rows, k-step of 16 rows
-  return umma_smem_desc(base + kk * 2048, 16384, 1024);
 }
 
 // Forward softmax passes over my row of the score tile (fp32, TMEM columns [0, 128)), in two versions: the
@@ -746,9 +616,6 @@ __global__ void attn_delta_generic_kernel(const bf16* __restrict__ dO, const bf1
 // the exp2 unit (16 results per clock and SM) is the bound: 1024 cycles per [128 x 128] of scores.
 constexpr int FWD3_THREADS = 192;                      // 4 softmax warps + the MMA-issuing warp + the TMA warp
 constexpr float FWD3_RAISE_LOG2 = 8.f;                 // raise the reference maximum only beyond 2^8
-#ifndef FWD3_FMA_OF_8
-#define FWD3_FMA_OF_8 3
-#endif
 
 template <int D>
 struct Fwd3Smem {
@@ -762,7 +629,7 @@ struct Fwd3Smem {
   static constexpr int TOTAL = OFF_BAR + 256 + 1024;
 };
 
-template <int D, bool WIN>
+template <int D>
 __global__ void __launch_bounds__(FWD3_THREADS, 2)
 attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const AttnArgs a) {
@@ -781,25 +648,14 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   int start, len, qb, nblk;
   int beyond = 0;
-  int run = 0;
-  if (!(WIN ? locate_window_tile<false>(a, blockIdx.y, start, len, nblk, qb, run, &beyond)
-            : locate_tile(a.cu, a.n_docs, blockIdx.y, start, len, qb, nblk, &beyond))) {
+  if (!locate_tile(a.cu, a.n_docs, blockIdx.y, start, len, qb, nblk, &beyond)) {
     zero_padding_rows<D>(a, beyond, blockIdx.x);
     return;
   }
-  if (!WIN) qb -= 1;                                   // weight = kv blocks up to the diagonal = qb + 1
+  qb -= 1;
   const int h = blockIdx.x;
   const int hkv = h / (a.hq / a.hk);
-  int n_kv = min(2 * qb + 2, (len + 63) >> 6);         // 64-row kv blocks up to and including the diagonal
-  // windowed: the blocks of the sinks, then those from the first row's first key on; `skip` blocks between them are left out
-  int n_snk = 0, skip = 0;
-  if (WIN) {
-    const int lo = max(0, qb * 128 - a.window + 1) >> 6;
-    n_snk = min((a.sinks + 63) >> 6, lo);
-    skip = lo - n_snk;
-    n_kv -= skip;
-  }
-  const auto block_of = [&](int j, int s_, int k_) { return WIN && j >= s_ ? j + k_ : j; };
+  const int n_kv = min(2 * qb + 2, (len + 63) >> 6);   // 64-row kv blocks up to and including the diagonal
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -847,14 +703,13 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int u_start = __shfl_sync(0xffffffffu, start, 0);
     const int u_qb = __shfl_sync(0xffffffffu, qb, 0);
     const int u_nkv = __shfl_sync(0xffffffffu, n_kv, 0);
-    const int u_snk = __shfl_sync(0xffffffffu, n_snk, 0), u_skip = __shfl_sync(0xffffffffu, skip, 0);
     if (elect_one()) {
       mbar_expect_tx(bar_q, L::QT);
 #pragma unroll
       for (int p = 0; p < PANELS; ++p) tma_load_2d(sQ + p * 16384, &tmQ, bar_q, h * D + p * 64, u_start + u_qb * 128);
     }
     for (int j = 0; j < u_nkv && ok; ++j) {
-      const int st = j % NS, kv_row = u_start + block_of(j, u_snk, u_skip) * 64;
+      const int st = j % NS;
       if (j >= NS) {                                    // the stage's previous block: S(j - NS) complete
         ok = __all_sync(0xffffffffu, mbar_wait(k_empty + st, ((j / NS) - 1) & 1, abort_flag, a.status, CB_ERR_WAIT_EMPTY) && ok);
         if (!ok) break;
@@ -863,7 +718,7 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         mbar_expect_tx(k_full + st, L::KT);
 #pragma unroll
         for (int p = 0; p < PANELS; ++p)
-          tma_load_2d(sK + st * L::KT + p * 8192, &tmK, k_full + st, hkv * D + p * 64, kv_row);
+          tma_load_2d(sK + st * L::KT + p * 8192, &tmK, k_full + st, hkv * D + p * 64, u_start + j * 64);
       }
       if (j >= NS) {                                    // P V of block j - NS complete
         ok = __all_sync(0xffffffffu, mbar_wait(v_empty + st, ((j / NS) - 1) & 1, abort_flag, a.status, CB_ERR_WAIT_EMPTY) && ok);
@@ -873,7 +728,7 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         mbar_expect_tx(v_full + st, L::KT);
 #pragma unroll
         for (int p = 0; p < PANELS; ++p)
-          tma_load_2d(sV + st * L::KT + p * 8192, &tmV, v_full + st, hkv * D + p * 64, kv_row);
+          tma_load_2d(sV + st * L::KT + p * 8192, &tmV, v_full + st, hkv * D + p * 64, u_start + j * 64);
       }
     }
     __syncwarp();
@@ -961,19 +816,8 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       CB_PHASE(2);
       // columns j*64 + c <= qb*128 + r are visible; only the blocks that touch the diagonal need the test
-      const int kb = block_of(j, n_snk, skip);
-      const int lim = qb * 128 + r - kb * 64;
-      const bool edge = WIN && kb * 64 + a.window <= qb * 128 + 127;   // some row's window begins after the block's first key
-      const bool masked = edge || kb >= 2 * qb;
-      if (edge) {
-        const int lo = lim - a.window + 1, snk = a.sinks - kb * 64;
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          if (c < lo && c >= snk) s0[c] = 0xff800000u;
-          if (c + 32 < lo && c + 32 >= snk) s1[c] = 0xff800000u;
-        }
-      }
-      if (kb >= 2 * qb) {
+      const int lim = qb * 128 + r - j * 64;
+      if (j >= 2 * qb) {
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
           if (c > lim) s0[c] = 0xff800000u;             // -inf
@@ -1021,44 +865,9 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (up) m_ref = mx;
       }
       CB_PHASE(4);
-      // a row of a windowed tile may have seen no key yet: its scores are all -inf and stand for zeros against any reference
-      const float mb = WIN && m_ref == -INFINITY ? 0.f : m_ref * sl2;
+      const float mb = m_ref * sl2;
       uint32_t pk[32];
       float rs0 = 0.f, rs1 = 0.f;
-      if (WIN) {
-        // two scores an instruction; FWD3_FMA_OF_8 pairs in eight exponentiate on the FMA pipe where nothing is masked
-        const uint64_t sc = f2_pack(sl2, sl2), nb = f2_pack(-mb, -mb);
-        uint64_t sum = f2_pack(0.f, 0.f), sum1 = sum;
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float e0, e1;
-            f2_unpack(f2_fma(f2_pack(__uint_as_float(i < 16 ? s0[2 * i] : s1[2 * i - 32]),
-                                     __uint_as_float(i < 16 ? s0[2 * i + 1] : s1[2 * i - 31])), sc, nb), e0, e1);
-            e0 = ex2_approx(e0);
-            e1 = ex2_approx(e1);
-            if (i & 1) sum1 = f2_add(sum1, f2_pack(e0, e1)); else sum = f2_add(sum, f2_pack(e0, e1));
-            pk[i] = pack_bf16x2(e0, e1);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const uint64_t x = f2_fma(f2_pack(__uint_as_float(i < 16 ? s0[2 * i] : s1[2 * i - 32]),
-                                              __uint_as_float(i < 16 ? s0[2 * i + 1] : s1[2 * i - 31])), sc, nb);
-            float e0, e1;
-            if ((i * FWD3_FMA_OF_8) % 8 < FWD3_FMA_OF_8) {
-              ex2_fma2(x, e0, e1);
-            } else {
-              f2_unpack(x, e0, e1);
-              e0 = ex2_approx(e0);
-              e1 = ex2_approx(e1);
-            }
-            if (i & 1) sum1 = f2_add(sum1, f2_pack(e0, e1)); else sum = f2_add(sum, f2_pack(e0, e1));
-            pk[i] = pack_bf16x2(e0, e1);
-          }
-        }
-        f2_unpack(f2_add(sum, sum1), rs0, rs1);
-      } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float e0 = ex2_approx(fmaf(__uint_as_float(s0[2 * i]), sl2, -mb));
@@ -1071,7 +880,6 @@ attn_fwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         rs1 += e2 + e3;
         pk[i] = pack_bf16x2(e0, e1);
         pk[16 + i] = pack_bf16x2(e2, e3);
-      }
       }
       l_run += rs0 + rs1;
       CB_PHASE(5);
@@ -1562,10 +1370,6 @@ constexpr int BWD3_SOFTMAX_WARPS = 8;
 constexpr int BWD3_THREADS = 512;                     // warps 14 and 15 only complete the last warpgroup
 // registers a thread after the split: 256 x 144 + 128 x 144 + 128 x 80 = the 512 x 128 at launch
 constexpr int BWD3_REGS_SOFTMAX = 144, BWD3_REGS_DQ = 144, BWD3_REGS_ISSUE = 80;
-template <int N>
-__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int D, bool WIN>
 __global__ void __launch_bounds__(BWD3_THREADS, 1)
@@ -2063,12 +1867,12 @@ int cb_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse
     if (!a.o_tma) mo = mq;                              // O is not TMA-addressable: every block stores row by row
     if (D == 64) {
       static bool cfg = false;
-      if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<64, false>, cb::Fwd3Smem<64>::TOTAL); if (e) return e; cfg = true; }
-      cb::attn_fwd3_kernel<64, false><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<64>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
+      if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<64>, cb::Fwd3Smem<64>::TOTAL); if (e) return e; cfg = true; }
+      cb::attn_fwd3_kernel<64><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<64>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
     } else {
       static bool cfg = false;
-      if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<128, false>, cb::Fwd3Smem<128>::TOTAL); if (e) return e; cfg = true; }
-      cb::attn_fwd3_kernel<128, false><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<128>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
+      if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<128>, cb::Fwd3Smem<128>::TOTAL); if (e) return e; cfg = true; }
+      cb::attn_fwd3_kernel<128><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<128>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
     }
     return static_cast<int>(cudaGetLastError());
   }
@@ -2093,38 +1897,6 @@ int cb_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse
     static bool cfg = false;
     if (!cfg) { e = set_smem(cb::attn_fwd_kernel<128>, cb::FwdSmem<128>::TOTAL); if (e) return e; cfg = true; }
     cb::attn_fwd_kernel<128><<<grid, cb::ATT_THREADS, cb::FwdSmem<128>::TOTAL, s>>>(mq, mk, mv, a);
-  }
-  return static_cast<int>(cudaGetLastError());
-}
-
-// Forward over the last `window` (>= 1) keys and the first `sinks` (>= 0) of each document; the rest as cb_attn_fwd.
-int cb_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu, int n_docs, int T,
-                       int hq, int hk, int D, long long ldq, long long ldk, long long ldv, long long ldo, float scale, int window,
-                       int sinks, int* status, void* stream) {
-  if ((D != 64 && D != 128) || hk <= 0 || hq % hk != 0 || T <= 0 || n_docs <= 0 || window < 1 || sinks < 0) return -1;
-  CUtensorMap mq, mk64, mv64, mo;
-  int e = cbhost::make_tmap(&mq, q, static_cast<unsigned long long>(hq) * D, T, ldq, 64, 128);
-  if (!e) e = cbhost::make_tmap(&mk64, k, static_cast<unsigned long long>(hk) * D, T, ldk, 64, 64);
-  if (!e) e = cbhost::make_tmap(&mv64, v, static_cast<unsigned long long>(hk) * D, T, ldv, 64, 64);
-  if (e) return e;
-  cb::AttnArgs a = {};
-  a.T = T; a.hq = hq; a.hk = hk; a.n_docs = n_docs; a.cu = cu; a.scale = scale;
-  a.O = static_cast<cb::bf16*>(o); a.ldo = ldo; a.lse = lse; a.status = status;
-  a.window = std::min(window, T); a.sinks = std::min(sinks, T);
-  a.o_tma = cbhost::make_tmap(&mo, o, static_cast<unsigned long long>(hq) * D, T, ldo, 64, 128) == 0 ? 1 : 0;
-  if (!a.o_tma) mo = mq;
-  const long long tiles = (T + 127LL) / 128 + n_docs;
-  if (tiles > 65535) return -1;
-  const dim3 grid(hq, static_cast<unsigned>(tiles));
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (D == 64) {
-    static bool cfg = false;
-    if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<64, true>, cb::Fwd3Smem<64>::TOTAL); if (e) return e; cfg = true; }
-    cb::attn_fwd3_kernel<64, true><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<64>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
-  } else {
-    static bool cfg = false;
-    if (!cfg) { e = set_smem(cb::attn_fwd3_kernel<128, true>, cb::Fwd3Smem<128>::TOTAL); if (e) return e; cfg = true; }
-    cb::attn_fwd3_kernel<128, true><<<grid, cb::FWD3_THREADS, cb::Fwd3Smem<128>::TOTAL, s>>>(mq, mk64, mv64, mo, a);
   }
   return static_cast<int>(cudaGetLastError());
 }

@@ -230,6 +230,14 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -338,6 +346,11 @@ __device__ __forceinline__ float ex2_fma(float x) {
   const float r = __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
   return x < -125.f ? 0.f : r;                         // masked scores (-inf) give an exact zero, like ex2.approx.ftz
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {     // one instruction
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // Two 32-bit values in one 64-bit register: one instruction does both (rounding each as the single one does).  They halve the
 // instructions to issue, not the work of the FMA pipe.
 __device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
@@ -360,23 +373,6 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-// ex2_fma for two values that no mask has touched: below -125 the result is 2^-125, not zero
-__device__ __forceinline__ void ex2_fma2(uint64_t x, float& lo, float& hi) {
-  float a, b;
-  f2_unpack(x, a, b);
-  const uint64_t xc = f2_pack(fmaxf(a, -125.f), fmaxf(b, -125.f));
-  const uint64_t t = f2_add(xc, f2_pack(12582912.f, 12582912.f));
-  const uint64_t n = f2_add(t, f2_pack(-12582912.f, -12582912.f));
-  const uint64_t f = f2_fma(n, f2_pack(-1.f, -1.f), xc);
-  uint64_t p = f2_fma(f2_pack(0.05508868396282196f, 0.05508868396282196f), f, f2_pack(0.24260404706001282f, 0.24260404706001282f));
-  p = f2_fma(p, f, f2_pack(0.6932762265205383f, 0.6932762265205383f));
-  p = f2_fma(p, f, f2_pack(0.9999289512634277f, 0.9999289512634277f));
-  float pa, pb, ta, tb;
-  f2_unpack(p, pa, pb);
-  f2_unpack(t, ta, tb);
-  lo = __int_as_float(__float_as_int(pa) + (__float_as_int(ta) << 23));
-  hi = __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23));
 }
 __device__ __forceinline__ float tanh_approx(float x) {
   float y;
