@@ -1106,6 +1106,10 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       load_q(0);
     }
     ok = __all_sync(0xffffffffu, mbar_wait(bar_kv, 0, abort_flag, a.status, CB_ERR_WAIT_FULL));
+    if (WIN && (jb + 1) * 128 > len) {                 // keys behind the document's end: 0 x NaN is NaN
+      zero_tile_rows<PANELS>(sK, len - jb * 128);
+      zero_tile_rows<PANELS>(sV, len - jb * 128);
+    }
   }
 
   const int r = q4 * 32 + (tid & 31);
@@ -1133,6 +1137,10 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     CB_PHASE(0);
     if (w0) {
       ok = __all_sync(0xffffffffu, mbar_wait(q_full, it & 1, abort_flag, a.status, CB_ERR_WAIT_FULL) && ok);
+      if (WIN && ok && (i + 1) * 128 > len) {          // queries behind it
+        zero_tile_rows<PANELS>(sQ, len - i * 128);
+        zero_tile_rows<PANELS>(sdO, len - i * 128);
+      }
       tc_fence_after();
       if (elect_one()) {
         if (ok) {
@@ -1152,8 +1160,7 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const float lse2 = row_ok ? lse_n * LOG2E : INFINITY, dlt = dlt_n;
     row_stats(it + 1, lse_n, dlt_n);
     const bool diag = WIN ? i == jb : it == 0;
-    const bool edge = WIN && (i - jb) * 128 + 127 >= a.window;         // some query's window begins after the block's first key
-    const int lo = rg - a.window + 1 - jb * 128, snk = a.sinks - jb * 128;
+    const bool cut = WIN && (diag || (i - jb) * 128 + 127 >= a.window);  // by the diagonal or by some query's window
     CB_PHASE(1);
     // ---- phase 1: P = exp(S - lse), masked, to shared memory
     ok &= mbar_wait(bar_s, it & 1, abort_flag, a.status, CB_ERR_WAIT_TMEM_FULL);
@@ -1163,18 +1170,31 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     // my 64 probabilities stay in registers as bf16 pairs (pk) for phase 2; rows past the end of the document
     // carry lse = +inf and so exponentiate to exact zeros, only the diagonal block tests columns against rows
     uint32_t pk[2][16];
+    float pf[WIN ? 2 : 1][32];
 #pragma unroll
     for (int cl = 0; cl < 2; ++cl) {
       const int c = half * 2 + cl;
       uint32_t s[32];
       tmem_ld_32x32(t_row + C_S + c * 32, s);
       tmem_ld_wait();
-      if (WIN && edge) {
+      if (WIN) {
+        // two scores an instruction; the probabilities stay in 32 bits for dS, so that they are rounded once for dV and not for dS
+        if (cut) {
+          const int at = jb * 128 + c * 32;
+          const uint32_t see = low_bits(rg + 1 - at) & (~low_bits(rg - a.window + 1 - at) | low_bits(a.sinks - at));
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
-          if (c * 32 + k < lo && c * 32 + k >= snk) s[k] = 0xff800000u;                  // -inf
-      }
-      if (diag) {
+          for (int k = 0; k < 32; ++k)
+            if ((see >> k & 1u) == 0) s[k] = 0xff800000u;                                // -inf
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          float e0, e1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), f2_pack(sl2, sl2), f2_pack(-lse2, -lse2)), e0, e1);
+          pf[WIN ? cl : 0][2 * k] = ex2_approx(e0);
+          pf[WIN ? cl : 0][2 * k + 1] = ex2_approx(e1);
+          pk[cl][k] = pack_bf16x2(pf[WIN ? cl : 0][2 * k], pf[WIN ? cl : 0][2 * k + 1]);
+        }
+      } else if (diag) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           float e0 = ex2_approx(fmaf(__uint_as_float(s[2 * k]), sl2, -lse2));
@@ -1218,6 +1238,24 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
     for (int cl = 0; cl < 2; ++cl) {
       const int c = half * 2 + cl;
+      if (WIN) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {                // 16 columns at a time: 64 probabilities are held
+          uint32_t dp[16], ds[8];
+          tmem_ld_32x16(t_row + C_S + c * 32 + hh * 16, dp);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int at = hh * 16 + 2 * k;
+            float d0, d1;
+            f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(dp[2 * k]), __uint_as_float(dp[2 * k + 1])), f2_pack(-dlt, -dlt)),
+                             f2_pack(pf[WIN ? cl : 0][at], pf[WIN ? cl : 0][at + 1])), d0, d1);
+            ds[k] = pack_bf16x2(d0, d1);
+          }
+          store_row_chunk16_packed(sP, r, c * 2 + hh, ds);
+        }
+        continue;
+      }
       uint32_t dp[32];
       tmem_ld_32x32(t_row + C_S + c * 32, dp);
       tmem_ld_wait();
@@ -1266,6 +1304,10 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         uint32_t dq[32];
         tmem_ld_32x32(t_row + C_S + c * 32, dq);
         tmem_ld_wait();
+        if (WIN && !row_ok) {                          // rows of the next document: nothing, whatever this one holds
+#pragma unroll
+          for (int k = 0; k < 32; ++k) dq[k] = 0u;
+        }
         uint8_t* dstrow = sP + c * 16384 + r * 128;
 #pragma unroll
         for (int cc = 0; cc < 8; ++cc)
@@ -1504,8 +1546,9 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const bool in = (u_ib + it) * 128 + lane + 32 * k < len;
-          sStat[st * 256 + lane + 32 * k] = in ? lse_n[k] * LOG2E : INFINITY;
-          sStat[st * 256 + 128 + lane + 32 * k] = dlt_n[k];
+          const float l2 = in ? lse_n[k] * LOG2E : INFINITY;
+          sStat[st * 256 + lane + 32 * k] = WIN ? -l2 : l2;
+          sStat[st * 256 + 128 + lane + 32 * k] = WIN ? -dlt_n[k] : dlt_n[k];
         }
         arrive_w(st_full + st);
         fetch_stats(it + 1);
@@ -1525,6 +1568,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const uint32_t kA = smem_u32(sK), vA = smem_u32(sV), dsA = smem_u32(sdS);
       auto issue_s = [&](int it) {                       // S^T(it) = K Q(it)^T
         if (!wait_w(q_full + (it & 1), it >> 1, CB_ERR_WAIT_FULL)) return;
+        if (WIN && (ib + it + 1) * 128 > len) zero_tile_rows<PANELS>(sQ + (it & 1) * L::TILE, len - (ib + it) * 128);   // 0 x NaN is NaN
         const uint32_t qA = smem_u32(sQ + (it & 1) * L::TILE);
         tc_fence_after();
         if (elect_one()) {
@@ -1536,6 +1580,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       };
       auto issue_dp = [&](int it) {                      // dP^T(it) = V dO(it)^T
         if (!wait_w(do_full + it % NDO, it / NDO, CB_ERR_WAIT_FULL)) return;
+        if (WIN && (ib + it + 1) * 128 > len) zero_tile_rows<PANELS>(sdO + (it % NDO) * L::TILE, len - (ib + it) * 128);
         const uint32_t doA = smem_u32(sdO + (it % NDO) * L::TILE);
         tc_fence_after();
         if (elect_one()) {
@@ -1545,9 +1590,14 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           umma_commit(dp_full);
         }
       };
+      const bool key_tail = WIN && (jb + 1) * 128 > len;
       wait_w(k_full, 0, CB_ERR_WAIT_FULL);
+      if (key_tail && ok) zero_tile_rows<PANELS>(sK, len - jb * 128);
       if (ok) issue_s(0);
-      if (ok && wait_w(v_full, 0, CB_ERR_WAIT_FULL)) issue_dp(0);
+      if (ok && wait_w(v_full, 0, CB_ERR_WAIT_FULL)) {
+        if (key_tail) zero_tile_rows<PANELS>(sV, len - jb * 128);
+        issue_dp(0);
+      }
       CB_PHASE(12);
       for (int it = 0; it < u_n && ok; ++it) {
         if (!wait_w(p_ready, it, CB_ERR_WAIT_TMEM_EMPTY)) break;
@@ -1652,20 +1702,24 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       CB_PHASE(1);
       tc_fence_after();
       uint32_t pk[2][16];
+      float pf[WIN ? 2 : 1][32];
       {
         uint32_t s[2][32];
         tmem_ld_32x32(t_s, s[0]);
         tmem_ld_32x32(t_s + 32, s[1]);
         tmem_ld_wait();
-        if (WIN && (ib + it - jb) * 128 + 127 >= a.window && jb * 128 + r >= a.sinks) {
-          const int hi = (jb - ib - it) * 128 + r + a.window - half * 64;                // my key is behind these queries' windows
+        if (WIN && (ib + it == jb || (ib + it - jb) * 128 + 127 >= a.window)) {          // cut by the diagonal or by some query's window
+          const int key = jb * 128 + r;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (c >= hi) s[0][c] = 0xff800000u;                                          // -inf
-            if (c + 32 >= hi) s[1][c] = 0xff800000u;
+          for (int c = 0; c < 2; ++c) {
+            const int at = (ib + it) * 128 + half * 64 + c * 32;
+            const uint32_t see = ~low_bits(key - at) & (key < a.sinks ? 0xffffffffu : low_bits(key + a.window - at));
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if ((see >> k & 1u) == 0) s[c][k] = 0xff800000u;                           // -inf
           }
         }
-        if (WIN ? ib + it == jb : it == 0) {           // the diagonal block: queries before my key see nothing of it
+        if (!WIN && it == 0) {                         // the diagonal block: queries before my key see nothing of it
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             if (half * 64 + c < r) s[0][c] = 0xff800000u;                // -inf
@@ -1677,6 +1731,16 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float4 l = lse4[c * 8 + k];
+            if (WIN) {                                 // two scores an instruction; P stays in 32 bits for dS (statistics: negated)
+              float* e = &pf[WIN ? c : 0][4 * k];
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c][4 * k]), __uint_as_float(s[c][4 * k + 1])), f2_pack(sl2, sl2), f2_pack(l.x, l.y)), e[0], e[1]);
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(s[c][4 * k + 2]), __uint_as_float(s[c][4 * k + 3])), f2_pack(sl2, sl2), f2_pack(l.z, l.w)), e[2], e[3]);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) e[q] = ex2_approx(e[q]);
+              pk[c][2 * k] = pack_bf16x2(e[0], e[1]);
+              pk[c][2 * k + 1] = pack_bf16x2(e[2], e[3]);
+              continue;
+            }
             const float e0 = ex2_approx(fmaf(__uint_as_float(s[c][4 * k]), sl2, -l.x)), e1 = ex2_approx(fmaf(__uint_as_float(s[c][4 * k + 1]), sl2, -l.y));
             const float e2 = ex2_approx(fmaf(__uint_as_float(s[c][4 * k + 2]), sl2, -l.z));
             const float e3 = ex2_fma(fmaf(__uint_as_float(s[c][4 * k + 3]), sl2, -l.w));      // one in four on the FMA pipe
@@ -1693,7 +1757,24 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (!wait_w(dp_full, it, CB_ERR_WAIT_TMEM_FULL)) break;
       CB_PHASE(3);
       tc_fence_after();
-      {                                                // dS = P (dP - delta), over pk
+      if (WIN) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t dp[32];
+          tmem_ld_32x32(t_dp + c * 32, dp);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 d = dlt4[c * 8 + k];
+            const float* p = &pf[WIN ? c : 0][4 * k];
+            float d0, d1, d2, d3;
+            f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(dp[4 * k]), __uint_as_float(dp[4 * k + 1])), f2_pack(d.x, d.y)), f2_pack(p[0], p[1])), d0, d1);
+            f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(dp[4 * k + 2]), __uint_as_float(dp[4 * k + 3])), f2_pack(d.z, d.w)), f2_pack(p[2], p[3])), d2, d3);
+            pk[c][2 * k] = pack_bf16x2(d0, d1);
+            pk[c][2 * k + 1] = pack_bf16x2(d2, d3);
+          }
+        }
+      } else {                                         // dS = P (dP - delta), over pk
         uint32_t dp[2][32];
         tmem_ld_32x32(t_dp, dp[0]);
         tmem_ld_32x32(t_dp + 32, dp[1]);

@@ -126,6 +126,27 @@ __device__ __forceinline__ void store_row_chunk32_packed(uint8_t* base, int r, i
   }
 }
 
+// the same for 16 packed values
+__device__ __forceinline__ void store_row_chunk16_packed(uint8_t* base, int r, int c16, const uint32_t (&v)[8]) {
+  uint8_t* row = base + (c16 >> 2) * 16384 + r * 128;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int cc = (c16 & 3) * 2 + q;
+    *reinterpret_cast<uint4*>(row + ((cc ^ (r & 7)) << 4)) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  }
+}
+
+// Zeros rows [first, 128) of a tile that a TMA load has filled, for the tensor core; called by one whole warp.  The rows are those of
+// the next document, or padding that may hold anything: what multiplies them is zero, but 0 x NaN is NaN.
+template <int PANELS>
+__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int first) {
+  for (int i = first * 8 + static_cast<int>(threadIdx.x & 31); i < 128 * 8; i += 32)
+#pragma unroll
+    for (int p = 0; p < PANELS; ++p) reinterpret_cast<uint4*>(tile + p * 16384)[i] = make_uint4(0u, 0u, 0u, 0u);
+  fence_async_smem();
+  __syncwarp();
+}
+
 // descriptors over a [128 rows x D] bf16 tile stored as D/64 panels of 16 KB
 __device__ __forceinline__ uint64_t desc_kmajor(uint32_t base, int kk) {      // K = columns, k-step of 16 columns
   return umma_smem_desc(base + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024);

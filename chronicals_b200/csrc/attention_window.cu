@@ -151,11 +151,7 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       // probabilities are zero, and so have the V rows to be: 0 x NaN is NaN.
       const int j = u_nkv - 1, st = j % NS;
       if (wait_w(v_full + st, (j / NS) & 1, CB_ERR_WAIT_FULL)) {
-        for (int i = (len - qb * 128) * 8 + (tid & 31); i < 128 * 8; i += 32)
-#pragma unroll
-          for (int p = 0; p < PANELS; ++p) reinterpret_cast<uint4*>(sV + st * L::TILE + p * 16384)[i] = make_uint4(0u, 0u, 0u, 0u);
-        fence_async_smem();
-        __syncwarp();
+        zero_tile_rows<PANELS>(sV + st * L::TILE, len - qb * 128);
         if (elect_one()) mbar_arrive(v_clean);
       }
     }

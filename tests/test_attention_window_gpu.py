@@ -165,3 +165,21 @@ def test_entry_points_refuse_bad_arguments():
     assert fwd(docs=70000) == -1                                      # more tiles than a grid has rows
     assert _ext.lib().cb_attn_window_bwd(p, p, p, p, p, f.data_ptr(), cu.data_ptr(), 1, 128, 2, 1, 64, 256, 256, 256, 256, 256, 0.125, 0, 0,
                                          f.data_ptr(), f.data_ptr(), f.data_ptr(), f.data_ptr(), p, 256, st, _ext.stream_ptr()) == -1
+
+
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (32, 8, 64), (4, 2, 128)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -1e30])
+def test_documents_keep_to_themselves(hq, hk, d, value):
+    """Whatever the document in the middle and the padding behind the last one hold, the others' results are the same."""
+    lens, pad, window, sinks = [600, 70, 650], 50, 200, 3
+    qkv, do, cu = _inputs(hq, hk, d, lens, pad)
+    want = _truth(qkv, do, hq, hk, d, lens, window, sinks)
+    a, b, T = 600, 670, 1320
+    for t in (qkv, do):
+        t[a:b] = value
+        t[T:] = value
+    o, g = _run(qkv, do, cu, hq, hk, d, window, sinks)
+    assert (o[T:] == 0).all() and (g[T:] == 0).all()
+    for rows in (slice(0, a), slice(b, T)):
+        for x, y in ((o, want[0]), (g, want[1])):
+            assert torch.isfinite(x[rows]).all() and (x[rows].double() - y[rows]).norm() <= 2.0 ** -7 * y[rows].norm()
