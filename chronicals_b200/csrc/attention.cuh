@@ -22,6 +22,7 @@ struct AttnArgs {
   int o_tma;            // forward: a tensor map over O exists, whole blocks may leave by TMA store
   // windowed forms: a query sees the last `window` keys of its document, its own among them, and the document's first `sinks`
   int window, sinks;
+  bf16* o_lo;           // forward, [T, hq, D] without gaps or null: O less its rounding to bf16, rounded itself (for delta)
   int sink_run;         // backward: query blocks per CTA of a key block that holds sinks
 };
 

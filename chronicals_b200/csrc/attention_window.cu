@@ -312,6 +312,19 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         uint32_t w[16];
 #pragma unroll
         for (int q = 0; q < 16; ++q) w[q] = pack_bf16x2(__uint_as_float(o[2 * q]) * inv, __uint_as_float(o[2 * q + 1]) * inv);
+        if (a.o_lo != nullptr && row_ok) {
+          uint4* lo = reinterpret_cast<uint4*>(a.o_lo + (t * a.hq + h) * D + c * 32);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = unpack_bf16x2(w[4 * q + i]);
+              v[i] = pack_bf16x2(__uint_as_float(o[8 * q + 2 * i]) * inv - f.x, __uint_as_float(o[8 * q + 2 * i + 1]) * inv - f.y);
+            }
+            lo[q] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
         if (whole) {
           store_row_chunk32_packed(sQ, r, c, w);
         } else if (row_ok) {
@@ -371,11 +384,13 @@ extern "C" {
 
 // q [T, hq, D] (row pitch ldq elements), k / v [T, hk, D]; cu: int32 [n_docs + 1] on the device; window >= 1, sinks >= 0.
 // o [T, hq, D] with pitch ldo; lse [hq, T] fp32.  Rows of o at or beyond cu[n_docs] (padding) are written as zeros, their
-// lse entries are left untouched.  D is 64 or 128, hq a multiple of hk.
+// lse entries are left untouched.  o_lo (null: none), [T, hq, D] without gaps: what o's rounding left out, for the backward pass.
+// D is 64 or 128, hq a multiple of hk.
 int cb_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu, int n_docs, int T,
                        int hq, int hk, int D, long long ldq, long long ldk, long long ldv, long long ldo, float scale, int window,
-                       int sinks, int* status, void* stream) {
-  if ((D != 64 && D != 128) || hk <= 0 || hq % hk != 0 || T <= 0 || n_docs <= 0 || window < 1 || sinks < 0) return -1;
+                       int sinks, void* o_lo, int* status, void* stream) {
+  if ((D != 64 && D != 128) || hk <= 0 || hq % hk != 0 || T <= 0 || n_docs <= 0 || window < 1 || sinks < 0 ||
+      (reinterpret_cast<uintptr_t>(o_lo) & 15) != 0) return -1;
   const long long tiles = (T + 127LL) / 128 + n_docs;
   if (tiles > 65535) return -1;
   CUtensorMap mq, mk, mv, mo;
@@ -386,6 +401,7 @@ int cb_attn_window_fwd(const void* q, const void* k, const void* v, void* o, flo
   cb::AttnArgs a = {};
   a.T = T; a.hq = hq; a.hk = hk; a.n_docs = n_docs; a.cu = cu; a.scale = scale;
   a.O = static_cast<cb::bf16*>(o); a.ldo = ldo; a.lse = lse; a.status = status;
+  a.o_lo = static_cast<cb::bf16*>(o_lo);
   a.window = std::min(window, T); a.sinks = std::min(sinks, T);
   a.o_tma = cbhost::make_tmap(&mo, o, static_cast<unsigned long long>(hq) * D, T, ldo, 64, 128) == 0 ? 1 : 0;
   if (!a.o_tma) mo = mq;                                // O is not TMA-addressable: every block stores row by row

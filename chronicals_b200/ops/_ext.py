@@ -60,8 +60,8 @@ _PROTOTYPES = {
     "cb_kd_place": [P, L, I, I, I, I, P, L, I, P, L, I, I, F, P, P, P, P],
     "cb_attn_fwd": [P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, P, P],
     "cb_attn_bwd": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, F, P, P, P, P, P, L, P, P, I],
-    "cb_attn_window_fwd": [P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, I, I, P, P],
-    "cb_attn_window_bwd": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, F, I, I, P, P, P, P, P, L, P, P],
+    "cb_attn_window_fwd": [P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, I, I, P, P, P],
+    "cb_attn_window_bwd": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, F, I, I, P, P, P, P, P, P, L, P, P],
     "cb_gemm2sm_bf16": [P, P, P, P, P, I, I, I, L, L, L, L, I, I, I, I, P, P],
     "cb_gemm2sm_supported": [P, L, I],
     "cb_gemm2sm_bf16_ex": [P, P, P, P, P, I, I, I, L, L, L, L, I, I, I, I, I, P, P],

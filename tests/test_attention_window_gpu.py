@@ -160,10 +160,10 @@ def test_entry_points_refuse_bad_arguments():
 
     def fwd(T=128, docs=1, hq=2, hk=1, d=64, window=4, sinks=0):
         return _ext.lib().cb_attn_window_fwd(p, p, p, p, f.data_ptr(), cu.data_ptr(), docs, T, hq, hk, d, 256, 256, 256, 256, 0.125, window,
-                                             sinks, st, _ext.stream_ptr())
+                                             sinks, None, st, _ext.stream_ptr())
     assert fwd(T=0) == fwd(docs=0) == fwd(hk=0) == fwd(hq=3, hk=2) == fwd(d=80) == fwd(window=0) == fwd(sinks=-1) == -1
     assert fwd(docs=70000) == -1                                      # more tiles than a grid has rows
-    assert _ext.lib().cb_attn_window_bwd(p, p, p, p, p, f.data_ptr(), cu.data_ptr(), 1, 128, 2, 1, 64, 256, 256, 256, 256, 256, 0.125, 0, 0,
+    assert _ext.lib().cb_attn_window_bwd(p, p, p, p, p, f.data_ptr(), cu.data_ptr(), 1, 128, 2, 1, 64, 256, 256, 256, 256, 256, 0.125, 0, 0, None,
                                          f.data_ptr(), f.data_ptr(), f.data_ptr(), f.data_ptr(), p, 256, st, _ext.stream_ptr()) == -1
 
 
