@@ -2096,11 +2096,14 @@ int attn_bwd(const void* q, const void* k, const void* v, const void* o, const v
   a.lse = const_cast<float*>(lse); a.delta = delta; a.dq_acc = dq_acc; a.dk_part = dk_part; a.dv_part = dv_part;
   a.status = status;
   dim3 grid(hq, (T + 127) / 128 + n_docs);            // x: query head (fastest, the heads of a group share K/V in L2); y: tile by descending weight
+  const long long tile_heads = static_cast<long long>(hq) * ((T + 127) / 128);
   if (window > 0) {
     a.window = std::min(window, T);
     a.sinks = std::min(sinks, T);
-    // runs as long as the loop of a key block without sinks, and no shorter than 8: a CTA of less is mostly set-up
-    a.sink_run = std::max(8, (a.window + 127) / 128 + 1);
+    // Runs as long as the loop of a key block without sinks, and no shorter than 6, since a CTA of less is mostly set-up (14 heads of
+    // 64, 8192 tokens, window 128: runs of 2 / 4 / 6 / 8 blocks 91 / 81 / 76 / 79 us), or than 3 where the grid leaves SMs free
+    // (1024 tokens: 18 / 16 / 20 / 24, of 3 14).
+    a.sink_run = std::max(tile_heads <= cbhost::num_sms() ? 3 : 6, (a.window + 127) / 128 + 1);
     const long long tiles = (T + 127LL) / 128 + n_docs;
     const long long all = tiles + (a.sinks + 127LL) / 128 * (tiles / a.sink_run + n_docs);
     if (all > 65535) return -1;
@@ -2110,9 +2113,11 @@ int attn_bwd(const void* q, const void* k, const void* v, const void* o, const v
   // wins where the grid does not fill the SMs twice over (1 x 2048 tokens, 14 heads: 44 against 80 us; 4 x 512: 23 / 26)
   // or its loops are long (2 x 4096: 276 / 290; 4 x 2048, 32 heads: 403 / 350, so no earlier than 4096), unless the
   // documents are so short that a CTA is mostly set-up (20 x 100: 19 / 15).  Lengths as the average over the documents.
-  const bool few = static_cast<long long>(hq) * ((T + 127) / 128) <= 2LL * cbhost::num_sms() && T >= 512LL * n_docs;
-  const bool short_loops = window > 0 ? std::min<long long>(2LL * window, T / n_docs) < 4096 : T < 4096LL * n_docs;
-  if (D == 64 && !few && short_loops) {
+  // With a window the loops are about as long for every document: only the grid decides (14 heads of 64: 2048 tokens, window 16
+  // and sinks 42 / 24 us, window 1024 47 / 40; 8192 tokens, window 128 / 1024 / 4096 79 / 87, 177 / 171, 364 / 362; 32 heads,
+  // 16,384 tokens, window 4096 1806 / 1895).
+  const bool few = tile_heads <= 2LL * cbhost::num_sms() && (window > 0 || T >= 512LL * n_docs);
+  if (D == 64 && !few && (window > 0 || T < 4096LL * n_docs)) {
     e = window > 0 ? launch_bwd2<64, true>(grid, s, mq, mk, mv, mdo, mdq, a) : launch_bwd2<64, false>(grid, s, mq, mk, mv, mdo, mdq, a);
     if (e) return e;
   } else {
