@@ -81,6 +81,8 @@ struct GemmArgs {
   // K range; partial tiles are added into a zero-initialised fp32 C with red.global.add
   int items_per_ksplit;           // 0: no split
   int kb_per_split;
+  int slab_rows;                  // > 0: every K range has an output of its own, slab_rows rows further down in C, which it
+  int slab_add;                   // ... is written to, or (1) added to: one sum an element and launch, in a fixed order
 };
 
 template <int BLOCK_N, int STAGES>
@@ -437,7 +439,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             CB_DEBUG_CHECK_ST(g.status, colbase >= 0 && row0w >= 0 && (colbase * (g.out_fp32 ? 4 : 2)) % 16 == 0,
                               CB_DBG_TMA_COORD, colbase);
             if (lane == 0 && row0w < g.M) {          // a box that starts past the last row has nothing to write
-              if (g.items_per_ksplit > 0) tma_reduce_add_2d(&tmC, stg + buf * 4096, colbase, row0w);   // split K: sum the ranges
+              const int slab = g.slab_rows > 0 ? item0 / g.items_per_ksplit * g.slab_rows : 0;
+              if (g.items_per_ksplit > 0 && (g.slab_rows == 0 || g.slab_add))
+                tma_reduce_add_2d(&tmC, stg + buf * 4096, colbase, slab + row0w);                      // split K: sum the ranges
+              else if (slab > 0) tma_store_2d(&tmC, stg + buf * 4096, colbase, slab + row0w);
               else tma_store_2d(&tmC, stg + buf * 4096, colbase, row0w);
               tma_store_commit();
             }
@@ -654,6 +659,20 @@ cce_combine_rows_kernel(const float* __restrict__ part_m, const float* __restric
   if (smoothing != 0.f) loss = (1.f - smoothing) * loss + smoothing * (lse - sl / static_cast<float>(V_total));
   loss += z_weight * lse * lse;
   loss_rows[row] = valid ? loss : 0.f;
+}
+
+// out[m, n] = sum over the slabs of a product that was cut along K, in their order.  slab: elements from one to the next.
+__global__ void __launch_bounds__(256)
+slab_sum_kernel(const float* __restrict__ slabs, bf16* __restrict__ out, int n_slabs, long long slab, long long n4) {
+  const long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
+  if (i >= n4) return;
+  float4 a = reinterpret_cast<const float4*>(slabs)[i];
+#pragma unroll 4
+  for (int s = 1; s < n_slabs; ++s) {
+    const float4 b = reinterpret_cast<const float4*>(slabs + s * slab)[i];
+    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+  }
+  reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
 }
 
 // Single block: deterministic sum of per-row losses and the valid count; writes
@@ -973,6 +992,72 @@ int cb_gemm_bf16_tp(const void* A, const void* B, void* C, const void* bias, int
     if (e) return e;
   }
   return dispatch<cb::EPI_STORE>(bn, a_mn, b_mn, ta, tb, tc, g, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
+extern "C" {
+
+// How many K ranges (slabs) pay for a product [M, N] over K in one launch of 128 x 128 tiles, each with an fp32 output of its own;
+// 1: none, the plain product is estimated faster.  Few output tiles leave SMs idle: d(hidden) of a loss over a vocabulary has a
+// handful of tiles and the longest K there is.  Estimated as in choose_kernel, with the slabs' way through memory; up to 96.
+int cb_gemm_slabs(int M, int N, int K, int a_mn, int b_mn, int sms) {
+  if (M <= 0 || N <= 0 || K <= 0 || sms < 2) return 1;
+  const long long tiles = static_cast<long long>((M + 127) / 128) * ((N + 127) / 128), kb = (K + 63) / 64;
+  double best_us = 0.0;
+  choose_kernel(M, N, K, a_mn, b_mn, 4, true, sms, &best_us);
+  best_us *= 0.92;                                          // how far the estimates are off
+  int best = 1;
+  for (int n = 2; n <= 96 && n <= kb; ++n) {
+    const long long per = (kb + n - 1) / n, used = (kb + per - 1) / per;
+    if (used != n) continue;
+    const double us = 4.34 + 2.0 + static_cast<double>((tiles * n + sms - 1) / sms) * (0.28 * per + 1.0) + 1e-6 * M * N * (8.0 * n + 2.0) / 5.0;
+    if (us < best_us) {
+      best_us = us;
+      best = n;
+    }
+  }
+  return best;
+}
+
+// C [n_slabs, ceil(M / 128) * 128, N] fp32 without gaps: the product over the i-th K range in slab i (add: added to it).  A shorter K
+// than cb_gemm_slabs was asked about reaches the first slabs only, so the longest comes first (add = 0 has to reach all).
+int cb_gemm_bf16_slabs(const void* A, const void* B, float* C, int M, int N, int K, long long lda, long long ldb, int a_mn, int b_mn,
+                       int n_slabs, int add, int* status, void* stream) {
+  if (M <= 0 || N <= 0 || N % 4 != 0 || K <= 0 || n_slabs < 1 || (reinterpret_cast<uintptr_t>(C) & 15) != 0) return -1;
+  const int bn = 128;
+  CUtensorMap ta, tb, tc;
+  int e = build_maps(&ta, &tb, A, B, M, N, K, lda, ldb, a_mn, b_mn, bn);
+  if (e) return e;
+  cb::GemmArgs g = {};
+  g.M = M; g.N = N; g.K = K;
+  g.num_m_blocks = (M + 127) / 128;
+  g.num_n_tiles = (N + bn - 1) / bn;
+  g.tiles_per_item = 1;
+  const int num_kb = (K + 63) / 64;
+  g.kb_per_split = (num_kb + n_slabs - 1) / n_slabs;
+  const int used = (num_kb + g.kb_per_split - 1) / g.kb_per_split;
+  if (!add && used != n_slabs) return -1;                   // a slab would stay unwritten
+  g.items_per_ksplit = g.num_m_blocks * g.num_n_tiles;
+  if (static_cast<long long>(g.items_per_ksplit) * used > 0x7fffffffLL) return -1;
+  g.num_items = g.items_per_ksplit * used;
+  g.slab_rows = g.num_m_blocks * 128;
+  g.slab_add = add ? 1 : 0;
+  g.C = C; g.ldc = N; g.out_fp32 = 1; g.tma_store = 1;
+  e = cbhost::make_tmap(&tc, C, N, static_cast<unsigned long long>(g.slab_rows) * n_slabs, N, 32, 32, 4);
+  if (e) return e;
+  g.status = status;
+  return dispatch<cb::EPI_STORE>(bn, a_mn, b_mn, ta, tb, tc, g, static_cast<cudaStream_t>(stream));
+}
+
+// out [M, N] bf16 without gaps = the sum of the slabs
+int cb_slab_sum(const float* slabs, void* out, int M, int N, int n_slabs, void* stream) {
+  if (M <= 0 || N <= 0 || N % 4 != 0 || n_slabs < 1) return -1;
+  const long long n4 = static_cast<long long>(M) * N / 4, blocks = (n4 + 255) / 256;
+  if (blocks > 0x7fffffffLL) return -1;
+  cb::slab_sum_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      slabs, static_cast<cb::bf16*>(out), n_slabs, static_cast<long long>((M + 127) / 128 * 128) * N, n4);
+  return static_cast<int>(cudaGetLastError());
 }
 
 }  // extern "C"

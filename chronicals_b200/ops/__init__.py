@@ -1181,8 +1181,14 @@ class _LinearDistillFn(torch.autograd.Function):
         need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         Vc = _cce_chunk(M, K, V, _sm_count(dev))
         G = torch.empty(M, Vc, dtype=torch.bfloat16, device=dev)
-        # sums over several chunks stay in fp32; one chunk is rounded where it is computed
-        dh = torch.empty(M, K, dtype=torch.float32 if Vc < V else hidden.dtype, device=dev) if need_dh else None
+        # Sums over several chunks stay in fp32; one chunk is rounded where it is computed.  Few tokens make few tiles of dH with the
+        # whole vocabulary to sum over: ranges of it go to slabs of their own, which are added up at the end.
+        slabs = _ext.lib().cb_gemm_slabs(M, K, min(Vc, V), 0, 1, _sm_count(dev)) if need_dh else 1
+        dh = parts = None
+        if slabs > 1:
+            parts = torch.empty(slabs, -(-M // 128) * 128, K, dtype=torch.float32, device=dev)
+        elif need_dh:
+            dh = torch.empty(M, K, dtype=torch.float32 if Vc < V else hidden.dtype, device=dev)
         dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_dw else None
         for c0 in range(0, V, Vc):
             vc = min(Vc, V - c0)
@@ -1195,10 +1201,17 @@ class _LinearDistillFn(torch.autograd.Function):
                                  gscale.data_ptr(), g1.data_ptr(), _ext.stream_ptr())
             _ext.check(code, "kd_place")
             Gc = G[:, :vc]
-            if need_dh:   # dH += G_c @ W_c
+            if slabs > 1:
+                code = L.cb_gemm_bf16_slabs(Gc.data_ptr(), wc.data_ptr(), parts.data_ptr(), M, K, vc, Gc.stride(0), wc.stride(0), 0, 1,
+                                            slabs, int(c0 > 0), status.data_ptr(), _ext.stream_ptr())
+                _ext.check(code, "gemm_bf16_slabs")
+            elif need_dh:   # dH += G_c @ W_c
                 gemm(Gc, wc, b_mn=True, out=dh, accumulate=c0 > 0)
             if need_dw:   # dW_c = G_c^T @ H
                 gemm(Gc, hidden, a_mn=True, b_mn=True, out=dw[c0:c0 + vc])
+        if slabs > 1:
+            dh = torch.empty(M, K, dtype=hidden.dtype, device=dev)
+            _ext.check(L.cb_slab_sum(parts.data_ptr(), dh.data_ptr(), M, K, slabs, _ext.stream_ptr()), "slab_sum")
         return dh.to(hidden.dtype) if need_dh else None, dw, None, None, None, None, None, None
 
 

@@ -53,6 +53,9 @@ _PROTOTYPES = {
     "cb_ce_logits_grad": [P, P, P, P, P, P, L, L, L, I, I, L, F, F, P],
     "cb_cce_forward_t": [P, P, P, I, I, I, L, L, I, F, P, P, P, P, P, P],
     "cb_cce_dlogits_t": [P, P, P, P, P, P, P, I, I, I, L, L, L, I, I, F, F, F, P, P],
+    "cb_gemm_slabs": [I, I, I, I, I, I],
+    "cb_gemm_bf16_slabs": [P, P, P, I, I, I, L, L, I, I, I, I, P, P],
+    "cb_slab_sum": [P, P, I, I, I, P],
     "cb_kd_max_entries": [],
     "cb_kd_logits": [P, L, L, I, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P],
     "cb_kd_logits_grad": [P, P, L, L, L, I, I, P, L, I, P, L, I, I, P, L, F, P, P, P, P, P, P],
@@ -158,7 +161,7 @@ def lib() -> ctypes.CDLL:
 # device kernels launched by one call of each entry point (0: host-only query)
 _KERNELS_PER_CALL = {"cb_gemm2sm_supported": 0, "cb_gemm2sm_cost_ns": 0, "cb_gemm_choice": 0, "cb_glu_bwd_fused_pays": 0, "cb_cce_chunk": 0, "cb_cce_num_splits": 0, "cb_rmsnorm_max_n": 0, "cb_rmsnorm_bwd_blocks": 0, "cb_opt_chunk": 0,
                      "cb_embedding_rank_max": 0, "cb_embedding_part_rows": 0, "cb_embedding_bwd": 2, "cb_cce_combine": 2, "cb_rmsnorm_bwd": 2, "cb_grad_clip_coef": 2, "cb_attn_bwd": 3, "cb_attn_window_bwd": 3,
-                     "cb_kd_max_entries": 0, "cb_kd_logits": 2, "cb_kd_linear_rows": 2}
+                     "cb_gemm_slabs": 0, "cb_kd_max_entries": 0, "cb_kd_logits": 2, "cb_kd_linear_rows": 2}
 LAUNCH_COUNT = [0]
 
 

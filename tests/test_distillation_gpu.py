@@ -272,3 +272,41 @@ def test_more_entries_than_the_kernels_take_follow_the_formula():
     loss = ops.distillation_logits(z, idx, lg)
     short = ops.distillation_logits(z, idx[:, :-1], lg[:, :-1].masked_fill(idx[:, :-1] == 0, NEG))
     assert math.isfinite(loss.item()) and math.isfinite(short.item()) and abs(loss.item() - short.item()) < 0.1
+
+
+@pytest.mark.parametrize("M,N,K,n", [(1, 64, 4096, 7), (120, 256, 5000, 13), (129, 72, 640, 3), (300, 896, 1000, 16), (5, 8, 64, 1)])
+def test_product_in_slabs(M, N, K, n):
+    """Ranges of the inner dimension in slabs of their own, a second product over a shorter one added, summed in order."""
+    g = torch.Generator(device=DEV).manual_seed(M + K)
+    L, S = _ext.lib(), _ext.status_buffer(torch.device("cuda", torch.cuda.current_device())).data_ptr()
+    slabs = torch.full((n, -(-M // 128) * 128, N), math.nan, device=DEV)
+    out = torch.full((M, N), math.nan, dtype=BF, device=DEV)
+    want = torch.zeros(M, N, dtype=torch.float64, device=DEV)
+    size = torch.zeros_like(want)
+    for add, k in ((0, K), (1, K), (1, max(8, K // 3 // 8 * 8))):
+        a, b = (torch.randn(*s, device=DEV, generator=g).to(BF) for s in ((M, -(-k // 8) * 8), (k, N)))
+        code = L.cb_gemm_bf16_slabs(a.data_ptr(), b.data_ptr(), slabs.data_ptr(), M, N, k, a.stride(0), N, 0, 1, n, add, S, _ext.stream_ptr())
+        per = -(-(-(-k // 64)) // n)
+        if not add and -(-(-(-k // 64)) // per) != n:                 # blocks of 64 that leave a slab without any are refused
+            assert code == -1
+            return
+        assert code == 0
+        want += a[:, :k].double() @ b.double()
+        size += a[:, :k].double().abs() @ b.double().abs()
+    assert L.cb_slab_sum(slabs.data_ptr(), out.data_ptr(), M, N, n, _ext.stream_ptr()) == 0
+    _ext.check_status()
+    # the sums in 32 bits, a few roundings of the sum of sizes (n slabs of at least 64 products in one accumulator); then half a step
+    assert _over(out.double() - want, torch.finfo(BF).eps / 2 * want.abs() + 2.0 ** -20 * size + 1e-12) == 0
+
+
+def test_slabs_only_where_tiles_are_few():
+    L = _ext.lib()
+    assert L.cb_gemm_slabs(120, 256, 32000, 0, 1, 148) > 8 and L.cb_gemm_slabs(8192, 896, 8192, 0, 1, 148) == 1
+    for M in (1, 100, 500, 1021, 3000):
+        for K in (64, 1000, 32000, 151936):
+            n = L.cb_gemm_slabs(M, 896, K, 0, 1, 148)
+            per = -(-(-(-K // 64)) // n)
+            assert 1 <= n <= 96 and -(-(-(-K // 64)) // per) == n    # every slab of the first product is written
+    assert L.cb_gemm_bf16_slabs(None, None, None, 0, 8, 8, 8, 8, 0, 1, 1, 0, None, None) == -1
+    assert L.cb_gemm_bf16_slabs(None, None, None, 8, 6, 8, 8, 8, 0, 1, 1, 0, None, None) == -1
+    assert L.cb_slab_sum(None, None, 8, 6, 1, None) == -1
