@@ -304,11 +304,11 @@ kd_logits_grad_kernel(const T* __restrict__ logits, T* __restrict__ dlogits, lon
   }
 }
 
-// out[0] = mean (or sum) of the rows' losses, out[1] = rows that take part; with gscale also the factor of each row's
+// loss = mean (or sum) of the rows' losses, n_rows = rows that take part; with gscale also the factor of each row's
 // d(logits), tau / n, tau or 0.  stats.y == -1 marks the rows that take no part.  One block, a fixed order.
 __global__ void __launch_bounds__(1024)
 kd_finalize_kernel(const float* __restrict__ loss_rows, const float2* __restrict__ stats, long long rows, int mean, float tau,
-                   float* __restrict__ out, float* __restrict__ gscale) {
+                   float* __restrict__ loss, float* __restrict__ n_rows, float* __restrict__ gscale) {
   __shared__ float red[32];
   float sum = 0.f, cnt = 0.f;
   for (long long i = threadIdx.x; i < rows; i += blockDim.x) {
@@ -320,8 +320,8 @@ kd_finalize_kernel(const float* __restrict__ loss_rows, const float2* __restrict
   cnt = kd_block_sum(cnt, red);
   const float n = mean ? fmaxf(cnt, 1.f) : 1.f;
   if (threadIdx.x == 0) {
-    out[0] = sum / n;
-    out[1] = cnt;
+    loss[0] = sum / n;
+    n_rows[0] = cnt;
   }
   if (gscale != nullptr)
     for (long long i = threadIdx.x; i < rows; i += blockDim.x) gscale[i] = stats[i].y == -1.f ? 0.f : tau / n;
@@ -459,10 +459,10 @@ extern "C" {
 
 int cb_kd_max_entries() { return cb::KD_MAX_K; }
 
-// Held logits: stats [rows, 2], q [rows, K], loss_rows [rows], out [2] = mean (or sum) of the losses, rows that take part.
+// Held logits: stats [rows, 2], q [rows, K], loss_rows [rows]; loss: their mean (or sum), n_rows: the rows that take part.
 int cb_kd_logits(const void* logits, long long rows, long long ld, int V, int is_bf16, const void* idx, long long ld_idx, int idx64,
                  const void* lg, long long ld_lg, int lg_bf16, int K, const long long* labels, long long ignore_index, float tau,
-                 int mean, float* stats, float* q, float* loss_rows, float* out, void* stream) {
+                 int mean, float* stats, float* q, float* loss_rows, float* loss, float* n_rows, void* stream) {
   cb::KdTeacher t;
   if (rows <= 0 || rows > 0x7fffffffLL || V <= 0 || !kd_teacher(&t, idx, ld_idx, idx64, lg, ld_lg, lg_bf16, K, labels, ignore_index, tau))
     return -1;
@@ -486,7 +486,7 @@ int cb_kd_logits(const void* logits, long long rows, long long ld, int V, int is
                                 : cudaLaunchKernelEx(&cfg, cb::kd_logits_kernel<float>, static_cast<const float*>(logits), ld, V, t, c2,
                                                      st, q, loss_rows);
   if (e != cudaSuccess) return static_cast<int>(e);
-  cb::kd_finalize_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(loss_rows, st, rows, mean, tau, out, nullptr);
+  cb::kd_finalize_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(loss_rows, st, rows, mean, tau, loss, n_rows, nullptr);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -513,11 +513,11 @@ int cb_kd_logits_grad(const void* logits, void* dlogits, long long rows, long lo
 }
 
 // From hidden states, after cb_cce_forward_t: part_m / part_s [n_splits, M].  lse, loss_rows, gscale [M], stats [M, 2], coef [M, K],
-// out [2] as above.
+// loss and n_rows as above.
 int cb_kd_linear_rows(const void* hidden, long long ldh, const void* weight, long long ldw, int H, int V, int M, const float* part_m,
                       const float* part_s, int n_splits, const void* idx, long long ld_idx, int idx64, const void* lg, long long ld_lg,
                       int lg_bf16, int K, const long long* labels, long long ignore_index, float tau, int mean, float* lse,
-                      float* stats, float* coef, float* loss_rows, float* out, float* gscale, void* stream) {
+                      float* stats, float* coef, float* loss_rows, float* loss, float* n_rows, float* gscale, void* stream) {
   cb::KdTeacher t;
   if (M <= 0 || V <= 0 || H <= 0 || H % 8 != 0 || ldh % 8 != 0 || ldw % 8 != 0 ||
       ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15) != 0 ||
@@ -532,7 +532,7 @@ int cb_kd_linear_rows(const void* hidden, long long ldh, const void* weight, lon
       static_cast<const cb::bf16*>(hidden), ldh, static_cast<const cb::bf16*>(weight), ldw, H, V, M, part_m, part_s, n_splits, t,
       kd_scale(tau), lse, st, coef, loss_rows);
   CB_CHECK_CUDA(cudaGetLastError());
-  cb::kd_finalize_kernel<<<1, 1024, 0, s>>>(loss_rows, st, M, mean, tau, out, gscale);
+  cb::kd_finalize_kernel<<<1, 1024, 0, s>>>(loss_rows, st, M, mean, tau, loss, n_rows, gscale);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -630,12 +630,16 @@ def qk_rope_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, position_i
 
 def _same_device(op: str, *tensors: Optional[torch.Tensor]) -> None:
     """Kernels run on the current device's stream: refuses tensors of several devices, or of one that is not current."""
-    devs = {t.device for t in tensors if t is not None}
-    if len(devs) > 1:
-        raise ValueError(f"{op}: tensors on several devices: {sorted(map(str, devs))}")
-    for d in devs:
-        if d.type == "cuda" and d.index != torch.cuda.current_device():
-            raise ValueError(f"{op}: tensors on {d}, but the current device is cuda:{torch.cuda.current_device()}")
+    index = -2
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()                         # -1: not on a GPU
+            if index == -2:
+                index = i
+            elif i != index:
+                raise ValueError(f"{op}: tensors on several devices: {sorted({str(x.device) for x in tensors if x is not None})}")
+    if index >= 0 and index != torch.cuda.current_device():
+        raise ValueError(f"{op}: tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
 
 
 @functools.lru_cache(maxsize=64)
@@ -707,8 +711,11 @@ def qk_rope_axes_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
         pos = position_ids.long()
         if pos.stride(1) != 1:
             pos = pos.contiguous()
-        return _QKRopeAxesFn.apply(qkv, cos.float().contiguous(), sin.float().contiguous(), pos,
-                                   (num_q_heads, num_kv_heads, head_dim, sections, bool(cyclic), bool(interleaved), bool(inverse)))
+        cos, sin = cos.float().contiguous(), sin.float().contiguous()
+        cfg = (num_q_heads, num_kv_heads, head_dim, sections, bool(cyclic), bool(interleaved), bool(inverse))
+        if torch.is_grad_enabled() and qkv.requires_grad:
+            return _QKRopeAxesFn.apply(qkv, cos, sin, pos, cfg)
+        return _rope_axes_launch(qkv, qkv, cos, sin, pos, *cfg)
     T, nqk = qkv.shape[0], (num_q_heads + num_kv_heads) * head_dim
     c, s = ref.rope_axes_tables(cos, sin, position_ids, ref.rope_axis_map(sections, cyclic))
     y = ref.apply_rope(qkv[:, :nqk].reshape(T, -1, head_dim), c, s, None, interleaved, inverse)
@@ -1062,13 +1069,18 @@ def _distill_args(op, lead, V, idx, lg, temperature, labels, reduction, *others)
     if V < 1:
         raise ValueError(f"{op}: the vocabulary is empty")
     _same_device(op, idx, lg, labels, *others)
-    idx, lg = idx.reshape(-1, K), lg.detach().reshape(-1, K)
+    lg = lg.detach() if lg.requires_grad else lg
+    if idx.dim() != 2:
+        idx, lg = idx.reshape(-1, K), lg.reshape(-1, K)
     if idx.dtype not in (torch.int64, torch.int32):
         idx = idx.long()
     if lg.dtype not in (torch.float32, torch.bfloat16, torch.float64):
         lg = lg.float()
-    idx, lg = (t if t.stride(1) == 1 else t.contiguous() for t in (idx, lg))
-    return idx, lg, None if labels is None else labels.reshape(-1).long().contiguous()
+    idx = idx if idx.stride(1) == 1 else idx.contiguous()
+    lg = lg if lg.stride(1) == 1 else lg.contiguous()
+    if labels is not None and not (labels.dim() == 1 and labels.dtype == torch.int64 and labels.is_contiguous()):
+        labels = labels.reshape(-1).long().contiguous()
+    return idx, lg, labels
 
 
 def _teacher_ptrs(idx, lg):
@@ -1077,37 +1089,46 @@ def _teacher_ptrs(idx, lg):
 
 
 class _DistillLogitsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, idx, lg, labels, ignore_index, tau, mean):
-        rows, V = logits.shape
-        f32 = dict(dtype=torch.float32, device=logits.device)
-        stats, q = torch.empty(rows, 2, **f32), torch.empty(rows, idx.shape[1], **f32)
-        loss_rows, out = torch.empty(rows, **f32), torch.empty(2, **f32)
-        code = _ext.lib().cb_kd_logits(logits.data_ptr(), rows, logits.stride(0), V, int(logits.dtype == torch.bfloat16),
-                                       *_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau, int(mean), stats.data_ptr(),
-                                       q.data_ptr(), loss_rows.data_ptr(), out.data_ptr(), _ext.stream_ptr())
-        _ext.check(code, "kd_logits")
-        ctx.save_for_backward(logits, idx, lg, labels, stats, q, out)
-        ctx.cfg = (ignore_index, tau, mean)
-        ctx.set_materialize_grads(False)
-        return out[0], loss_rows
+    """``reduction``: the loss, reduced, or of every row.  Everything kept for the backward pass is in one buffer: stats [rows, 2], the
+    number of rows that take part, a place for the other reduction's loss, and the merged teacher probabilities [rows, K]."""
 
     @staticmethod
-    def backward(ctx, gout, grows):
-        logits, idx, lg, labels, stats, q, out = ctx.saved_tensors
-        ignore_index, tau, mean = ctx.cfg
+    def forward(ctx, logits, idx, lg, labels, ignore_index, tau, reduction):
+        rows, V = logits.shape
+        each = reduction == "none"
+        buf = torch.empty(rows * (2 + idx.shape[1]) + 1 + (1 if each else rows), dtype=torch.float32, device=logits.device)
+        loss = torch.empty((rows,) if each else (), dtype=torch.float32, device=logits.device)
+        stats = buf.data_ptr()
+        n, other, q = stats + 8 * rows, stats + 8 * rows + 4, stats + 8 * rows + (8 if each else 4 + 4 * rows)
+        code = _ext.lib().cb_kd_logits(logits.data_ptr(), rows, logits.stride(0), V, int(logits.dtype == torch.bfloat16),
+                                       *_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau, int(reduction == "mean"), stats, q,
+                                       loss.data_ptr() if each else other, other if each else loss.data_ptr(), n, _ext.stream_ptr())
+        _ext.check(code, "kd_logits")
+        ctx.save_for_backward(logits, idx, lg, labels, buf)
+        ctx.cfg = (ignore_index, tau, reduction)
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        logits, idx, lg, labels, buf = ctx.saved_tensors
+        ignore_index, tau, reduction = ctx.cfg
         rows, V = logits.shape
         ld = logits.stride(0)
         # rows as far apart as the logits', so that both start at the same distance from a 16-byte boundary
         dl = torch.empty_strided((rows, V), (ld, 1) if V <= ld < 2 * V else (V, 1), dtype=logits.dtype, device=logits.device)
-        gout = None if gout is None else gout.float()
-        grows = None if grows is None else grows.float().contiguous()
+        grad = grad if grad.dtype == torch.float32 and grad.is_contiguous() else grad.float().contiguous()
+        each = reduction == "none"
+        stats, g = buf.data_ptr(), grad.data_ptr()
+        n, q = stats + 8 * rows, stats + 8 * rows + (8 if each else 4 + 4 * rows)
         code = _ext.lib().cb_kd_logits_grad(logits.data_ptr(), dl.data_ptr(), rows, ld, dl.stride(0), V,
                                             int(logits.dtype == torch.bfloat16), *_teacher_ptrs(idx, lg), _ext.ptr(labels),
-                                            ignore_index, tau, stats.data_ptr(), q.data_ptr(), _ext.ptr(gout),
-                                            out[1].data_ptr() if mean else None, _ext.ptr(grows), _ext.stream_ptr())
+                                            ignore_index, tau, stats, q, None if each else g,
+                                            n if reduction == "mean" else None, g if each else None, _ext.stream_ptr())
         _ext.check(code, "kd_logits_grad")
         return dl, None, None, None, None, None, None
+
+
+_KD_MAX_ENTRIES = 4096               # entries a row that the kernels take (KD_MAX_K in csrc/distill.cu)
 
 
 def distillation_logits(logits: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor, temperature: float = 1.0,
@@ -1122,12 +1143,12 @@ def distillation_logits(logits: torch.Tensor, teacher_indices: torch.Tensor, tea
     V = logits.shape[-1]
     idx, lg, y = _distill_args("distillation_logits", logits.shape[:-1], V, teacher_indices, teacher_logits, temperature, labels,
                                reduction, logits)
-    z = logits.reshape(-1, V)
+    z = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if (z.is_cuda and not _ext.reference_forced() and z.dtype in (torch.bfloat16, torch.float32) and z.stride(1) == 1 and z.shape[0]
-            and idx.shape[1] <= _ext.lib().cb_kd_max_entries()):
+            and idx.shape[1] <= _KD_MAX_ENTRIES):
         lg = lg.float() if lg.dtype == torch.float64 else lg
-        loss, rows = _DistillLogitsFn.apply(z, idx, lg, y, ignore_index, float(temperature), reduction == "mean")
-        return rows.view(logits.shape[:-1]) if reduction == "none" else loss
+        loss = _DistillLogitsFn.apply(z, idx, lg, y, ignore_index, float(temperature), reduction)
+        return loss.view(logits.shape[:-1]) if reduction == "none" else loss
     rows, valid = ref.distillation_rows(z, idx, lg, float(temperature), y, ignore_index)
     return ref.reduce_rows(rows.view(logits.shape[:-1]), valid, reduction)
 
@@ -1138,46 +1159,49 @@ class _LinearDistillFn(torch.autograd.Function):
     the product's epilogue and the teacher's words over it."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, idx, lg, labels, ignore_index, tau, mean):
+    def forward(ctx, hidden, weight, idx, lg, labels, ignore_index, tau, reduction):
         L = _ext.lib()
         M, K = hidden.shape
         V = weight.shape[0]
         dev = hidden.device
-        f32 = dict(dtype=torch.float32, device=dev)
         n_splits = L.cb_cce_num_splits(M, V)
-        part = torch.empty(2, n_splits, M, **f32)
+        part = torch.empty(2 * n_splits * M, dtype=torch.float32, device=dev)
+        p0 = part.data_ptr()
+        p1 = p0 + 4 * n_splits * M
         code = L.cb_cce_forward_t(hidden.data_ptr(), weight.data_ptr(), None, M, V, K, hidden.stride(0), weight.stride(0), 0,
-                                  math.log2(math.e) / tau, part[0].data_ptr(), part[1].data_ptr(), None, None,
-                                  _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr())
+                                  math.log2(math.e) / tau, p0, p1, None, None, _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr())
         _ext.check(code, "cce_forward_t")
-        lse, loss_rows, gscale = torch.empty(3, M, **f32)
-        stats, coef, out = torch.empty(M, 2, **f32), torch.empty(M, idx.shape[1], **f32), torch.empty(2, **f32)
-        code = L.cb_kd_linear_rows(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), K, V, M,
-                                   part[0].data_ptr(), part[1].data_ptr(), n_splits, *_teacher_ptrs(idx, lg), _ext.ptr(labels),
-                                   ignore_index, tau, int(mean), lse.data_ptr(), stats.data_ptr(), coef.data_ptr(),
-                                   loss_rows.data_ptr(), out.data_ptr(), gscale.data_ptr(), _ext.stream_ptr())
+        # stats [M, 2], losses, log-sum-exps and factors of the rows [M] each, p - q at the teacher's words [M, K]; the number of rows
+        buf = torch.empty(1 + M * (5 + idx.shape[1]), dtype=torch.float32, device=dev)
+        each = reduction == "none"
+        loss = torch.empty((M,) if each else (), dtype=torch.float32, device=dev)
+        stats = buf.data_ptr()
+        rows, n = stats + 8 * M, stats + 4 * (buf.numel() - 1)
+        code = L.cb_kd_linear_rows(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), K, V, M, p0, p1, n_splits,
+                                   *_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau, int(reduction == "mean"),
+                                   stats + 12 * M, stats, stats + 20 * M, loss.data_ptr() if each else rows,
+                                   rows if each else loss.data_ptr(), n, stats + 16 * M, _ext.stream_ptr())
         _ext.check(code, "kd_linear_rows")
-        ctx.save_for_backward(hidden, weight, idx, lg, lse, coef, gscale, stats)
-        ctx.tau = tau
-        ctx.set_materialize_grads(False)
-        return out[0], loss_rows
+        ctx.save_for_backward(hidden, weight, idx, lg, buf)
+        ctx.cfg = (tau, reduction)
+        return loss
 
     @staticmethod
-    def backward(ctx, gout, grows):
-        hidden, weight, idx, lg, lse, coef, gscale, stats = ctx.saved_tensors
+    def backward(ctx, grad):
+        hidden, weight, idx, lg, buf = ctx.saved_tensors
+        tau, reduction = ctx.cfg
         L = _ext.lib()
         M, K = hidden.shape
         V = weight.shape[0]
         dev = hidden.device
         status = _ext.status_buffer(dev)
-        if grows is None and gout is not None:
-            g1 = gout.float().reshape(1).contiguous()
-        else:                                          # gradient arriving through the rows' losses
-            scale = gscale * gout.float() if gout is not None else torch.zeros_like(gscale)
-            if grows is not None:
-                scale = scale + grows.float() * ctx.tau * (stats[:, 1] != -1.0)
-            gscale = scale.contiguous()
-            g1 = torch.ones(1, dtype=torch.float32, device=dev)
+        stats = buf.data_ptr()
+        lse, gscale, coef = stats + 12 * M, stats + 16 * M, stats + 20 * M
+        if reduction == "none":                        # the factor of every row's d(logits) comes with the rows' gradients
+            scale = buf[4 * M:5 * M] * grad
+            gscale, g1 = scale.data_ptr(), torch.ones(1, dtype=torch.float32, device=dev)
+        else:
+            g1 = grad if grad.dtype == torch.float32 else grad.float()
         need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         Vc = _cce_chunk(M, K, V, _sm_count(dev))
         G = torch.empty(M, Vc, dtype=torch.bfloat16, device=dev)
@@ -1193,12 +1217,12 @@ class _LinearDistillFn(torch.autograd.Function):
         for c0 in range(0, V, Vc):
             vc = min(Vc, V - c0)
             wc = weight[c0:c0 + vc]
-            code = L.cb_cce_dlogits_t(hidden.data_ptr(), wc.data_ptr(), None, lse.data_ptr(), gscale.data_ptr(), g1.data_ptr(),
+            code = L.cb_cce_dlogits_t(hidden.data_ptr(), wc.data_ptr(), None, lse, gscale, g1.data_ptr(),
                                       G.data_ptr(), M, vc, K, hidden.stride(0), weight.stride(0), G.stride(0), c0, V, 0.0, 0.0,
-                                      math.log2(math.e) / ctx.tau, status.data_ptr(), _ext.stream_ptr())
+                                      math.log2(math.e) / tau, status.data_ptr(), _ext.stream_ptr())
             _ext.check(code, "cce_dlogits_t")
-            code = L.cb_kd_place(G.data_ptr(), G.stride(0), c0, vc, V, M, *_teacher_ptrs(idx, lg), ctx.tau, coef.data_ptr(),
-                                 gscale.data_ptr(), g1.data_ptr(), _ext.stream_ptr())
+            code = L.cb_kd_place(G.data_ptr(), G.stride(0), c0, vc, V, M, *_teacher_ptrs(idx, lg), tau, coef, gscale,
+                                 g1.data_ptr(), _ext.stream_ptr())
             _ext.check(code, "kd_place")
             Gc = G[:, :vc]
             if slabs > 1:
@@ -1226,15 +1250,15 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indi
         raise ValueError(f"linear_distillation: weight {tuple(weight.shape)} does not fit hidden states {tuple(hidden.shape)}")
     idx, lg, y = _distill_args("linear_distillation", lead, weight.shape[0], teacher_indices, teacher_logits, temperature, labels,
                                reduction, hidden, weight)
-    h = hidden.reshape(-1, hidden.shape[-1])
+    h = hidden if hidden.dim() == 2 else hidden.reshape(-1, hidden.shape[-1])
     if (_fast(h, weight) and h.shape[1] % 8 == 0 and h.shape[0] and _gemm_ok(weight)
             and weight.stride(0) >= weight.shape[1] and h.shape[1] * 2 + idx.shape[1] * 12 <= 200 * 1024
-            and idx.shape[1] <= _ext.lib().cb_kd_max_entries()):
+            and idx.shape[1] <= _KD_MAX_ENTRIES):
         if not _gemm_ok(h) or h.stride(0) < h.shape[1]:
             h = h.clone(memory_format=torch.contiguous_format)
         lg = lg.float() if lg.dtype == torch.float64 else lg
-        loss, rows = _LinearDistillFn.apply(h, weight, idx, lg, y, ignore_index, float(temperature), reduction == "mean")
-        return rows.view(lead) if reduction == "none" else loss
+        loss = _LinearDistillFn.apply(h, weight, idx, lg, y, ignore_index, float(temperature), reduction)
+        return loss.view(lead) if reduction == "none" else loss
     wide = torch.float64 if h.dtype == torch.float64 else torch.float32
     rows, valid = ref.distillation_rows(h.to(wide) @ weight.to(wide).t(), idx, lg, float(temperature), y, ignore_index)
     return ref.reduce_rows(rows.view(lead), valid, reduction)

@@ -57,9 +57,9 @@ _PROTOTYPES = {
     "cb_gemm_bf16_slabs": [P, P, P, I, I, I, L, L, I, I, I, I, P, P],
     "cb_slab_sum": [P, P, I, I, I, P],
     "cb_kd_max_entries": [],
-    "cb_kd_logits": [P, L, L, I, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P],
+    "cb_kd_logits": [P, L, L, I, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P, P],
     "cb_kd_logits_grad": [P, P, L, L, L, I, I, P, L, I, P, L, I, I, P, L, F, P, P, P, P, P, P],
-    "cb_kd_linear_rows": [P, L, P, L, I, I, I, P, P, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P, P, P],
+    "cb_kd_linear_rows": [P, L, P, L, I, I, I, P, P, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P, P, P, P],
     "cb_kd_place": [P, L, I, I, I, I, P, L, I, P, L, I, I, F, P, P, P, P],
     "cb_attn_fwd": [P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, P, P],
     "cb_attn_bwd": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, F, P, P, P, P, P, L, P, P, I],

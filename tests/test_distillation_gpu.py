@@ -261,7 +261,7 @@ def test_entry_points_refuse_bad_sizes():
 
     def call(rows=2, V=16, K=2, tau=1.0):
         return L.cb_kd_logits(z.data_ptr(), rows, 16, V, 0, idx.data_ptr(), 2, 1, f.data_ptr(), 2, 0, K, None, -100, tau, 1, f.data_ptr(),
-                              f.data_ptr(), f.data_ptr(), f.data_ptr(), _ext.stream_ptr())
+                              f.data_ptr(), f.data_ptr(), f.data_ptr(), f.data_ptr(), _ext.stream_ptr())
     assert call(rows=0) == call(V=0) == call(K=0) == call(K=L.cb_kd_max_entries() + 1) == call(tau=0.0) == call(tau=math.nan) == -1
 
 
@@ -310,3 +310,16 @@ def test_slabs_only_where_tiles_are_few():
     assert L.cb_gemm_bf16_slabs(None, None, None, 0, 8, 8, 8, 8, 0, 1, 1, 0, None, None) == -1
     assert L.cb_gemm_bf16_slabs(None, None, None, 8, 6, 8, 8, 8, 0, 1, 1, 0, None, None) == -1
     assert L.cb_slab_sum(None, None, 8, 6, 1, None) == -1
+
+
+@pytest.mark.parametrize("linear", [False, True])
+def test_loss_may_be_changed_in_place_before_the_backward_pass(linear):
+    T, H, V, K = 30, 64, 500, 4
+    x = (torch.randn(T, H, device=DEV).to(BF).requires_grad_(), torch.randn(V, H, device=DEV).mul(0.2).to(BF).requires_grad_())
+    x = x if linear else (torch.randn(T, V, device=DEV).requires_grad_(),)
+    op = ops.linear_distillation if linear else ops.distillation_logits
+    idx, lg = entries(T, V, K, device=DEV)
+    want = torch.autograd.grad(op(*x, idx, lg) * 0.5, x)
+    loss = op(*x, idx, lg)
+    loss.mul_(0.5)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, x), want))
