@@ -328,17 +328,30 @@ kd_finalize_kernel(const float* __restrict__ loss_rows, const float2* __restrict
 }
 
 // ------------------------------------------------------------------ from hidden states and the output weight
+// idle[b] = 1 where none of the rows [128 b, 128 b + 128) takes part: the vocabulary products leave such blocks out (prompts are often
+// long, and masked).
+__global__ void __launch_bounds__(128)
+kd_idle_kernel(const KdTeacher t, int V, long long M, int* __restrict__ idle) {
+  const long long row = blockIdx.x * 128LL + threadIdx.x;
+  bool on = false;
+  if (row < M && (t.labels == nullptr || t.labels[row] != t.ignore_index))
+    for (int k = 0; k < t.K && !on; ++k) on = kd_index(t, row, k, V) >= 0 && kd_logit(t, row, k) * t.inv_tau != -INFINITY;
+  const int any = __syncthreads_or(on);
+  if (threadIdx.x == 0) idle[blockIdx.x] = any ? 0 : 1;
+}
+
 // One block a row, after the vocabulary product has left its partial maxima and sums: the row's log-sum-exp, the student's logits of
 // the teacher's words (dot products of the hidden row, kept in shared memory, with gathered weight rows: KD_DOTS rows a warp at
 // a time, so that as many loads are in flight), the loss, and coef[row, K] = p - q, what d(logits) holds at those words.
-// Bound by the gathers: K weight rows a token.
-constexpr int KD_DOTS = 4;
+// Bound by the gathers: K weight rows a token.  8192 x 896, 64 words a row, a fifth of the rows masked: 152 us (5 TB/s, part of it from
+// L2); 4 rows at a time 196, 8 278, 256 threads 181.
+constexpr int KD_DOTS = 2, KD_ROW_THREADS = 128;
 
-__global__ void __launch_bounds__(CE_THREADS)
+__global__ void __launch_bounds__(KD_ROW_THREADS)
 kd_linear_rows_kernel(const bf16* __restrict__ hidden, long long ldh, const bf16* __restrict__ weight, long long ldw, int H, int V,
                       int M, const float* __restrict__ part_m, const float* __restrict__ part_s, int n_splits, const KdTeacher t,
                       float c2, float* __restrict__ lse, float2* __restrict__ stats, float* __restrict__ coef,
-                      float* __restrict__ loss_rows) {
+                      int* __restrict__ words, float* __restrict__ loss_rows) {
   extern __shared__ uint8_t kd_smem[];
   uint4* s_h = reinterpret_cast<uint4*>(kd_smem);      // H / 8 vectors
   int* s_idx = reinterpret_cast<int*>(s_h + H / 8);
@@ -346,6 +359,14 @@ kd_linear_rows_kernel(const bf16* __restrict__ hidden, long long ldh, const bf16
   float* s_z = s_q + t.K;                              // the student's logits
   __shared__ float red[32];
   const long long row = blockIdx.x;
+  if (!kd_load(t, row, V, s_idx, s_q)) {               // its partial sums may not exist
+    if (threadIdx.x == 0) {
+      stats[row] = make_float2(0.f, -1.f);
+      loss_rows[row] = 0.f;
+      lse[row] = 1e30f;                                // probabilities of zero, whatever the logits
+    }
+    return;
+  }
   KdAcc a;
   {
     float m = -INFINITY;
@@ -360,15 +381,7 @@ kd_linear_rows_kernel(const bf16* __restrict__ hidden, long long ldh, const bf16
     a.s = kd_block_sum(s, red);
   }
   const float log2s = log2f(a.s);
-  const bool on = kd_load(t, row, V, s_idx, s_q);
   if (threadIdx.x == 0) lse[row] = (a.M + log2s) * KD_LN2;
-  if (!on) {
-    if (threadIdx.x == 0) {
-      stats[row] = make_float2(0.f, -1.f);
-      loss_rows[row] = 0.f;
-    }
-    return;
-  }
   const int nv = H / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   for (int i = threadIdx.x; i < nv; i += blockDim.x) s_h[i] = reinterpret_cast<const uint4*>(hidden + row * ldh)[i];
   __syncthreads();
@@ -413,6 +426,7 @@ kd_linear_rows_kernel(const bf16* __restrict__ hidden, long long ldh, const bf16
       d = exp2f(l2) - word;
     }
     coef[row * t.K + k] = d;
+    words[row * t.K + k] = s_idx[k];
   }
   sum = kd_block_sum(sum, red);
   if (threadIdx.x == 0) {
@@ -421,19 +435,19 @@ kd_linear_rows_kernel(const bf16* __restrict__ hidden, long long ldh, const bf16
   }
 }
 
-// G[row, i - c0] = gscale gout (p - q) for the teacher's words i in [c0, c0 + Vc), over the softmax's part that the product left
+// G[row, i - c0] = gscale gout (p - q) for the teacher's words i in [c0, c0 + Vc), over the softmax's part that the product left.
+// words [M, K]: -1 for an absent entry.  A warp a row: every chunk looks at every entry, so the entries are read as plainly as can be.
 __global__ void __launch_bounds__(CE_THREADS)
-kd_place_kernel(bf16* __restrict__ G, long long ldg, int c0, int Vc, int V, long long M, const KdTeacher t,
+kd_place_kernel(bf16* __restrict__ G, long long ldg, int c0, int Vc, long long M, int K, const int* __restrict__ words,
                 const float* __restrict__ coef, const float* __restrict__ gscale, const float* __restrict__ gout) {
-  const long long at = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
-  if (at >= M * t.K) return;
-  const long long row = at / t.K;
-  const int k = static_cast<int>(at - row * t.K), i = kd_index(t, row, k, V) - c0;
-  if (i < 0 || i >= Vc) return;
+  const long long row = blockIdx.x * static_cast<long long>(CE_THREADS / 32) + (threadIdx.x >> 5);
+  if (row >= M) return;
   const float gs = gscale[row];
-  if (gs == 0.f) return;
-  if (kd_logit(t, row, k) * t.inv_tau == -INFINITY) return;                // absent: the softmax's part stands
-  G[row * ldg + i] = __float2bfloat16(coef[at] * gs * gout[0]);           // every entry of one index writes the same value
+  if (gs == 0.f) return;                               // a row that takes no part has no words either
+  for (int k = threadIdx.x & 31; k < K; k += 32) {
+    const int w = words[row * K + k], i = w - c0;
+    if (w >= 0 && i >= 0 && i < Vc) G[row * ldg + i] = __float2bfloat16(coef[row * K + k] * gs * gout[0]);   // one index, one value
+  }
 }
 
 }  // namespace cb
@@ -512,12 +526,21 @@ int cb_kd_logits_grad(const void* logits, void* dlogits, long long rows, long lo
   return static_cast<int>(cudaGetLastError());
 }
 
-// From hidden states, after cb_cce_forward_t: part_m / part_s [n_splits, M].  lse, loss_rows, gscale [M], stats [M, 2], coef [M, K],
-// loss and n_rows as above.
+// From hidden states, first of all: idle [ceil(M / 128)]
+int cb_kd_idle(const void* idx, long long ld_idx, int idx64, const void* lg, long long ld_lg, int lg_bf16, int K, const long long* labels,
+               long long ignore_index, float tau, int V, int M, int* idle, void* stream) {
+  cb::KdTeacher t;
+  if (M <= 0 || V <= 0 || !kd_teacher(&t, idx, ld_idx, idx64, lg, ld_lg, lg_bf16, K, labels, ignore_index, tau)) return -1;
+  cb::kd_idle_kernel<<<(M + 127) / 128, 128, 0, static_cast<cudaStream_t>(stream)>>>(t, V, M, idle);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// From hidden states, after cb_cce_forward_t: part_m / part_s [n_splits, M].  lse, loss_rows, gscale [M], stats [M, 2], coef and
+// words [M, K], loss and n_rows as above.
 int cb_kd_linear_rows(const void* hidden, long long ldh, const void* weight, long long ldw, int H, int V, int M, const float* part_m,
                       const float* part_s, int n_splits, const void* idx, long long ld_idx, int idx64, const void* lg, long long ld_lg,
                       int lg_bf16, int K, const long long* labels, long long ignore_index, float tau, int mean, float* lse,
-                      float* stats, float* coef, float* loss_rows, float* loss, float* n_rows, float* gscale, void* stream) {
+                      float* stats, float* coef, int* words, float* loss_rows, float* loss, float* n_rows, float* gscale, void* stream) {
   cb::KdTeacher t;
   if (M <= 0 || V <= 0 || H <= 0 || H % 8 != 0 || ldh % 8 != 0 || ldw % 8 != 0 ||
       ((reinterpret_cast<uintptr_t>(hidden) | reinterpret_cast<uintptr_t>(weight)) & 15) != 0 ||
@@ -528,23 +551,21 @@ int cb_kd_linear_rows(const void* hidden, long long ldh, const void* weight, lon
   if (smem > 227 * 1024 - 1024) return -1;
   if (smem > 48 * 1024) CB_CHECK_CUDA(cudaFuncSetAttribute(cb::kd_linear_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
   float2* st = reinterpret_cast<float2*>(stats);
-  cb::kd_linear_rows_kernel<<<M, cb::CE_THREADS, smem, s>>>(
+  cb::kd_linear_rows_kernel<<<M, cb::KD_ROW_THREADS, smem, s>>>(
       static_cast<const cb::bf16*>(hidden), ldh, static_cast<const cb::bf16*>(weight), ldw, H, V, M, part_m, part_s, n_splits, t,
-      kd_scale(tau), lse, st, coef, loss_rows);
+      kd_scale(tau), lse, st, coef, words, loss_rows);
   CB_CHECK_CUDA(cudaGetLastError());
   cb::kd_finalize_kernel<<<1, 1024, 0, s>>>(loss_rows, st, M, mean, tau, loss, n_rows, gscale);
   return static_cast<int>(cudaGetLastError());
 }
 
-// The teacher's words in a chunk [c0, c0 + Vc) of d(logits)
-int cb_kd_place(void* G, long long ldg, int c0, int Vc, int V, int M, const void* idx, long long ld_idx, int idx64, const void* lg,
-                long long ld_lg, int lg_bf16, int K, float tau, const float* coef, const float* gscale, const float* gout, void* stream) {
-  cb::KdTeacher t;
-  if (M <= 0 || Vc <= 0 || !kd_teacher(&t, idx, ld_idx, idx64, lg, ld_lg, lg_bf16, K, nullptr, 0, tau)) return -1;
-  const long long n = static_cast<long long>(M) * K, blocks = (n + cb::CE_THREADS - 1) / cb::CE_THREADS;
-  if (blocks > 0x7fffffffLL) return -1;
-  cb::kd_place_kernel<<<static_cast<unsigned>(blocks), cb::CE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<cb::bf16*>(G), ldg, c0, Vc, V, M, t, coef, gscale, gout);
+// The teacher's words in a chunk [c0, c0 + Vc) of d(logits), as cb_kd_linear_rows left them
+int cb_kd_place(void* G, long long ldg, int c0, int Vc, int M, int K, const int* words, const float* coef, const float* gscale,
+                const float* gout, void* stream) {
+  if (M <= 0 || Vc <= 0 || K < 1) return -1;
+  constexpr int rows = cb::CE_THREADS / 32;
+  cb::kd_place_kernel<<<(M + rows - 1) / rows, cb::CE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<cb::bf16*>(G), ldg, c0, Vc, M, K, words, coef, gscale, gout);
   return static_cast<int>(cudaGetLastError());
 }
 

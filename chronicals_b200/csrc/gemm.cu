@@ -50,6 +50,7 @@ struct GemmArgs {
   long long ld_add;
   // cut-cross-entropy
   const long long* labels;  // [M], global vocab ids, ignore_index allowed; null: no row has a label
+  const int* idle;          // [m-blocks] or null: 1 = no row of the block takes part, its logits are not formed and its d(logits) are zero
   float e2_scale;           // log2(e) over the temperature: a logit v stands for 2^(v e2_scale)
   float* part_m;            // [n_splits, M]
   float* part_s;            // [n_splits, M]
@@ -157,6 +158,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         int m_blk = item % g.num_m_blocks + g.rot_blocks;
         if (m_blk >= g.num_m_blocks) m_blk -= g.num_m_blocks;
         const int split = item / g.num_m_blocks;
+        if (EPI != EPI_STORE && g.idle != nullptr && g.idle[m_blk]) continue;
         const int nt0 = split * g.tiles_per_item;
         const int nt1 = min(nt0 + g.tiles_per_item, g.num_n_tiles);
         if (g.panel_blocks > 0) {
@@ -228,6 +230,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const int kb0 = g.items_per_ksplit > 0 ? ks * g.kb_per_split : 0;
         const int kb1 = g.items_per_ksplit > 0 ? min(num_kb, kb0 + g.kb_per_split) : num_kb;
         const int split = item / g.num_m_blocks;
+        if (EPI != EPI_STORE && g.idle != nullptr && g.idle[item % g.num_m_blocks]) continue;
         const int nt0 = split * g.tiles_per_item;
         const int nt1 = min(nt0 + g.tiles_per_item, g.num_n_tiles);
         for (int nt = nt0; nt < nt1 && ok; ++nt, ++tile_cnt) {
@@ -280,6 +283,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       // reduce-scatter epilogue: this m-block's rows live on rank m_blk / push_blocks
       bf16* push_base = g.push_blocks > 0 ? reinterpret_cast<bf16*>(g.push_c[m_blk / g.push_blocks]) : nullptr;
       const bool row_ok = row < g.M;
+      const bool idle = EPI != EPI_STORE && g.idle != nullptr && g.idle[m_blk];
+      if (EPI == EPI_LSE && idle) continue;
 
       // per-row state of the cut-cross-entropy epilogues
       float run_m = -INFINITY, run_s = 0.f, run_sum = 0.f;
@@ -297,16 +302,18 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
       }
 
-      for (int nt = nt0; nt < nt1 && ok; ++nt, ++tile_cnt) {
+      for (int nt = nt0; nt < nt1 && ok; ++nt, tile_cnt += EPI != EPI_STORE && idle ? 0 : 1) {
         const uint32_t acc = tile_cnt & 1u;
         const uint32_t acc_phase = (tile_cnt >> 1) & 1u;
-        bool w = mbar_wait(tfull + acc, acc_phase, abort_flag, g.status, CB_ERR_WAIT_TMEM_FULL);
-        w = __all_sync(0xffffffffu, w);
-        if (!w) {
-          ok = false;
-          break;
+        if (EPI == EPI_STORE || !idle) {
+          bool w = mbar_wait(tfull + acc, acc_phase, abort_flag, g.status, CB_ERR_WAIT_TMEM_FULL);
+          w = __all_sync(0xffffffffu, w);
+          if (!w) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
         }
-        tc_fence_after();
         const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BLOCK_N;
 
         if (EPI != EPI_LSE && g.tma_store) {
@@ -347,6 +354,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
                   for (int j = 0; j < 32; ++j)
                     if (j == rel) v[j] -= hit;
+                }
+                if (idle) {                            // no product was formed
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v[j] = 0.f;
                 }
               } else {
                 if (g.bias != nullptr) {
@@ -511,6 +522,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                   for (int j = 0; j < 32; ++j)
                     if (j == rel) v[j] -= hit;
                 }
+                if (idle) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                }
               } else {
                 if (g.bias != nullptr) {
 #pragma unroll
@@ -584,7 +599,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty + acc);
+        if ((EPI == EPI_STORE || !idle) && lane == 0) mbar_arrive(tempty + acc);
       }
       if (EPI == EPI_LSE && ok && row_ok) {
         const long long o = static_cast<long long>(split) * g.M + row;
@@ -1143,10 +1158,11 @@ int cb_cce_num_splits(int M, int V) {
 }
 
 // Forward: per-row log-sum-exp partials of hidden[M,K] * weight[V,K]^T over the temperature (part_m: the maximum of the
-// logits themselves), target logit where there are labels (else labels and tgt are null).
+// logits themselves), target logit where there are labels (else labels and tgt are null).  idle [ceil(M / 128)] or null: blocks of
+// 128 rows that are left out, their partials unwritten (and, in cb_cce_dlogits_t, their d(logits) zero).
 int cb_cce_forward_t(const void* hidden, const void* weight, const long long* labels, int M, int V, int K,
-                     long long ldh, long long ldw, int col_offset, float e2_scale, float* part_m, float* part_s, float* part_sum,
-                     float* tgt, int* status, void* stream) {
+                     long long ldh, long long ldw, int col_offset, float e2_scale, const int* idle, float* part_m, float* part_s,
+                     float* part_sum, float* tgt, int* status, void* stream) {
   const int bn = 256;
   CUtensorMap ta, tb;
   int e = build_maps(&ta, &tb, hidden, weight, M, V, K, ldh, ldw, 0, 0, bn);
@@ -1160,6 +1176,7 @@ int cb_cce_forward_t(const void* hidden, const void* weight, const long long* la
   g.num_items = g.num_m_blocks * n_splits;
   g.labels = labels;
   g.e2_scale = e2_scale;
+  g.idle = idle;
   g.part_m = part_m; g.part_s = part_s; g.part_sum = part_sum; g.tgt = tgt;
   g.col_offset = col_offset;
   g.status = status;
@@ -1171,7 +1188,7 @@ int cb_cce_forward_t(const void* hidden, const void* weight, const long long* la
 int cb_cce_forward(const void* hidden, const void* weight, const long long* labels, int M, int V, int K,
                    long long ldh, long long ldw, int col_offset, float* part_m, float* part_s, float* part_sum,
                    float* tgt, int* status, void* stream) {
-  return cb_cce_forward_t(hidden, weight, labels, M, V, K, ldh, ldw, col_offset, 1.4426950408889634f, part_m, part_s, part_sum,
+  return cb_cce_forward_t(hidden, weight, labels, M, V, K, ldh, ldw, col_offset, 1.4426950408889634f, nullptr, part_m, part_s, part_sum,
                           tgt, status, stream);
 }
 
@@ -1192,7 +1209,7 @@ int cb_cce_combine(const float* part_m, const float* part_s, const float* part_s
 int cb_cce_dlogits_t(const void* hidden, const void* weight_chunk, const long long* labels, const float* lse,
                      const float* gscale, const float* gout, void* G, int M, int Vc, int K, long long ldh,
                      long long ldw, long long ldg, int col_offset, int V_total, float smoothing, float z_weight,
-                     float e2_scale, int* status, void* stream) {
+                     float e2_scale, const int* idle, int* status, void* stream) {
   const int bn = pick_block_n(M, Vc, 0);
   CUtensorMap ta, tb;
   int e = build_maps(&ta, &tb, hidden, weight_chunk, M, Vc, K, ldh, ldw, 0, 0, bn);
@@ -1206,6 +1223,7 @@ int cb_cce_dlogits_t(const void* hidden, const void* weight_chunk, const long lo
   g.C = G; g.ldc = ldg; g.out_fp32 = 0; g.accumulate = 0;
   g.labels = labels; g.lse = lse; g.gscale = gscale; g.gout = gout;
   g.e2_scale = e2_scale;
+  g.idle = idle;
   g.z_weight = z_weight; g.smoothing = smoothing; g.V_total = V_total; g.col_offset = col_offset;
   g.status = status;
   CUtensorMap tc;
@@ -1219,7 +1237,7 @@ int cb_cce_dlogits(const void* hidden, const void* weight_chunk, const long long
                    long long ldw, long long ldg, int col_offset, int V_total, float smoothing, float z_weight,
                    int* status, void* stream) {
   return cb_cce_dlogits_t(hidden, weight_chunk, labels, lse, gscale, gout, G, M, Vc, K, ldh, ldw, ldg, col_offset, V_total,
-                          smoothing, z_weight, 1.4426950408889634f, status, stream);
+                          smoothing, z_weight, 1.4426950408889634f, nullptr, status, stream);
 }
 
 }  // extern "C"

@@ -1168,35 +1168,42 @@ class _LinearDistillFn(torch.autograd.Function):
         part = torch.empty(2 * n_splits * M, dtype=torch.float32, device=dev)
         p0 = part.data_ptr()
         p1 = p0 + 4 * n_splits * M
+        # blocks of 128 rows of which none takes part (a masked prompt's, say) are left out of the vocabulary products
+        idle = torch.empty(-(-M // 128), dtype=torch.int32, device=dev)
+        code = L.cb_kd_idle(*_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau, V, M, idle.data_ptr(), _ext.stream_ptr())
+        _ext.check(code, "kd_idle")
         code = L.cb_cce_forward_t(hidden.data_ptr(), weight.data_ptr(), None, M, V, K, hidden.stride(0), weight.stride(0), 0,
-                                  math.log2(math.e) / tau, p0, p1, None, None, _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr())
+                                  math.log2(math.e) / tau, idle.data_ptr(), p0, p1, None, None, _ext.status_buffer(dev).data_ptr(),
+                                  _ext.stream_ptr())
         _ext.check(code, "cce_forward_t")
-        # stats [M, 2], losses, log-sum-exps and factors of the rows [M] each, p - q at the teacher's words [M, K]; the number of rows
-        buf = torch.empty(1 + M * (5 + idx.shape[1]), dtype=torch.float32, device=dev)
+        # stats [M, 2], losses, log-sum-exps and factors of the rows [M] each, p - q at the teacher's words [M, K] and the words (int32),
+        # the number of rows
+        N = idx.shape[1]
+        buf = torch.empty(1 + M * (5 + 2 * N), dtype=torch.float32, device=dev)
         each = reduction == "none"
         loss = torch.empty((M,) if each else (), dtype=torch.float32, device=dev)
         stats = buf.data_ptr()
         rows, n = stats + 8 * M, stats + 4 * (buf.numel() - 1)
         code = L.cb_kd_linear_rows(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0), K, V, M, p0, p1, n_splits,
                                    *_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau, int(reduction == "mean"),
-                                   stats + 12 * M, stats, stats + 20 * M, loss.data_ptr() if each else rows,
+                                   stats + 12 * M, stats, stats + 20 * M, stats + (20 + 4 * N) * M, loss.data_ptr() if each else rows,
                                    rows if each else loss.data_ptr(), n, stats + 16 * M, _ext.stream_ptr())
         _ext.check(code, "kd_linear_rows")
-        ctx.save_for_backward(hidden, weight, idx, lg, buf)
-        ctx.cfg = (tau, reduction)
+        ctx.save_for_backward(hidden, weight, buf, idle)
+        ctx.cfg = (tau, reduction, N)
         return loss
 
     @staticmethod
     def backward(ctx, grad):
-        hidden, weight, idx, lg, buf = ctx.saved_tensors
-        tau, reduction = ctx.cfg
+        hidden, weight, buf, idle = ctx.saved_tensors
+        tau, reduction, N = ctx.cfg
         L = _ext.lib()
         M, K = hidden.shape
         V = weight.shape[0]
         dev = hidden.device
         status = _ext.status_buffer(dev)
         stats = buf.data_ptr()
-        lse, gscale, coef = stats + 12 * M, stats + 16 * M, stats + 20 * M
+        lse, gscale, coef, words = stats + 12 * M, stats + 16 * M, stats + 20 * M, stats + (20 + 4 * N) * M
         if reduction == "none":                        # the factor of every row's d(logits) comes with the rows' gradients
             scale = buf[4 * M:5 * M] * grad
             gscale, g1 = scale.data_ptr(), torch.ones(1, dtype=torch.float32, device=dev)
@@ -1219,10 +1226,9 @@ class _LinearDistillFn(torch.autograd.Function):
             wc = weight[c0:c0 + vc]
             code = L.cb_cce_dlogits_t(hidden.data_ptr(), wc.data_ptr(), None, lse, gscale, g1.data_ptr(),
                                       G.data_ptr(), M, vc, K, hidden.stride(0), weight.stride(0), G.stride(0), c0, V, 0.0, 0.0,
-                                      math.log2(math.e) / tau, status.data_ptr(), _ext.stream_ptr())
+                                      math.log2(math.e) / tau, idle.data_ptr(), status.data_ptr(), _ext.stream_ptr())
             _ext.check(code, "cce_dlogits_t")
-            code = L.cb_kd_place(G.data_ptr(), G.stride(0), c0, vc, V, M, *_teacher_ptrs(idx, lg), tau, coef, gscale,
-                                 g1.data_ptr(), _ext.stream_ptr())
+            code = L.cb_kd_place(G.data_ptr(), G.stride(0), c0, vc, M, N, words, coef, gscale, g1.data_ptr(), _ext.stream_ptr())
             _ext.check(code, "kd_place")
             Gc = G[:, :vc]
             if slabs > 1:

@@ -51,16 +51,17 @@ _PROTOTYPES = {
     "cb_embedding_bwd": [P, P, P, P, P, L, I, L, I, P],
     "cb_ce_logits": [P, P, L, L, I, I, L, F, F, P, P, P],
     "cb_ce_logits_grad": [P, P, P, P, P, P, L, L, L, I, I, L, F, F, P],
-    "cb_cce_forward_t": [P, P, P, I, I, I, L, L, I, F, P, P, P, P, P, P],
-    "cb_cce_dlogits_t": [P, P, P, P, P, P, P, I, I, I, L, L, L, I, I, F, F, F, P, P],
+    "cb_cce_forward_t": [P, P, P, I, I, I, L, L, I, F, P, P, P, P, P, P, P],
+    "cb_cce_dlogits_t": [P, P, P, P, P, P, P, I, I, I, L, L, L, I, I, F, F, F, P, P, P],
+    "cb_kd_idle": [P, L, I, P, L, I, I, P, L, F, I, I, P, P],
     "cb_gemm_slabs": [I, I, I, I, I, I],
     "cb_gemm_bf16_slabs": [P, P, P, I, I, I, L, L, I, I, I, I, P, P],
     "cb_slab_sum": [P, P, I, I, I, P],
     "cb_kd_max_entries": [],
     "cb_kd_logits": [P, L, L, I, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P, P],
     "cb_kd_logits_grad": [P, P, L, L, L, I, I, P, L, I, P, L, I, I, P, L, F, P, P, P, P, P, P],
-    "cb_kd_linear_rows": [P, L, P, L, I, I, I, P, P, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P, P, P, P],
-    "cb_kd_place": [P, L, I, I, I, I, P, L, I, P, L, I, I, F, P, P, P, P],
+    "cb_kd_linear_rows": [P, L, P, L, I, I, I, P, P, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P, P, P, P, P],
+    "cb_kd_place": [P, L, I, I, I, I, P, P, P, P, P],
     "cb_attn_fwd": [P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, P, P],
     "cb_attn_bwd": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, F, P, P, P, P, P, L, P, P, I],
     "cb_attn_window_fwd": [P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, I, I, P, P, P],

@@ -323,3 +323,28 @@ def test_loss_may_be_changed_in_place_before_the_backward_pass(linear):
     loss = op(*x, idx, lg)
     loss.mul_(0.5)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, x), want))
+
+
+@pytest.mark.parametrize("T,masked", [(700, [(0, 300)]), (700, [(128, 384), (600, 700)]), (513, [(0, 512)]), (256, [(0, 256)]), (384, [(5, 380)])])
+def test_blocks_of_rows_that_take_no_part(T, masked):
+    """Whole blocks of 128 masked rows are left out of the products, mixed ones are not; large logits in masked rows do no harm."""
+    H, V, K, tau = 128, 3000, 6, 1.5
+    g = torch.Generator(device=DEV).manual_seed(T)
+    h = torch.randn(T, H, device=DEV, generator=g).to(BF)
+    labels = torch.zeros(T, dtype=torch.int64, device=DEV)
+    for a, b in masked:
+        labels[a:b] = -100
+        h[a:b] *= 100
+    h.requires_grad_()
+    w = (torch.randn(V, H, device=DEV, generator=g) / 8).to(BF).requires_grad_()
+    idx, lg = entries(T, V, K, device=DEV)
+    h64, w64 = h.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    rows, valid = definition(h64 @ w64.t(), idx, lg, tau, labels)
+    want = torch.autograd.grad(rows.sum() / max(1, int(valid.sum())), (h64, w64))
+    loss = ops.linear_distillation(h, w, idx, lg, tau, labels)
+    assert abs(loss.item() - rows.sum().item() / max(1, int(valid.sum()))) <= 1e-4
+    got = torch.autograd.grad(loss, (h, w))
+    _ext.check_status()
+    for a, b in zip(got, want):
+        assert ((a.double() - b).norm() <= 2.0 ** -7 * b.norm()).item()
+    assert (got[0][labels == -100] == 0).all()
