@@ -1070,7 +1070,7 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   int ib, n_it;                                        // the first query block and how many
   if (WIN) {
     int run;
-    if (!locate_window_tile<true>(a, blockIdx.y, start, len, nblk, jb, run)) return;
+    if (!locate_window_tile<true, D == 64>(a, blockIdx.y, start, len, nblk, jb, run)) return;
     window_query_blocks(a, jb, run, nblk, ib, n_it);
     if (n_it <= 0) return;                             // a run that ends before the key block begins
   } else {
@@ -1472,7 +1472,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   int ib, n_it;                                        // the first query block and how many
   if (WIN) {
     int run;
-    if (!locate_window_tile<true>(a, blockIdx.y, start, len, nblk, jb, run)) return;
+    if (!locate_window_tile<true, D == 64>(a, blockIdx.y, start, len, nblk, jb, run)) return;
     window_query_blocks(a, jb, run, nblk, ib, n_it);
     if (n_it <= 0) return;                             // a run that ends before the key block begins
   } else {
@@ -2100,6 +2100,7 @@ int attn_bwd(const void* q, const void* k, const void* v, const void* o, const v
   if (window > 0) {
     a.window = std::min(window, T);
     a.sinks = std::min(sinks, T);
+    a.cap = (a.window + 126) / 128 + 1;
     // Runs as long as the loop of a key block without sinks, and no shorter than 6, since a CTA of less is mostly set-up (14 heads of
     // 64, 8192 tokens, window 128: runs of 2 / 4 / 6 / 8 blocks 91 / 81 / 76 / 79 us), or than 3 where the grid leaves SMs free
     // (1024 tokens: 18 / 16 / 20 / 24, of 3 14).

@@ -23,55 +23,97 @@ struct AttnArgs {
   // windowed forms: a query sees the last `window` keys of its document, its own among them, and the document's first `sinks`
   int window, sinks;
   bf16* o_lo;           // forward, [T, hq, D] without gaps or null: O less its rounding to bf16, rounded itself (for delta)
+  int cap;              // blocks of 128 that a tile's loop visits at most, sinks apart
   int sink_run;         // backward: query blocks per CTA of a key block that holds sinks
 };
 
-// The tile of a windowed kernel: CTA b's, document by document, the weights being all but equal (a window's worth of blocks).
-// Forward, one tile per query block, the last block of a document first.  Backward, one per key block; a key block that holds sinks
-// is seen by every later query of its document, and its query blocks are shared out over CTAs in runs of a.sink_run, which come
-// first in their document.  blk: the block of the tile, run: of which run (-1: a key block without sinks).
-template <bool BWD>
+// The lane that item b falls into where every lane has `mine` of them, and b within that lane; b < the sum of all
+__device__ __forceinline__ int lane_of_item(int& b, int mine) {
+  const int lane = threadIdx.x & 31;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  const int src = __ffs(__ballot_sync(0xffffffffu, b < upto)) - 1;
+  b -= __shfl_sync(0xffffffffu, upto - mine, src);
+  return src;
+}
+
+// The tile of a windowed kernel: CTA b's.  Forward, one tile per query block, the last block of a document first; backward, one per
+// key block.  Key blocks that hold sinks are seen by every later query of their document: their query blocks are shared out over
+// CTAs in runs of a.sink_run, which come first.  blk: the block of the tile, run: of which run (-1: a key block without sinks).
+//
+// BY_WEIGHT (head size 64): two to 32 documents are handed out by weight, the blocks that a tile's loop visits, at most a.cap: first all tiles of full weight,
+// then those of every lower one, of which a document has at most one (14 / 2 heads of 64, 9 documents in 8192 tokens, window 1024,
+// backward: 124 us in the order of the documents, 114 so).  More of them go in their order: a search through more lengths than a
+// register holds, level by level, takes longer than it saves (40 documents: 74 and 94 us).  A single document's tiles are in that
+// order already; with heads of 128, whose tiles take more rounds, the order of the documents is the faster one (16 documents, 28 / 4
+// heads, window 512: 248 and 260 us).
+template <bool BWD, bool BY_WEIGHT>
 __device__ __forceinline__ bool locate_window_tile(const AttnArgs& a, int b, int& start, int& len, int& nblk, int& blk, int& run,
                                                    int* beyond = nullptr) {
   const int lane = threadIdx.x & 31;
   const int with_sinks = BWD ? (a.sinks + 127) >> 7 : 0;
+  run = -1;
   for (int d0 = 0; d0 < a.n_docs; d0 += 32) {
-    const int d = d0 + lane;
     int st = 0, ln = 0;
-    if (d < a.n_docs) {
-      st = a.cu[d];
-      ln = a.cu[d + 1] - st;
+    if (d0 + lane < a.n_docs) {
+      st = a.cu[d0 + lane];
+      ln = a.cu[d0 + lane + 1] - st;
     }
-    const int nb = (ln + 127) >> 7, ns = min(nb, with_sinks);
-    const int runs = BWD ? (nb + a.sink_run - 1) / a.sink_run : 0;
-    const int mine = nb - ns + ns * runs;
-    int upto = mine;                                   // tiles of the documents up to mine
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
+    const int nb = (ln + 127) >> 7, ns = min(nb, with_sinks), own = nb - ns;
+    const int in_runs = BWD && ns > 0 ? ns * ((nb + a.sink_run - 1) / a.sink_run) : 0;
+    const int all = __reduce_add_sync(0xffffffffu, own + in_runs);
+    if (b >= all) {
+      b -= all;
+      continue;
     }
-    const unsigned m = __ballot_sync(0xffffffffu, b < upto);
-    if (m != 0) {
-      const int src = __ffs(m) - 1;
-      const int at = b - __shfl_sync(0xffffffffu, upto - mine, src);
+    const auto take = [&](int src) {
       start = __shfl_sync(0xffffffffu, st, src);
       len = __shfl_sync(0xffffffffu, ln, src);
-      nblk = __shfl_sync(0xffffffffu, nb, src);
-      const int n_s = __shfl_sync(0xffffffffu, ns, src), n_r = __shfl_sync(0xffffffffu, runs, src);
-      if (!BWD) {
-        blk = nblk - 1 - at;
-        run = -1;
-      } else if (at < n_s * n_r) {
-        blk = at % n_s;
-        run = at / n_s;
+      nblk = (len + 127) >> 7;
+    };
+    if (!BY_WEIGHT || a.n_docs == 1 || a.n_docs > 32) {
+      take(lane_of_item(b, own + in_runs));
+      const int n_s = min(nblk, with_sinks), n_runs = n_s > 0 ? n_s * ((nblk + a.sink_run - 1) / a.sink_run) : 0;
+      if (b < n_runs) {
+        blk = b % n_s;
+        run = b / n_s;
       } else {
-        blk = at - n_s * n_r + n_s;
-        run = -1;
+        blk = BWD ? b - n_runs + n_s : nblk - 1 - b;
       }
       return true;
     }
-    b -= __shfl_sync(0xffffffffu, upto, 31);
+    if (BWD && with_sinks > 0) {
+      const int n = __reduce_add_sync(0xffffffffu, in_runs);
+      if (b < n) {
+        take(lane_of_item(b, in_runs));
+        const int n_s = min(nblk, with_sinks);
+        blk = b % n_s;
+        run = b / n_s;
+        return true;
+      }
+      b -= n;
+    }
+    const int full = max(0, own - a.cap + 1), n = __reduce_add_sync(0xffffffffu, full);
+    if (b < n) {
+      take(lane_of_item(b, full));
+      blk = BWD ? min(nblk, with_sinks) + b : nblk - 1 - b;
+      return true;
+    }
+    b -= n;
+    for (int w = min(__reduce_max_sync(0xffffffffu, own), a.cap - 1); w >= 1; --w) {
+      const unsigned m = __ballot_sync(0xffffffffu, own >= w);
+      const int c = __popc(m);
+      if (b < c) {
+        take(static_cast<int>(__fns(m, 0, b + 1)));
+        blk = BWD ? nblk - w : w - 1;
+        return true;
+      }
+      b -= c;
+    }
   }
   if (beyond != nullptr) *beyond = b;                  // index among the CTAs past the last tile
   return false;

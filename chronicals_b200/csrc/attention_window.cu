@@ -63,7 +63,7 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 
   int start, len, nblk, qb, run;
   int beyond = 0;
-  if (!locate_window_tile<false>(a, blockIdx.y, start, len, nblk, qb, run, &beyond)) {
+  if (!locate_window_tile<false, D == 64>(a, blockIdx.y, start, len, nblk, qb, run, &beyond)) {
     zero_padding_rows<D>(a, beyond, blockIdx.x);
     return;
   }
@@ -402,7 +402,7 @@ int cb_attn_window_fwd(const void* q, const void* k, const void* v, void* o, flo
   a.T = T; a.hq = hq; a.hk = hk; a.n_docs = n_docs; a.cu = cu; a.scale = scale;
   a.O = static_cast<cb::bf16*>(o); a.ldo = ldo; a.lse = lse; a.status = status;
   a.o_lo = static_cast<cb::bf16*>(o_lo);
-  a.window = std::min(window, T); a.sinks = std::min(sinks, T);
+  a.window = std::min(window, T); a.sinks = std::min(sinks, T); a.cap = (a.window + 126) / 128 + 1;
   a.o_tma = cbhost::make_tmap(&mo, o, static_cast<unsigned long long>(hq) * D, T, ldo, 64, 128) == 0 ? 1 : 0;
   if (!a.o_tma) mo = mq;                                // O is not TMA-addressable: every block stores row by row
   const dim3 grid(hq, static_cast<unsigned>(tiles));    // x: query head (fastest, the heads of a group share K / V in L2)

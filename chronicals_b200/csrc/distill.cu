@@ -304,6 +304,61 @@ kd_logits_grad_kernel(const T* __restrict__ logits, T* __restrict__ dlogits, lon
   }
 }
 
+// d(loss) / dz of fp32 logits as bf16, for the products that follow; with `lo` also what the rounding left out, in a second set of rows
+// (the products of few tokens have room for twice as many rows, and add the two in 32 bits).  Rows of both on 16-byte boundaries,
+// their pitches multiples of 8; a thread takes 8 values.  Blocks and words as in the kernel above.
+__global__ void __launch_bounds__(CE_THREADS)
+kd_logits_grad_split_kernel(const float* __restrict__ logits, bf16* __restrict__ hi, bf16* __restrict__ lo, long long ld, long long ldg,
+                            int V, const KdTeacher t, float c2, const float2* __restrict__ stats, const float* __restrict__ q,
+                            const float* __restrict__ gout, const float* __restrict__ n_rows, const float* __restrict__ grows) {
+  const long long row = blockIdx.x;
+  const float* lp = logits + row * ld;
+  bf16* hp = hi + row * ldg;
+  bf16* rp = lo != nullptr ? lo + row * ldg : nullptr;
+  const float2 st = stats[row];
+  float g = 0.f;
+  if (gout != nullptr) g += n_rows != nullptr ? gout[0] / fmaxf(n_rows[0], 1.f) : gout[0];
+  if (grows != nullptr) g += grows[row];
+  g *= t.tau;
+  const bool valid = !(st.y == -1.f);
+  const float gs = valid ? st.y * g : 0.f;
+  const auto put = [&](int i, float v) {
+    hp[i] = __float2bfloat16(v);
+    if (rp != nullptr) rp[i] = __float2bfloat16(v - __bfloat162float(hp[i]));
+  };
+  const int nvec = V / 8, y = blockIdx.y, per = (nvec + gridDim.y - 1) / gridDim.y;
+  const int v0 = min(nvec, y * per), v1 = min(nvec, v0 + per);
+  const bool highest = y == static_cast<int>(gridDim.y) - 1;
+  const int c0 = v0 * 8, c1 = highest ? V : v1 * 8;
+  for (int v = v0 + threadIdx.x; v < v1; v += blockDim.x) {
+    uint4 h = make_uint4(0u, 0u, 0u, 0u), l = h;
+    if (valid) {
+      const float4 a = reinterpret_cast<const float4*>(lp)[2 * v], b = reinterpret_cast<const float4*>(lp)[2 * v + 1];
+      float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}, f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = exp2f(fmaf(w[j], c2, -st.x)) * gs;
+      h = pack8(w);
+      unpack8(h, f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] -= f[j];
+      l = pack8(w);
+    }
+    reinterpret_cast<uint4*>(hp)[v] = h;
+    if (rp != nullptr) reinterpret_cast<uint4*>(rp)[v] = l;
+  }
+  if (highest)
+    for (int c = nvec * 8 + threadIdx.x; c < V; c += blockDim.x) put(c, valid ? exp2f(fmaf(lp[c], c2, -st.x)) * gs : 0.f);
+  if (!valid) return;
+  __syncthreads();                                     // the values above are written before those below
+  for (int k = threadIdx.x; k < t.K; k += blockDim.x) {
+    const int i = kd_index(t, row, k, V);
+    if (i >= c0 && i < c1) {
+      const float qk = q[row * t.K + k];
+      if (qk != 0.f) put(i, (exp2f(fmaf(lp[i], c2, -st.x)) * st.y - qk) * g);          // every entry of one index writes the same value
+    }
+  }
+}
+
 // loss = mean (or sum) of the rows' losses, n_rows = rows that take part; with gscale also the factor of each row's
 // d(logits), tau / n, tau or 0.  stats.y == -1 marks the rows that take no part.  One block, a fixed order.
 __global__ void __launch_bounds__(1024)
@@ -523,6 +578,24 @@ int cb_kd_logits_grad(const void* logits, void* dlogits, long long rows, long lo
   else
     cb::kd_logits_grad_kernel<float><<<grid, threads, 0, s>>>(static_cast<const float*>(logits), static_cast<float*>(dlogits), ld, ldd,
                                                               V, t, c2, st, q, gout, n_rows, grows);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// fp32 logits -> their gradient as bf16 hi [rows, V], and (lo not null) what the rounding left out
+int cb_kd_logits_grad_split(const float* logits, void* hi, void* lo, long long rows, long long ld, long long ldg, int V, const void* idx,
+                            long long ld_idx, int idx64, const void* lg, long long ld_lg, int lg_bf16, int K, const long long* labels,
+                            long long ignore_index, float tau, const float* stats, const float* q, const float* gout,
+                            const float* n_rows, const float* grows, void* stream) {
+  cb::KdTeacher t;
+  if (rows <= 0 || rows > 0x7fffffffLL || V <= 0 || ld % 8 != 0 || ldg % 8 != 0 ||
+      ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(hi) | reinterpret_cast<uintptr_t>(lo)) & 15) != 0 ||
+      !kd_teacher(&t, idx, ld_idx, idx64, lg, ld_lg, lg_bf16, K, labels, ignore_index, tau))
+    return -1;
+  int split = 1;                                        // blocks a row: until the chip is full, or a block has 2048 values
+  while (split < 64 && rows * split < 4LL * cbhost::num_sms() && V / (2 * split) >= 2048) split *= 2;
+  cb::kd_logits_grad_split_kernel<<<dim3(static_cast<unsigned>(rows), split), cb::CE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
+      logits, static_cast<cb::bf16*>(hi), static_cast<cb::bf16*>(lo), ld, ldg, V, t, kd_scale(tau), reinterpret_cast<const float2*>(stats), q,
+      gout, n_rows, grows);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -677,10 +677,10 @@ cce_combine_rows_kernel(const float* __restrict__ part_m, const float* __restric
 }
 
 // out[m, n] = sum over the slabs of a product that was cut along K, in a fixed order.  slab: elements from one to the next.  Eight
-// threads share the slabs of four values: few values and many slabs are bound by the latency of the loads (120 x 256 values, 50
+// threads share the slabs of four values (fold > 0: and of those `fold` elements further on, which are added): few values and many slabs are bound by the latency of the loads (120 x 256 values, 50
 // slabs: 8.6 us with a thread for all of them).
 __global__ void __launch_bounds__(256)
-slab_sum_kernel(const float* __restrict__ slabs, bf16* __restrict__ out, int n_slabs, long long slab, long long n4) {
+slab_sum_kernel(const float* __restrict__ slabs, bf16* __restrict__ out, int n_slabs, long long slab, long long n4, long long fold) {
   __shared__ float4 part[8][32];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const long long i = blockIdx.x * 32LL + x;
@@ -690,6 +690,10 @@ slab_sum_kernel(const float* __restrict__ slabs, bf16* __restrict__ out, int n_s
     for (int s = y; s < n_slabs; s += 8) {
       const float4 b = reinterpret_cast<const float4*>(slabs + s * slab)[i];
       a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+      if (fold > 0) {
+        const float4 c = reinterpret_cast<const float4*>(slabs + s * slab + fold)[i];
+        a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+      }
     }
   }
   part[y][x] = a;
@@ -1078,13 +1082,14 @@ int cb_gemm_bf16_slabs(const void* A, const void* B, float* C, int M, int N, int
   return dispatch<cb::EPI_STORE>(bn, a_mn, b_mn, ta, tb, tc, g, static_cast<cudaStream_t>(stream));
 }
 
-// out [M, N] bf16 without gaps = the sum of the slabs
-int cb_slab_sum(const float* slabs, void* out, int M, int N, int n_slabs, void* stream) {
+// out [M, N] bf16 without gaps = the sum of the slabs, whose rows (a multiple of 128) are those of the product; twice: a product of
+// 2 M rows, whose second M are added to the first
+int cb_slab_sum(const float* slabs, void* out, int M, int N, int n_slabs, int twice, void* stream) {
   if (M <= 0 || N <= 0 || N % 4 != 0 || n_slabs < 1) return -1;
-  const long long n4 = static_cast<long long>(M) * N / 4, blocks = (n4 + 31) / 32;
+  const long long n4 = static_cast<long long>(M) * N / 4, blocks = (n4 + 31) / 32, rows = (M * (twice ? 2LL : 1LL) + 127) / 128 * 128;
   if (blocks > 0x7fffffffLL) return -1;
   cb::slab_sum_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      slabs, static_cast<cb::bf16*>(out), n_slabs, static_cast<long long>((M + 127) / 128 * 128) * N, n4);
+      slabs, static_cast<cb::bf16*>(out), n_slabs, rows * N, n4, twice ? static_cast<long long>(M) * N : 0);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -1241,8 +1241,81 @@ class _LinearDistillFn(torch.autograd.Function):
                 gemm(Gc, hidden, a_mn=True, b_mn=True, out=dw[c0:c0 + vc])
         if slabs > 1:
             dh = torch.empty(M, K, dtype=hidden.dtype, device=dev)
-            _ext.check(L.cb_slab_sum(parts.data_ptr(), dh.data_ptr(), M, K, slabs, _ext.stream_ptr()), "slab_sum")
+            _ext.check(L.cb_slab_sum(parts.data_ptr(), dh.data_ptr(), M, K, slabs, 0, _ext.stream_ptr()), "slab_sum")
         return dh.to(hidden.dtype) if need_dh else None, dw, None, None, None, None, None, None
+
+
+# Few tokens: the logits are kept (fp32) instead of formed again, since that reads the whole weight a third time.  Up to a quarter of
+# the hidden size of tokens: what the logits' way through memory and back costs is then below it.  Kernels' time, without / with:
+# 1 token, 102,400 words of 2048 444 / 290 us, 35 tokens, 151,936 words of 896 320 / 217, 200 345 / 302; 500 tokens, 102,400 words of
+# 2048 771 / 638.
+_HELD_LOGITS_BYTES = 1 << 28
+
+
+def _hold_logits(M: int, K: int, V: int) -> bool:
+    return 4 * M <= K and 4 * M * V <= _HELD_LOGITS_BYTES
+
+
+class _LinearDistillHeldFn(torch.autograd.Function):
+    """The same with the logits held: one product, the loss and its gradient as in ``_DistillLogitsFn``, two products.  Up to 64 tokens
+    d(logits) goes into the products as two bf16 numbers a value, the second what the rounding of the first left out: they fill
+    rows that a tile of 128 has anyway, and few tokens average few roundings out."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, idx, lg, labels, ignore_index, tau, reduction):
+        M, K = hidden.shape
+        V = weight.shape[0]
+        ld = -(-V // 8) * 8
+        z = torch.empty(M, ld, dtype=torch.float32, device=hidden.device)
+        gemm(hidden, weight, out=z[:, :V] if V < ld else z)
+        each = reduction == "none"
+        buf = torch.empty(M * (2 + idx.shape[1]) + 1 + (1 if each else M), dtype=torch.float32, device=hidden.device)
+        loss = torch.empty((M,) if each else (), dtype=torch.float32, device=hidden.device)
+        stats = buf.data_ptr()
+        n, other, q = stats + 8 * M, stats + 8 * M + 4, stats + 8 * M + (8 if each else 4 + 4 * M)
+        code = _ext.lib().cb_kd_logits(z.data_ptr(), M, ld, V, 0, *_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau,
+                                       int(reduction == "mean"), stats, q, loss.data_ptr() if each else other,
+                                       other if each else loss.data_ptr(), n, _ext.stream_ptr())
+        _ext.check(code, "kd_logits")
+        ctx.save_for_backward(hidden, weight, idx, lg, labels, buf, z)
+        ctx.cfg = (ignore_index, tau, reduction)
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        hidden, weight, idx, lg, labels, buf, z = ctx.saved_tensors
+        ignore_index, tau, reduction = ctx.cfg
+        L = _ext.lib()
+        M, K = hidden.shape
+        V, ld = weight.shape[0], z.stride(0)
+        dev = hidden.device
+        grad = grad if grad.dtype == torch.float32 and grad.is_contiguous() else grad.float().contiguous()
+        each = reduction == "none"
+        stats, g = buf.data_ptr(), grad.data_ptr()
+        n, q = stats + 8 * M, stats + 8 * M + (8 if each else 4 + 4 * M)
+        two = M <= 64
+        R = 2 * M if two else M
+        G = torch.empty(R, ld, dtype=torch.bfloat16, device=dev)
+        code = L.cb_kd_logits_grad_split(z.data_ptr(), G.data_ptr(), G.data_ptr() + 2 * M * ld if two else None, M, ld, ld, V,
+                                         *_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau, stats, q, None if each else g,
+                                         n if reduction == "mean" else None, g if each else None, _ext.stream_ptr())
+        _ext.check(code, "kd_logits_grad_split")
+        Gv = G[:, :V] if V < ld else G
+        dh = dw = None
+        if ctx.needs_input_grad[0]:
+            slabs = L.cb_gemm_slabs(R, K, V, 0, 1, _sm_count(dev))
+            if slabs > 1 or two:
+                parts = torch.empty(slabs, -(-R // 128) * 128, K, dtype=torch.float32, device=dev)
+                code = L.cb_gemm_bf16_slabs(G.data_ptr(), weight.data_ptr(), parts.data_ptr(), R, K, V, ld, weight.stride(0), 0, 1, slabs, 0,
+                                            _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr())
+                _ext.check(code, "gemm_bf16_slabs")
+                dh = torch.empty(M, K, dtype=hidden.dtype, device=dev)
+                _ext.check(L.cb_slab_sum(parts.data_ptr(), dh.data_ptr(), M, K, slabs, int(two), _ext.stream_ptr()), "slab_sum")
+            else:
+                dh = gemm(Gv, weight, b_mn=True)
+        if ctx.needs_input_grad[1]:
+            dw = gemm(Gv, torch.cat((hidden, hidden)) if two else hidden, a_mn=True, b_mn=True)
+        return dh, dw, None, None, None, None, None, None
 
 
 def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor,
@@ -1263,7 +1336,8 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indi
         if not _gemm_ok(h) or h.stride(0) < h.shape[1]:
             h = h.clone(memory_format=torch.contiguous_format)
         lg = lg.float() if lg.dtype == torch.float64 else lg
-        loss = _LinearDistillFn.apply(h, weight, idx, lg, y, ignore_index, float(temperature), reduction)
+        fn = _LinearDistillHeldFn if _hold_logits(h.shape[0], h.shape[1], weight.shape[0]) else _LinearDistillFn
+        loss = fn.apply(h, weight, idx, lg, y, ignore_index, float(temperature), reduction)
         return loss.view(lead) if reduction == "none" else loss
     wide = torch.float64 if h.dtype == torch.float64 else torch.float32
     rows, valid = ref.distillation_rows(h.to(wide) @ weight.to(wide).t(), idx, lg, float(temperature), y, ignore_index)

@@ -293,7 +293,7 @@ def test_product_in_slabs(M, N, K, n):
         assert code == 0
         want += a[:, :k].double() @ b.double()
         size += a[:, :k].double().abs() @ b.double().abs()
-    assert L.cb_slab_sum(slabs.data_ptr(), out.data_ptr(), M, N, n, _ext.stream_ptr()) == 0
+    assert L.cb_slab_sum(slabs.data_ptr(), out.data_ptr(), M, N, n, 0, _ext.stream_ptr()) == 0
     _ext.check_status()
     # the sums in 32 bits, a few roundings of the sum of sizes (n slabs of at least 64 products in one accumulator); then half a step
     assert _over(out.double() - want, torch.finfo(BF).eps / 2 * want.abs() + 2.0 ** -20 * size + 1e-12) == 0
@@ -309,7 +309,7 @@ def test_slabs_only_where_tiles_are_few():
             assert 1 <= n <= 96 and -(-(-(-K // 64)) // per) == n    # every slab of the first product is written
     assert L.cb_gemm_bf16_slabs(None, None, None, 0, 8, 8, 8, 8, 0, 1, 1, 0, None, None) == -1
     assert L.cb_gemm_bf16_slabs(None, None, None, 8, 6, 8, 8, 8, 0, 1, 1, 0, None, None) == -1
-    assert L.cb_slab_sum(None, None, 8, 6, 1, None) == -1
+    assert L.cb_slab_sum(None, None, 8, 6, 1, 0, None) == -1
 
 
 @pytest.mark.parametrize("linear", [False, True])
@@ -348,3 +348,30 @@ def test_blocks_of_rows_that_take_no_part(T, masked):
     for a, b in zip(got, want):
         assert ((a.double() - b).norm() <= 2.0 ** -7 * b.norm()).item()
     assert (got[0][labels == -100] == 0).all()
+
+
+@pytest.mark.parametrize("T,V", [(1, 4096), (7, 5001), (64, 3000), (65, 3000)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_gradients_of_few_tokens_are_rounded_once(T, V, reduction):
+    """Up to 64 tokens d(logits) keeps what its rounding left out: the gradients are half a step of bf16 off, value by value."""
+    H, K, tau = 512, 9, 1.3
+    g = torch.Generator(device=DEV).manual_seed(T)
+    h = torch.randn(T, H, device=DEV, generator=g).to(BF).requires_grad_()
+    w = (torch.randn(V, H, device=DEV, generator=g) / 12).to(BF).requires_grad_()
+    idx, lg = entries(T, V, K, device=DEV)
+    h64, w64 = h.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    rows, valid = definition(h64 @ w64.t(), idx, lg, tau)
+    up = torch.rand(T, device=DEV, generator=g) if reduction == "none" else torch.tensor(0.7, device=DEV)
+    want = torch.autograd.grad(rows.to(DEV) if reduction == "none" else rows.sum().to(DEV) / int(valid.sum()), (h64, w64), up.double())
+    got = torch.autograd.grad(ops.linear_distillation(h, w, idx, lg, tau, reduction=reduction), (h, w), up)
+    _ext.check_status()
+    with torch.no_grad():
+        # sizes that cancel in the sums: |d(logits)| |W| and |d(logits)|^T |H|, at most the softmax's and the teacher's part apart
+        p = torch.softmax(h64 @ w64.t() / tau, 1)
+        q = torch.zeros_like(p).scatter_add_(1, idx.clamp(0, V - 1), torch.softmax(lg.double().masked_fill((idx < 0) | (idx >= V), -1e9) / tau, 1))
+        scale = tau * (up.double()[:, None] if reduction == "none" else up.double() / int(valid.sum()))
+        size = ((p + q) * scale) @ w64.abs(), ((p + q) * scale).t() @ h64.abs()
+    for a, b, c in zip(got, want, size):
+        if T <= 64:                                    # two bf16 numbers leave 2^-16 of d(logits), p and q are 2^-19 off
+            assert _over(a.double() - b, torch.finfo(BF).eps / 2 * b.abs() + 2.0 ** -15 * c) == 0
+        assert (a.double() - b).norm() <= 2.0 ** -7 * b.norm()
