@@ -60,8 +60,8 @@ __device__ __forceinline__ bool locate_window_tile(const AttnArgs& a, int b, int
   for (int d0 = 0; d0 < a.n_docs; d0 += 32) {
     int st = 0, ln = 0;
     if (d0 + lane < a.n_docs) {
-      st = a.cu[d0 + lane];
-      ln = a.cu[d0 + lane + 1] - st;
+      st = min(max(a.cu[d0 + lane], 0), a.T);            // boundaries outside [0, T] or out of order lead to no address outside
+      ln = min(max(a.cu[d0 + lane + 1], st), a.T) - st;
     }
     const int nb = (ln + 127) >> 7, ns = min(nb, with_sinks), own = nb - ns;
     const int in_runs = BWD && ns > 0 ? ns * ((nb + a.sink_run - 1) / a.sink_run) : 0;
@@ -132,7 +132,7 @@ __device__ __forceinline__ void window_query_blocks(const AttnArgs& a, int jb, i
 // caller need not clear the output first.
 template <int D>
 __device__ __forceinline__ void zero_padding_rows(const AttnArgs& a, int beyond, int h) {
-  const int valid = a.cu[a.n_docs];
+  const int valid = max(a.cu[a.n_docs], 0);
   const long long row0 = static_cast<long long>(valid) + static_cast<long long>(beyond) * 128;
   constexpr int CH = D / 8;                            // 16-byte chunks per row of one head
   for (int i = threadIdx.x; i < 128 * CH; i += blockDim.x) {

@@ -787,9 +787,10 @@ def attention_qkv_packed(qkv: torch.Tensor, cu_seqlens: torch.Tensor, num_q_head
     projection output; returns ``[T, hq * D]``.
 
     With a ``window`` a query sees the last ``window`` tokens of its document, its own among them, and the document's first
-    ``sinks`` tokens; time and gradients then grow with the window instead of with the document.  Masked scores are dropped
-    whatever they hold, but a masked key's V row is multiplied by an exact zero, so V (and in the backward pass the output's
-    gradient) has to be finite."""
+    ``sinks`` tokens; time and gradients then grow with the window instead of with the document.  Documents do not reach each
+    other, nor does padding reach them, whatever they hold.  Within a document masked scores are dropped whatever they are, but
+    a masked key's V row is multiplied by an exact zero, so that V (and in the backward pass the output's gradient) has to be
+    finite.  The additions into dQ, dK and dV come in any order: their last bits of 32 differ from call to call."""
     from . import attention_cuda as _ac
     if window is not None or sinks:
         from .attention import window_band
@@ -1322,8 +1323,9 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indi
                         temperature: float = 1.0, labels: Optional[torch.Tensor] = None, ignore_index: int = -100,
                         reduction: str = "mean") -> torch.Tensor:
     """:func:`distillation_logits` of ``hidden @ weight.T`` without ever holding the ``[tokens, vocab]`` logits, as
-    :func:`linear_cross_entropy` is :func:`cross_entropy_logits`.  bf16 on CUDA runs on the kernels; the hidden states of rows that
-    take no part have to be finite."""
+    :func:`linear_cross_entropy` is :func:`cross_entropy_logits` (a few tokens' logits are held, in fp32).  bf16 on CUDA runs on the
+    kernels; the hidden states of rows that take no part have to be finite.  Like every product here it uses the device's one
+    workspace for split tiles: calls on two streams of a device must not overlap."""
     lead = hidden.shape[:-1]
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
         raise ValueError(f"linear_distillation: weight {tuple(weight.shape)} does not fit hidden states {tuple(hidden.shape)}")

@@ -9,6 +9,7 @@ Tokens at or after ``cu_seqlens[-1]`` are padding and produce zeros.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional, Sequence
 
 import torch
@@ -49,8 +50,12 @@ def _sdpa_docs(q, k, v, bounds: Sequence[int], causal: bool, scale: float) -> to
 
 def window_band(op: str, window: Optional[int], sinks: int, causal: bool = True) -> tuple:
     """``()`` without a window, else the checked ``(window, sinks)``."""
-    if isinstance(window, bool) or not (window is None or isinstance(window, int)) or isinstance(sinks, bool) or not isinstance(sinks, int):
-        raise ValueError(f"{op}: window {window!r} and sinks {sinks!r} must be whole numbers")
+    try:
+        if isinstance(window, bool) or isinstance(sinks, bool):
+            raise TypeError
+        window, sinks = None if window is None else operator.index(window), operator.index(sinks)
+    except TypeError:
+        raise ValueError(f"{op}: window {window!r} and sinks {sinks!r} must be whole numbers") from None
     if sinks < 0:
         raise ValueError(f"{op}: sinks {sinks} must not be negative")
     if window is None:

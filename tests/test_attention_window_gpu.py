@@ -183,3 +183,34 @@ def test_documents_keep_to_themselves(hq, hk, d, value):
     for rows in (slice(0, a), slice(b, T)):
         for x, y in ((o, want[0]), (g, want[1])):
             assert torch.isfinite(x[rows]).all() and (x[rows].double() - y[rows]).norm() <= 2.0 ** -7 * y[rows].norm()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bounds", [[0, 100, 5000], [0, 100, 60, 300], [-40, 100, 300], [0, 300, -7], [290, 10, 1 << 30]])
+def test_bad_boundaries_reach_no_other_memory(d, bounds):
+    """What such a batch gives is not defined; guards around every buffer stay as they are, and the next call is right."""
+    T, hq, hk, pad = 300, 2, 1, 256
+    qkv, do, cu = _inputs(hq, hk, d, [T], 0)
+    want = _run(qkv, do, cu, hq, hk, d, 40, 3)
+    nq, n = hq * d, (hq + 2 * hk) * d
+    buf = torch.full((pad + T * nq + pad,), 7.0, dtype=BF, device=DEV)
+    o = buf[pad:pad + T * nq].view(T, nq)
+    lse = torch.full((hq * T + 2 * pad,), 7.0, device=DEV)
+    bad = torch.tensor(bounds, dtype=torch.int32, device=DEV)
+    st = _ext.status_buffer(qkv.device).data_ptr()
+    at = qkv.data_ptr()
+    args = (len(bounds) - 1, T, hq, hk, d, n, n, n, nq)
+    assert _ext.lib().cb_attn_window_fwd(at, at + 2 * nq, at + 2 * (nq + hk * d), o.data_ptr(), lse.data_ptr() + 4 * pad, bad.data_ptr(), *args,
+                                         d ** -0.5, 40, 3, None, st, _ext.stream_ptr()) == 0
+    acc = torch.full((pad + hq * T // 4 * 4 + 64 + T * n + pad,), 7.0, device=DEV)
+    delta = acc.data_ptr() + 4 * pad
+    dq = delta + 4 * (-(-hq * T // 64) * 64)
+    g = torch.full((pad + T * n + pad,), 7.0, dtype=BF, device=DEV)
+    assert _ext.lib().cb_attn_window_bwd(at, at + 2 * nq, at + 2 * (nq + hk * d), o.data_ptr(), do.data_ptr(), lse.data_ptr() + 4 * pad,
+                                         bad.data_ptr(), *args, nq, d ** -0.5, 40, 3, None, delta, dq, dq + 4 * T * nq,
+                                         dq + 4 * T * (nq + hk * d), g.data_ptr() + 2 * pad, n, st, _ext.stream_ptr()) == 0
+    _ext.check_status()
+    for t, m in ((buf, T * nq), (lse, hq * T), (g, T * n)):
+        assert (t[:pad] == 7).all() and (t[pad + m:] == 7).all()
+    assert (acc[:pad] == 7).all() and (acc[-pad + 64:] == 7).all()
+    assert torch.equal(_run(qkv, do, cu, hq, hk, d, 40, 3)[0], want[0])
