@@ -674,7 +674,7 @@ class _QKRopeAxesFn(torch.autograd.Function):
     def backward(ctx, dqkv):
         cos, sin, pos = ctx.saved_tensors
         # the gradient that comes in may be another node's too: the rotated one goes to a buffer of its own
-        g = dqkv if _rope_axes_rows(dqkv) else dqkv.contiguous()
+        g = dqkv if _rope_axes_rows(dqkv) else dqkv.clone(memory_format=torch.contiguous_format)
         return _rope_axes_launch(g, torch.empty_like(g, memory_format=torch.contiguous_format), cos, sin, pos, *ctx.cfg[:-1],
                                  not ctx.cfg[-1]), None, None, None, None
 
@@ -711,7 +711,7 @@ def qk_rope_axes_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
         pos = position_ids.long()
         if pos.stride(1) != 1:
             pos = pos.contiguous()
-        cos, sin = cos.float().contiguous(), sin.float().contiguous()
+        cos, sin = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos.float().contiguous(), sin.float().contiguous()))
         cfg = (num_q_heads, num_kv_heads, head_dim, sections, bool(cyclic), bool(interleaved), bool(inverse))
         if torch.is_grad_enabled() and qkv.requires_grad:
             return _QKRopeAxesFn.apply(qkv, cos, sin, pos, cfg)

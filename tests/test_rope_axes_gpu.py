@@ -94,6 +94,23 @@ def test_gradient_leaves_the_incoming_one_as_it_is(pairs):
     _check(x.grad, turned(w, cos, sin, pos, ref.rope_axis_map(sec), hq + hk, d, pairs, inverse=True))
 
 
+def test_gradient_and_tables_off_the_16_byte_boundary():
+    T, hq, hk, d, sections = 13, 2, 1, 64, (8, 12, 12)
+    x, cos, sin, pos = _inputs(T, hq, hk, d, 3)
+    axes = ref.rope_axis_map(sections)
+    up = torch.randn(x.numel() + 3, device=DEV).to(torch.bfloat16)
+    wide = torch.empty(2, cos.numel() + 1, device=DEV)[:, 1:]
+    c, s = (w.copy_(t.flatten()).view_as(t) for w, t in zip(wide, (cos, sin)))
+    assert c.data_ptr() % 16 and up[3:].data_ptr() % 16
+    leaf = x.clone().requires_grad_()
+    y = ops.qk_rope_axes_(leaf * 1, c, s, pos, hq, hk, d, sections)
+    _check(y.detach(), turned(x, cos, sin, pos, axes, hq + hk, d, False))
+    # the gradient that reaches the node starts six bytes into that of the larger buffer
+    (g,) = torch.autograd.grad(torch.cat((x.new_zeros(3), y.flatten())), leaf, up)
+    want = turned(up[3:].view_as(x), cos, sin, pos, axes, hq + hk, d, False, True)
+    _check(g, want)
+
+
 def test_leaf_in_place_is_refused():
     x, cos, sin, pos = _inputs(4, 1, 1, 64, 1)
     with pytest.raises(RuntimeError):
