@@ -2105,10 +2105,13 @@ int attn_bwd(const void* q, const void* k, const void* v, const void* o, const v
     // 64, 8192 tokens, window 128: runs of 2 / 4 / 6 / 8 blocks 91 / 81 / 76 / 79 us), or than 3 where the grid leaves SMs free
     // (1024 tokens: 18 / 16 / 20 / 24, of 3 14).
     a.sink_run = std::max(tile_heads <= cbhost::num_sms() ? 3 : 6, (a.window + 127) / 128 + 1);
-    const long long tiles = (T + 127LL) / 128 + n_docs;
-    const long long all = tiles + (a.sinks + 127LL) / 128 * (tiles / a.sink_run + n_docs);
-    if (all > 65535) return -1;
-    grid.y = static_cast<unsigned>(all);
+    // A document of n blocks has min(n, s) key blocks with sinks and ceil(n / run) runs of each.  Longer runs where the grid would
+    // have too many rows (many sinks in documents of millions of tokens).
+    const long long tiles = (T + 127LL) / 128 + n_docs, with_sinks = (a.sinks + 127LL) / 128;
+    const auto rows = [&] { return tiles + with_sinks * tiles / a.sink_run + std::min(with_sinks * n_docs, tiles); };
+    while (rows() > 65535 && a.sink_run < T) a.sink_run *= 2;
+    if (rows() > 65535) return -1;
+    grid.y = static_cast<unsigned>(rows());
   }
   // D = 64 runs two CTAs of the phase-by-phase kernel on an SM where one of the pipelined kernel fits, so the pipelined one
   // wins where the grid does not fill the SMs twice over (1 x 2048 tokens, 14 heads: 44 against 80 us; 4 x 512: 23 / 26)

@@ -81,6 +81,14 @@ def test_long_documents(hq, hk, d, lens, window, sinks):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+def test_many_sinks_in_many_short_documents(d):
+    """Every document's whole length is sinks: no more tiles than its own blocks ask for."""
+    hq, hk, lens = 2, 1, [7] * 1100 + [300]
+    qkv, do, cu = _inputs(hq, hk, d, lens, 0)
+    _check(_run(qkv, do, cu, hq, hk, d, 2, 8000), _truth(qkv, do, hq, hk, d, lens, 2, 8000), hq, hk, d, sum(lens))
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_large_scores(d):
     """Scores of several hundreds: the running maximum moves, and most probabilities vanish."""
     hq, hk, lens = 4, 2, [700, 130]
