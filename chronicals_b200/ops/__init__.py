@@ -1246,15 +1246,12 @@ class _LinearDistillFn(torch.autograd.Function):
         return dh.to(hidden.dtype) if need_dh else None, dw, None, None, None, None, None, None
 
 
-# Few tokens: the logits are kept (fp32) instead of formed again, since that reads the whole weight a third time.  Up to a quarter of
-# the hidden size of tokens: what the logits' way through memory and back costs is then below it.  Kernels' time, without / with:
-# 1 token, 102,400 words of 2048 444 / 290 us, 35 tokens, 151,936 words of 896 320 / 217, 200 345 / 302; 500 tokens, 102,400 words of
-# 2048 771 / 638.
-_HELD_LOGITS_BYTES = 1 << 28
-
-
-def _hold_logits(M: int, K: int, V: int) -> bool:
-    return 4 * M <= K and 4 * M * V <= _HELD_LOGITS_BYTES
+# Up to a gigabyte of them, the logits are kept (fp32) for the backward pass instead of formed again: a product less, and the loss's
+# kernels on held logits.
+# Kernels' time, formed twice / held, microseconds: 120 tokens, 32,000 words of 256 63 / 50, 1000 tokens of 151,936 words 577 / 540;
+# words of 896: 65 tokens, 151,936 words 306 / 225, 8000 tokens, 8000 words 442 / 397, 1021 tokens, 151,936 words 1012 / 1000;
+# words of 2048: 500 tokens, 151,936 words 1185 / 1029, 2600 tokens, 102,400 words 4168 / 3089.
+_HELD_LOGITS_BYTES = 1 << 30
 
 
 class _LinearDistillHeldFn(torch.autograd.Function):
@@ -1323,8 +1320,8 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indi
                         temperature: float = 1.0, labels: Optional[torch.Tensor] = None, ignore_index: int = -100,
                         reduction: str = "mean") -> torch.Tensor:
     """:func:`distillation_logits` of ``hidden @ weight.T`` without ever holding the ``[tokens, vocab]`` logits, as
-    :func:`linear_cross_entropy` is :func:`cross_entropy_logits` (a few tokens' logits are held, in fp32).  bf16 on CUDA runs on the
-    kernels; the hidden states of rows that take no part have to be finite.  Like every product here it uses the device's one
+    :func:`linear_cross_entropy` is :func:`cross_entropy_logits`, unless a gradient is wanted and all of them in fp32 take
+    no more than a gigabyte.  bf16 on CUDA runs on the kernels; the hidden states of rows that take no part have to be finite.  Like every product here it uses the device's one
     workspace for split tiles: calls on two streams of a device must not overlap."""
     lead = hidden.shape[:-1]
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
@@ -1338,7 +1335,8 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indi
         if not _gemm_ok(h) or h.stride(0) < h.shape[1]:
             h = h.clone(memory_format=torch.contiguous_format)
         lg = lg.float() if lg.dtype == torch.float64 else lg
-        fn = _LinearDistillHeldFn if _hold_logits(h.shape[0], h.shape[1], weight.shape[0]) else _LinearDistillFn
+        grad = torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
+        fn = _LinearDistillHeldFn if grad and 4 * h.shape[0] * weight.shape[0] <= _HELD_LOGITS_BYTES else _LinearDistillFn
         loss = fn.apply(h, weight, idx, lg, y, ignore_index, float(temperature), reduction)
         return loss.view(lead) if reduction == "none" else loss
     wide = torch.float64 if h.dtype == torch.float64 else torch.float32

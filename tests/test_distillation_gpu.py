@@ -14,6 +14,13 @@ NEG = -math.inf
 BF = torch.bfloat16
 
 
+@pytest.fixture(params=["logits held", "logits formed twice"])
+def form(request, monkeypatch):
+    """The two forms of the loss from hidden states, whatever the size."""
+    if request.param == "logits formed twice":
+        monkeypatch.setattr(ops, "_HELD_LOGITS_BYTES", 0)
+
+
 def _truth(z, idx, lg, tau, labels, up=None):
     z = z.detach().double().requires_grad_()
     rows, valid = definition(z, idx, lg, tau, labels)
@@ -66,6 +73,7 @@ def test_held_logits(T, V, K, tau, dtype, gap):
 
 @pytest.mark.parametrize("T,H,V,K,tau", [(1, 64, 520, 3, 1.0), (130, 256, 4096, 16, 1.0), (300, 896, 5001, 33, 2.0), (257, 128, 32000, 64, 0.7),
                                          (77, 2048, 9000, 5, 1.5), (64, 72, 100, 130, 1.0)])
+@pytest.mark.usefixtures("form")
 def test_from_hidden_states(T, H, V, K, tau):
     g = torch.Generator(device=DEV).manual_seed(T + H)
     h = torch.randn(T, H, device=DEV, generator=g).to(BF).requires_grad_()
@@ -77,7 +85,8 @@ def test_from_hidden_states(T, H, V, K, tau):
     rows, valid = definition(z64, idx, lg, tau, labels)
     n = max(1, int(valid.sum()))
     loss = ops.linear_distillation(h, w, idx, lg, tau, labels)
-    got = ops.linear_distillation(h, w, idx, lg, tau, labels, reduction="none")
+    with torch.no_grad():
+        got = ops.linear_distillation(h, w, idx, lg, tau, labels, reduction="none")
     # a logit is a sum of H products in 32 bits: 2^-24 of the sum of their sizes, a few times over
     size = (h64.detach().abs() @ w64.detach().abs().t()).max().item()
     tol = _loss_tolerance(z64, tau) + tau * 2.0 ** -20 * size
@@ -91,6 +100,7 @@ def test_from_hidden_states(T, H, V, K, tau):
     _ext.check_status()
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("linear", [False, True])
 @pytest.mark.parametrize("reduction", ["sum", "none", "mean"])
 def test_reductions_and_upstream_gradient(linear, reduction):
@@ -112,6 +122,7 @@ def test_reductions_and_upstream_gradient(linear, reduction):
         assert (a.double() - b).norm() <= (2.0 ** -7 if linear else 1e-5) * b.norm()
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("linear", [False, True])
 @pytest.mark.parametrize("idx_type,lg_type", [(torch.int32, BF), (torch.int16, torch.float16), (torch.int64, torch.float64), (torch.int32, torch.float32)])
 def test_types_and_layouts_of_the_teacher(linear, idx_type, lg_type):
@@ -127,6 +138,7 @@ def test_types_and_layouts_of_the_teacher(linear, idx_type, lg_type):
     assert torch.equal(op(*x, wide[:, K:2 * K], lg.t().contiguous().t(), reduction="none"), want)
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("linear", [False, True])
 def test_one_index_several_times(linear):
     T, H, V = 9, 64, 300
@@ -144,6 +156,7 @@ def test_one_index_several_times(linear):
 
 
 # absent by the type's lowest value over a small temperature, by -inf, by an index outside; a row of the lowest values alone
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("linear", [False, True])
 def test_masked_entries(linear):
     T, H, V, K, tau = 6, 64, 400, 5, 0.5
@@ -169,6 +182,7 @@ def test_masked_entries(linear):
     assert torch.allclose(same, op(*x, idx, torch.zeros_like(lg), 1.0, reduction="none"))
 
 
+@pytest.mark.usefixtures("form")
 def test_rows_that_take_no_part_are_not_read():
     z = torch.full((4, 1000), math.nan, device=DEV)
     z[0] = 1.0
@@ -180,6 +194,7 @@ def test_rows_that_take_no_part_are_not_read():
     assert torch.isfinite(grad).all() and (grad[1:] == 0).all()
 
 
+@pytest.mark.usefixtures("form")
 def test_nothing_takes_part():
     z = torch.randn(3, 700, device=DEV, requires_grad=True)
     h, w = torch.randn(3, 64, device=DEV).to(BF).requires_grad_(), torch.randn(700, 64, device=DEV).to(BF).requires_grad_()
@@ -201,6 +216,7 @@ def test_student_logits_of_minus_infinity():
     assert torch.isfinite(torch.autograd.grad(rows[0], z)[0]).all()
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("linear", [False, True])
 def test_the_same_bits_every_time(linear):
     T, H, V, K = 500, 256, 20000, 32
@@ -216,6 +232,7 @@ def test_the_same_bits_every_time(linear):
         assert all(torch.equal(a, b) for a, b in zip(first, now))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("linear", [False, True])
 def test_captured_and_replayed(linear):
     T, H, V, K = 90, 64, 3000, 8
@@ -312,6 +329,7 @@ def test_slabs_only_where_tiles_are_few():
     assert L.cb_slab_sum(None, None, 8, 6, 1, 0, None) == -1
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("linear", [False, True])
 def test_loss_may_be_changed_in_place_before_the_backward_pass(linear):
     T, H, V, K = 30, 64, 500, 4
@@ -325,6 +343,7 @@ def test_loss_may_be_changed_in_place_before_the_backward_pass(linear):
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, x), want))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("T,masked", [(700, [(0, 300)]), (700, [(128, 384), (600, 700)]), (513, [(0, 512)]), (256, [(0, 256)]), (384, [(5, 380)])])
 def test_blocks_of_rows_that_take_no_part(T, masked):
     """Whole blocks of 128 masked rows are left out of the products, mixed ones are not; large logits in masked rows do no harm."""
