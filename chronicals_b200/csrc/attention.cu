@@ -17,7 +17,9 @@
 // head, dQ / dK / dV out by reduce-adds; attn_bwd3_kernel (one CTA an SM, every
 // product in flight beside the softmax, warps by role) or, for short documents of
 // head size 64, attn_bwd2_kernel (two CTAs an SM, one phase after another); with
-// attn_delta_kernel before and attn_bwd_finalize_kernel after it.
+// attn_delta_kernel before and attn_bwd_finalize_kernel after it.  Both backward
+// kernels have a form for a sliding window with sinks (WIN); its forward kernel is
+// in attention_window.cu.
 //
 // Every thread that owns a score row reads it from TMEM with tcgen05.ld, so the
 // softmax needs no cross-thread shuffles.  The same swizzled image of a [128 x 64]
@@ -1425,6 +1427,11 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 // out of dV and dK as long as their Q and dO are finite: 0 x NaN and 0 x inf are NaN, in this form as in the one above (and
 // so it is with the V rows of the next document in the forward pass).  What this form writes to a neighbour's rows is
 // zero whatever either document holds.
+// WIN, in both forms: only the query blocks that see the key block; those of a key block with sinks, which every later query
+// sees, are shared out over CTAs in runs.  Blocks that the diagonal or a window's edge cuts test their scores by a bit mask; rows
+// behind the document are cleared in shared memory, so that it may be followed by anything.  P stays in 32 bits for dS and is
+// rounded once, for dV: a window averages few roundings out.  28 / 4 heads of 128, 8192 tokens, window 2048: 602 us (877
+// TFLOP/s of visible pairs); phase by phase, 14 / 2 heads of 64, 9 documents in 8192 tokens, window 1024: 114 us.
 // What bounds it now: 6600 cycles an iteration, of which the products with the waits between the roles take 5900 and the
 // softmax with them 5200 when the other is left out; the reduce-adds of dQ cost 60 us of 720.
 // Measured (kernel alone): 2 x 4096 tokens, 28 / 4 heads of 128: 1144 -> 721 us (526 -> 834 TFLOP/s); 27 documents in 8192

@@ -45,8 +45,8 @@ __device__ __forceinline__ int lane_of_item(int& b, int mine) {
 // key block.  Key blocks that hold sinks are seen by every later query of their document: their query blocks are shared out over
 // CTAs in runs of a.sink_run, which come first.  blk: the block of the tile, run: of which run (-1: a key block without sinks).
 //
-// BY_WEIGHT (head size 64): two to 32 documents are handed out by weight, the blocks that a tile's loop visits, at most a.cap: first all tiles of full weight,
-// then those of every lower one, of which a document has at most one (14 / 2 heads of 64, 9 documents in 8192 tokens, window 1024,
+// BY_WEIGHT (head size 64): two to 32 documents are handed out by weight, the blocks that a tile's loop visits, at most a.cap: first
+// all tiles of full weight, then those of every lower one, of which a document has at most one (14 / 2 heads of 64, 9 documents in 8192 tokens, window 1024,
 // backward: 124 us in the order of the documents, 114 so).  More of them go in their order: a search through more lengths than a
 // register holds, level by level, takes longer than it saves (40 documents: 74 and 94 us).  A single document's tiles are in that
 // order already; with heads of 128, whose tiles take more rounds, the order of the documents is the faster one (16 documents, 28 / 4

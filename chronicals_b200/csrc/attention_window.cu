@@ -21,8 +21,8 @@
 //                  between them.
 // Bound by the softmax's chain: of 3150 cycles a block and warp (head size 64, two warps a scheduler) the exponentials take 1700
 // beside the other CTA's (1024 alone, 16 a clock and SM), the rest is loads, maxima and waits that follow one another; leaving
-// every MMA out saves 4 %.  Measured, 14 / 2 heads of 64, 32,768 tokens, window 4096: 612 us (737 TFLOP/s of visible pairs); 28 / 4 heads
-// of 128, 8192 tokens, window 2048: 215 us (983).  The form of attention.cu (64 keys a block, two score tiles) took 690 and 221 with
+// every MMA out saves 4 %.  Measured, 14 / 2 heads of 64, 32,768 tokens, window 4096: 612 to 635 us by GPU (737 to 710 TFLOP/s of visible
+// pairs); 28 / 4 heads of 128, 8192 tokens, window 2048: 215 to 224 us (983 to 943).  On the GPU of the lower figures the form of attention.cu (64 keys a block, two score tiles) took 690 and 221 with
 // the same arithmetic, 822 and 232 with one score an instruction.  Tried besides: three and four CTAs an SM with one 64-key score
 // tile each 658 and 654 / -, two threads a row 650 / 234, P V in halves with P's half freed early 669 / 218, some exponentials on
 // the FMA pipe 618 (one pair in eight) to 690.

@@ -149,6 +149,7 @@ struct KdAcc {
 
 // Loss of a row of held logits.  gridDim.y blocks of a cluster share a row; the first one joins their sums and adds the teacher's
 // side.  stats[row] = (M, 1 / sum), or (0, -1) for a row that takes no part; q_out[row, K] = the merged q of each entry.
+// 4095 x 151,936 bf16, 64 words a row, a fifth of the rows masked: 176 us, 5.7 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(CE_THREADS)
 kd_logits_kernel(const T* __restrict__ logits, long long ld, int V, const KdTeacher t, float c2, float2* __restrict__ stats,
@@ -239,7 +240,7 @@ kd_logits_kernel(const T* __restrict__ logits, long long ld, int V, const KdTeac
 }
 
 // d(loss) / dz of held logits.  A block takes a stretch of a row: the softmax's part for every value, then the values of the
-// teacher's words that lie in it once more, with theirs.
+// teacher's words that lie in it once more, with theirs.  At the size above: 367 us, 6.1 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(CE_THREADS)
 kd_logits_grad_kernel(const T* __restrict__ logits, T* __restrict__ dlogits, long long ld, long long ldd, int V, const KdTeacher t,
@@ -306,7 +307,8 @@ kd_logits_grad_kernel(const T* __restrict__ logits, T* __restrict__ dlogits, lon
 
 // d(loss) / dz of fp32 logits as bf16, for the products that follow; with `lo` also what the rounding left out, in a second set of rows
 // (the products of few tokens have room for twice as many rows, and add the two in 32 bits).  Rows of both on 16-byte boundaries,
-// their pitches multiples of 8; a thread takes 8 values.  Blocks and words as in the kernel above.
+// their pitches multiples of 8; a thread takes 8 values.  Blocks and words as in the kernel above.  1021 x 151,936, a fifth of the rows
+// masked: 131 us, 6.2 TB/s.
 __global__ void __launch_bounds__(CE_THREADS)
 kd_logits_grad_split_kernel(const float* __restrict__ logits, bf16* __restrict__ hi, bf16* __restrict__ lo, long long ld, long long ldg,
                             int V, const KdTeacher t, float c2, const float2* __restrict__ stats, const float* __restrict__ q,
@@ -399,7 +401,7 @@ kd_idle_kernel(const KdTeacher t, int V, long long M, int* __restrict__ idle) {
 // the teacher's words (dot products of the hidden row, kept in shared memory, with gathered weight rows: KD_DOTS rows a warp at
 // a time, so that as many loads are in flight), the loss, and coef[row, K] = p - q, what d(logits) holds at those words.
 // Bound by the gathers: K weight rows a token.  8192 x 896, 64 words a row, a fifth of the rows masked: 152 us (5 TB/s, part of it from
-// L2); 4 rows at a time 196, 8 278, 256 threads 181.
+// L2), 178 after the products with their clock; 4 rows at a time 196, 8 278, 256 threads 181 (against 152).
 constexpr int KD_DOTS = 2, KD_ROW_THREADS = 128;
 
 __global__ void __launch_bounds__(KD_ROW_THREADS)
@@ -491,7 +493,8 @@ kd_linear_rows_kernel(const bf16* __restrict__ hidden, long long ldh, const bf16
 }
 
 // G[row, i - c0] = gscale gout (p - q) for the teacher's words i in [c0, c0 + Vc), over the softmax's part that the product left.
-// words [M, K]: -1 for an absent entry.  A warp a row: every chunk looks at every entry, so the entries are read as plainly as can be.
+// words [M, K]: -1 for an absent entry.  A warp a row: every chunk looks at every entry, so the entries are read as plainly as can be
+// (8192 rows of 64 words, 19 chunks: 5 us each, as long as a launch).
 __global__ void __launch_bounds__(CE_THREADS)
 kd_place_kernel(bf16* __restrict__ G, long long ldg, int c0, int Vc, long long M, int K, const int* __restrict__ words,
                 const float* __restrict__ coef, const float* __restrict__ gscale, const float* __restrict__ gout) {

@@ -8,7 +8,8 @@
 // Bound by memory: Q | K is read and written once.  A warp takes one token, because everything that depends on the
 // token alone (its positions, the cos / sin values of its pairs) is then fetched once and kept in registers for all its
 // heads: a lane owns 8 pairs of every (32 / lanes-a-head)-th head.  The loads of up to ROPE_BATCH heads are in flight
-// before the positions are looked at, so the chain positions -> table -> rotation runs beside them.
+// before the positions are looked at, so the chain positions -> table -> rotation runs beside them.  28 / 4 heads of 128, 32,768 tokens:
+// 85 us, 6.3 TB/s; 14 / 2 heads of 64, 8192 tokens: 8.6 us (of 34 MB, partly from L2).
 //
 // Beyond the formula the destination may differ from the source (the backward pass leaves the gradient it was given as
 // it is): V is then copied along.
