@@ -62,7 +62,7 @@ inline int ce_cluster(long long rows, int nvec) {
   int split = 1;
   while (split < 8 && ((rows * split < 4LL * num_sms() && nvec / (2 * split) >= 2048) ||
                        (rows * split < 24LL * num_sms() && nvec / (2 * split) >= 4096) ||
-                       (2 * rows * split <= num_sms() && nvec >= 3072 && nvec / (2 * split) >= 512)))
+                       (2 * rows * split <= num_sms() && nvec / 3 >= 1024 && nvec / (2 * split) >= 512)))
     split *= 2;
   return split;
 }
