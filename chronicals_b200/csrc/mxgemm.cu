@@ -416,7 +416,10 @@ mxgemm2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int nt = t / g.num_m_pairs;
         const int a_row = mp * 2 * BM + static_cast<int>(rank) * BM;
         const int b_row = nt * P_BN + static_cast<int>(rank) * P_BNH;
-        const unsigned char* sfa_row = g.sfa + static_cast<size_t>(mp * 2 + static_cast<int>(rank)) * g.sf_kb4 * SF_BYTES;
+        // an odd number of row blocks leaves the last pair's second CTA rows outside the matrix: zeros, whatever their scale, and
+        // the scales end with the last block
+        const int sf_blk = min(mp * 2 + static_cast<int>(rank), (g.M + BM - 1) / BM - 1);
+        const unsigned char* sfa_row = g.sfa + static_cast<size_t>(sf_blk) * g.sf_kb4 * SF_BYTES;
         const unsigned char* sfb0 = g.sfb + static_cast<size_t>(nt) * 2 * g.sf_kb4 * SF_BYTES;
         const unsigned char* sfb1 = sfb0 + static_cast<size_t>(g.sf_kb4) * SF_BYTES;
         for (int kb = 0; kb < num_kb; ++kb) {
