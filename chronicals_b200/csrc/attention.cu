@@ -1423,6 +1423,10 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 //   warp 13     TMA loads (Q two blocks deep, dO one) and the statistics of the query rows
 // TMEM: S^T [0, 128) with P^T over the first half of each 32 columns, dP^T [128, 256), dV, dK, and dQ over dP^T (D = 128)
 // or in columns of its own (D = 64, where dP need not wait for dQ to leave).
+// WIDE (windowed, D = 64): 16 softmax warps of 32 query columns each, three Q stages, and dS^T in the last 64 columns besides, from
+// where dK takes it (dQ needs it the other way round, from shared memory): at this head size the softmax takes as long as the
+// products.  14 heads, 8192 tokens, window 4096: 357 us with 8 softmax warps and two stages, 315 with 16 and three, 307 with
+// dS^T in tensor memory besides (at D = 128 16 warps are slower: 80 registers a thread); some exponentials on the FMA pipe 313 to 320.
 // A document's last query block brings rows of the next one with it.  Their probabilities are exact zeros, which keeps them
 // out of dV and dK as long as their Q and dO are finite: 0 x NaN and 0 x inf are NaN, in this form as in the one above (and
 // so it is with the V rows of the next document in the forward pass).  What this form writes to a neighbour's rows is
@@ -1436,41 +1440,53 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 // softmax with them 5200 when the other is left out; the reduce-adds of dQ cost 60 us of 720.
 // Measured (kernel alone): 2 x 4096 tokens, 28 / 4 heads of 128: 1144 -> 721 us (526 -> 834 TFLOP/s); 27 documents in 8192
 // tokens, the same heads: 393 -> 274; 8 x 1024: 412 -> 310; 14 / 2 heads of 64: 1 x 2048 80 -> 44, 1 x 4096 160 -> 141.
-template <int D>
+template <int D, bool WIN>
 struct Bwd3Smem {
+  static constexpr bool WIDE = D == 64 && WIN;
+  static constexpr int SW = WIDE ? 16 : 8;            // softmax warps
+  static constexpr int THREADS = (SW + 8) * 32;       // the last two warps only complete a warpgroup
   static constexpr int TILE = 128 * D * 2;
   static constexpr int OFF_K = 0;
   static constexpr int OFF_V = TILE;
-  static constexpr int OFF_Q = 2 * TILE;              // 2 stages
+  static constexpr int OFF_Q = 2 * TILE;
+  static constexpr int NQ = WIDE ? 3 : 2;             // Q stages
   static constexpr int NDO = D == 64 ? 2 : 1;         // dO stages
-  static constexpr int OFF_DO = 4 * TILE;
-  static constexpr int OFF_DS = (4 + NDO) * TILE;     // bf16 [128 keys x 128 queries] operand image
+  static constexpr int OFF_DO = (2 + NQ) * TILE;
+  static constexpr int OFF_DS = (2 + NQ + NDO) * TILE;                   // bf16 [128 keys x 128 queries] operand image
   static constexpr int OFF_DQ = OFF_DS + 32768;       // 4 warps x 2 boxes of 32 rows x 32 fp32 columns
-  static constexpr int OFF_ST = OFF_DQ + 32768;       // 2 stages x (lse, delta) x 128 query rows
-  static constexpr int OFF_BAR = OFF_ST + 2048;
+  static constexpr int OFF_ST = OFF_DQ + 32768;       // NQ stages x (lse, delta) x 128 query rows
+  static constexpr int OFF_BAR = OFF_ST + NQ * 1024;
   static constexpr int SLACK = 768;                   // for the alignment to 1024; the base is checked
   static constexpr int TOTAL = OFF_BAR + 256 + SLACK;
 };
-static_assert(Bwd3Smem<128>::TOTAL <= 232448, "shared memory per CTA");
-static_assert(Bwd3Smem<128>::OFF_DQ - Bwd3Smem<128>::OFF_Q >= 8 * 4 * 4096 && Bwd3Smem<64>::OFF_DQ - Bwd3Smem<64>::OFF_Q >= 8 * 2 * 4096,
-              "boxes of dV and dK at the end");
-constexpr int BWD3_SOFTMAX_WARPS = 8;
-constexpr int BWD3_THREADS = 512;                     // warps 14 and 15 only complete the last warpgroup
-// registers a thread after the split: 256 x 144 + 128 x 144 + 128 x 80 = the 512 x 128 at launch
-constexpr int BWD3_REGS_SOFTMAX = 144, BWD3_REGS_DQ = 144, BWD3_REGS_ISSUE = 80;
+static_assert(Bwd3Smem<128, false>::TOTAL <= 232448 && Bwd3Smem<64, true>::TOTAL <= 232448, "shared memory per CTA");
+static_assert(Bwd3Smem<128, false>::OFF_DQ - Bwd3Smem<128, false>::OFF_Q >= 8 * 4 * 4096 &&
+              Bwd3Smem<64, false>::OFF_DQ - Bwd3Smem<64, false>::OFF_Q >= 8 * 2 * 4096, "boxes of dV and dK at the end");
+// registers a thread after the split: 256 x 144 + 128 x 144 + 128 x 80 = the 512 x 128 at launch; WIDE: 512 x 88 + 128 x 72 + 128 x 56
+// = the 768 x 80
+template <bool WIDE>
+struct Bwd3Regs {
+  static constexpr int LAUNCH = WIDE ? 80 : 128;
+  static constexpr int SOFTMAX = WIDE ? 88 : 144, DQ = WIDE ? 72 : 144, ISSUE = WIDE ? 56 : 80;
+};
+static_assert(512 * Bwd3Regs<true>::SOFTMAX + 128 * (Bwd3Regs<true>::DQ + Bwd3Regs<true>::ISSUE) <= 768 * Bwd3Regs<true>::LAUNCH,
+              "registers at launch");
 
 template <int D, bool WIN>
-__global__ void __launch_bounds__(BWD3_THREADS, 1)
+__global__ void __launch_bounds__(Bwd3Smem<D, WIN>::THREADS, 1)
 attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmdO,
                  const __grid_constant__ CUtensorMap tmdQ, const __grid_constant__ CUtensorMap tmdK,
                  const __grid_constant__ CUtensorMap tmdV, const AttnArgs a) {
-  using L = Bwd3Smem<D>;
+  using L = Bwd3Smem<D, WIN>;
+  using R = Bwd3Regs<L::WIDE>;
   constexpr int PANELS = D / 64;
   constexpr uint32_t TMEM_COLS = 512;
   constexpr bool DQ_APART = D == 64;                   // columns are left for a dQ of its own
   constexpr uint32_t C_S = 0, C_DP = 128, C_DQ = DQ_APART ? 256 + 2 * D : 128, C_DV = 256, C_DK = 256 + D;
-  constexpr int NDO = L::NDO;
+  constexpr uint32_t C_DS = 448;                       // WIDE: dS^T, the A operand of dK
+  // (stage and round of the Q ring are written out where they are used: as functions they cost the other forms 1 %)
+  constexpr int NDO = L::NDO, NQ = L::NQ, SW = L::SW;
   constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, 0, 0);          // K Q^T, V dO^T
   constexpr uint32_t IDESC_KV = umma_idesc_bf16(128, D, 0, 1);           // P^T dO, dS^T Q
   constexpr uint32_t IDESC_DQ = umma_idesc_bf16(128, D, 1, 1);           // dS K
@@ -1500,10 +1516,10 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   float* sStat = reinterpret_cast<float*>(smem + L::OFF_ST);             // [stage][lse * log2(e) | delta][128]
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* v_full = k_full + 1;
-  uint64_t* q_full = v_full + 1;                      // [2]
-  uint64_t* q_empty = q_full + 2;                      // [2] dK(i) complete
-  uint64_t* st_full = q_empty + 2;                     // [2] statistics written (free with the Q stage)
-  uint64_t* do_full = st_full + 2;                     // [2]
+  uint64_t* q_full = v_full + 1;                       // [NQ]
+  uint64_t* q_empty = q_full + NQ;                     // [NQ] dK(i) complete
+  uint64_t* st_full = q_empty + NQ;                    // [NQ] statistics written (free with the Q stage)
+  uint64_t* do_full = st_full + NQ;                    // [2]
   uint64_t* do_empty = do_full + 2;                    // [2] dV(i) complete
   uint64_t* s_full = do_empty + 2;                     // S(i) complete
   uint64_t* p_ready = s_full + 1;                      // an arrival per softmax warp: S(i) read, P(i) in TMEM
@@ -1522,10 +1538,10 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   if (tid == 0) {
     mbar_init(k_full, 1); mbar_init(v_full, 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1); mbar_init(st_full + i, 1); }
+    for (int i = 0; i < NQ; ++i) { mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1); mbar_init(st_full + i, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(do_full + i, 1); mbar_init(do_empty + i, 1); }
-    mbar_init(s_full, 1); mbar_init(p_ready, BWD3_SOFTMAX_WARPS);
-    mbar_init(dp_full, 1); mbar_init(ds_ready, BWD3_SOFTMAX_WARPS); mbar_init(ds_free, 1); mbar_init(dq_full, 1); mbar_init(dq_free, 4);
+    mbar_init(s_full, 1); mbar_init(p_ready, SW);
+    mbar_init(dp_full, 1); mbar_init(ds_ready, SW); mbar_init(ds_free, 1); mbar_init(dq_full, 1); mbar_init(dq_free, 4);
     mbar_fence_init();
     *abort_flag = a.status[0] != 0 ? 1 : 0;
   }
@@ -1543,16 +1559,16 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     __syncwarp();
     if (elect_one()) mbar_arrive(bar);
   };
-  CB_PHASE_DECL_T(384, 0);             // slot 0: the MMA warp, slot 1: a softmax thread
+  CB_PHASE_DECL_T((SW + 4) * 32, 0);             // slot 0: the MMA warp, slot 1: a softmax thread
   // every wait ends in a warp-wide vote, so that the lanes of a warp leave their loop together
   auto wait_w = [&](uint64_t* bar, int phase, int code) {
     ok = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort_flag, a.status, code) && ok);
     return ok;
   };
 
-  if (warp >= 12) {
-    reg_dec<BWD3_REGS_ISSUE>();        // the whole warpgroup at one place, before its warps part
-    if (warp == 13) {
+  if (warp >= SW + 4) {
+    reg_dec<R::ISSUE>();        // the whole warpgroup at one place, before its warps part
+    if (warp == SW + 5) {
       // ------------------------------------------------------------------ loads
       const int u_start = __shfl_sync(0xffffffffu, start, 0);
       const int u_jb = __shfl_sync(0xffffffffu, jb, 0), u_ib = __shfl_sync(0xffffffffu, ib, 0);
@@ -1575,9 +1591,9 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         for (int p = 0; p < PANELS; ++p) tma_load_2d(sK + p * 16384, &tmK, k_full, hkv * D + p * 64, u_start + u_jb * 128);
       }
       for (int it = 0; it < u_n; ++it) {
-        const int st = it & 1;
+        const int st = (NQ == 2 ? (it & 1) : it % NQ);
         const int row0 = u_start + (u_ib + it) * 128;
-        if (it >= 2 && !wait_w(q_empty + st, (it >> 1) - 1, CB_ERR_WAIT_EMPTY)) break;
+        if (it >= NQ && !wait_w(q_empty + st, (NQ == 2 ? (it >> 1) : it / NQ) - 1, CB_ERR_WAIT_EMPTY)) break;
         if (elect_one()) {
           mbar_expect_tx(q_full + st, L::TILE);
   #pragma unroll
@@ -1607,15 +1623,15 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
       }
       __syncwarp();
-    } else if (warp == 12) {
+    } else if (warp == SW + 4) {
       // ------------------------------------------------------------------ MMA issue
       const int u_n = __shfl_sync(0xffffffffu, n_it, 0);
       const uint32_t u_tmem = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t kA = smem_u32(sK), vA = smem_u32(sV), dsA = smem_u32(sdS);
       auto issue_s = [&](int it) {                       // S^T(it) = K Q(it)^T
-        if (!wait_w(q_full + (it & 1), it >> 1, CB_ERR_WAIT_FULL)) return;
-        if (WIN && (ib + it + 1) * 128 > len) zero_tile_rows<PANELS>(sQ + (it & 1) * L::TILE, len - (ib + it) * 128);   // 0 x NaN is NaN
-        const uint32_t qA = smem_u32(sQ + (it & 1) * L::TILE);
+        if (!wait_w(q_full + (NQ == 2 ? (it & 1) : it % NQ), (NQ == 2 ? (it >> 1) : it / NQ), CB_ERR_WAIT_FULL)) return;
+        if (WIN && (ib + it + 1) * 128 > len) zero_tile_rows<PANELS>(sQ + (NQ == 2 ? (it & 1) : it % NQ) * L::TILE, len - (ib + it) * 128);   // 0 x NaN is NaN
+        const uint32_t qA = smem_u32(sQ + (NQ == 2 ? (it & 1) : it % NQ) * L::TILE);
         tc_fence_after();
         if (elect_one()) {
   #pragma unroll
@@ -1664,7 +1680,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (it + 1 < u_n) issue_dp(it + 1);
           if (!ok || (it > 0 && !wait_w(dq_free, it - 1, CB_ERR_WAIT_TMEM_EMPTY))) break;
         }
-        const uint32_t qA = smem_u32(sQ + (it & 1) * L::TILE);
+        const uint32_t qA = smem_u32(sQ + (NQ == 2 ? (it & 1) : it % NQ) * L::TILE);
         tc_fence_after();
         if (elect_one()) {
   #pragma unroll
@@ -1673,9 +1689,10 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           umma_commit(dq_full);
   #pragma unroll
           for (int kk = 0; kk < 8; ++kk)                 // dK += dS^T Q
-            umma_f16_ss(u_tmem + C_DK, desc_kmajor(dsA, kk), desc_mnmajor(qA, kk), IDESC_KV, (it | kk) != 0);
+            if (L::WIDE) umma_f16_ts(u_tmem + C_DK, u_tmem + C_DS + kk * 8, desc_mnmajor(qA, kk), IDESC_KV, (it | kk) != 0);
+            else umma_f16_ss(u_tmem + C_DK, desc_kmajor(dsA, kk), desc_mnmajor(qA, kk), IDESC_KV, (it | kk) != 0);
           umma_commit(ds_free);
-          umma_commit(q_empty + (it & 1));
+          umma_commit(q_empty + (NQ == 2 ? (it & 1) : it % NQ));
         }
         CB_PHASE(3);
         if (!DQ_APART && it + 1 < u_n) {
@@ -1687,78 +1704,111 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       __syncwarp();
     }
-  } else if (warp >= 8) {
-    reg_inc<BWD3_REGS_DQ>();
+  } else if (warp >= SW) {
+    if constexpr (R::DQ >= R::LAUNCH) reg_inc<R::DQ>();
+    else reg_dec<R::DQ>();
     // ------------------------------------------------------------------ dQ: TMEM -> shared memory -> TMA reduce-add
     // Rows past the end of the document belong to the next one and get zeros; a box of nothing else stays here.
-    const int q4 = warp - BWD3_SOFTMAX_WARPS;
+    const int q4 = warp - SW;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     uint8_t* box = smem + L::OFF_DQ + q4 * 8192;
     for (int it = 0; it < n_it; ++it) {
       if (!wait_w(dq_full, it, CB_ERR_WAIT_TMEM_FULL)) break;
       tc_fence_after();
-      uint32_t dq[D / 32][32];
+      if constexpr (L::WIDE) {
+        // 32 columns at a time: 72 registers
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) tmem_ld_32x32(t_row + C_DQ + c * 32, dq[c]);
-      tmem_ld_wait();
-      tc_fence_before();
-      arrive_w(dq_free);
-      if ((ib + it) * 128 + q4 * 32 + lane >= len) {   // rows of the next document: nothing, whatever either holds
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t v[32];
+          tmem_ld_32x32(t_row + C_DQ + c * 32, v);
+          tmem_ld_wait();
+          if (c == D / 32 - 1) {
+            tc_fence_before();
+            arrive_w(dq_free);
+          }
+          if ((ib + it) * 128 + q4 * 32 + lane >= len) {                 // rows of the next document: zeros
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c)
+            for (int k = 0; k < 32; ++k) v[k] = 0u;
+          }
+          if (elect_one()) tma_store_wait_read<1>();
+          __syncwarp();
+          uint8_t* row = box + (c & 1) * 4096 + lane * 128;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) dq[c][k] = 0u;
-      }
+          for (int cc = 0; cc < 8; ++cc)
+            *reinterpret_cast<uint4*>(row + ((cc ^ (lane & 7)) << 4)) = make_uint4(v[4 * cc], v[4 * cc + 1], v[4 * cc + 2], v[4 * cc + 3]);
+          fence_async_smem();
+          __syncwarp();
+          if (elect_one()) {
+            if ((ib + it) * 128 + q4 * 32 < len)
+              tma_reduce_add_2d(&tmdQ, box + (c & 1) * 4096, h * D + c * 32, start + (ib + it) * 128 + q4 * 32);
+            tma_store_commit();
+          }
+        }
+      } else {
+        uint32_t dq[D / 32][32];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        if (elect_one()) tma_store_wait_read<1>();     // the box's reduce before last has been read
-        __syncwarp();
-        uint8_t* row = box + (c & 1) * 4096 + lane * 128;
+        for (int c = 0; c < D / 32; ++c) tmem_ld_32x32(t_row + C_DQ + c * 32, dq[c]);
+        tmem_ld_wait();
+        tc_fence_before();
+        arrive_w(dq_free);
+        if ((ib + it) * 128 + q4 * 32 + lane >= len) {   // rows of the next document: nothing, whatever either holds
 #pragma unroll
-        for (int cc = 0; cc < 8; ++cc)
-          *reinterpret_cast<uint4*>(row + ((cc ^ (lane & 7)) << 4)) =
-              make_uint4(dq[c][4 * cc], dq[c][4 * cc + 1], dq[c][4 * cc + 2], dq[c][4 * cc + 3]);
-        fence_async_smem();
-        __syncwarp();
-        if (elect_one()) {
-          CB_DEBUG_CHECK_ST(a.status, start + (ib + it) * 128 >= 0, CB_DBG_TMA_COORD, start + (ib + it) * 128);
-          if ((ib + it) * 128 + q4 * 32 < len)
-            tma_reduce_add_2d(&tmdQ, box + (c & 1) * 4096, h * D + c * 32, start + (ib + it) * 128 + q4 * 32);
-          tma_store_commit();
+          for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) dq[c][k] = 0u;
+        }
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          if (elect_one()) tma_store_wait_read<1>();     // the box's reduce before last has been read
+          __syncwarp();
+          uint8_t* row = box + (c & 1) * 4096 + lane * 128;
+#pragma unroll
+          for (int cc = 0; cc < 8; ++cc)
+            *reinterpret_cast<uint4*>(row + ((cc ^ (lane & 7)) << 4)) =
+                make_uint4(dq[c][4 * cc], dq[c][4 * cc + 1], dq[c][4 * cc + 2], dq[c][4 * cc + 3]);
+          fence_async_smem();
+          __syncwarp();
+          if (elect_one()) {
+            CB_DEBUG_CHECK_ST(a.status, start + (ib + it) * 128 >= 0, CB_DBG_TMA_COORD, start + (ib + it) * 128);
+            if ((ib + it) * 128 + q4 * 32 < len)
+              tma_reduce_add_2d(&tmdQ, box + (c & 1) * 4096, h * D + c * 32, start + (ib + it) * 128 + q4 * 32);
+            tma_store_commit();
+          }
         }
       }
     }
     if (elect_one()) tma_store_wait_read<0>();
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ P and dS: my key r, 64 query columns
-    reg_inc<BWD3_REGS_SOFTMAX>();
+    // ------------------------------------------------------------------ P and dS: my key r, COLS query columns
+    reg_inc<R::SOFTMAX>();
+    constexpr int NC = 16 / SW, COLS = NC * 32;          // chunks of 32 columns
     const int q4 = warp & 3, half = warp >> 2;
     const int r = q4 * 32 + lane;
     const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
-    const uint32_t t_s = t_row + C_S + half * 64, t_dp = t_row + C_DP + half * 64;
+    const uint32_t t_s = t_row + C_S + half * COLS, t_dp = t_row + C_DP + half * COLS;
     const float sl2 = a.scale * LOG2E;
     CB_PHASE(12);
     for (int it = 0; it < n_it; ++it) {
-      const float4* lse4 = reinterpret_cast<const float4*>(sStat + (it & 1) * 256 + half * 64);
+      const float4* lse4 = reinterpret_cast<const float4*>(sStat + (NQ == 2 ? (it & 1) : it % NQ) * 256 + half * COLS);
       const float4* dlt4 = lse4 + 32;
-      if (!wait_w(st_full + (it & 1), it >> 1, CB_ERR_WAIT_FULL)) break;
+      if (!wait_w(st_full + (NQ == 2 ? (it & 1) : it % NQ), (NQ == 2 ? (it >> 1) : it / NQ), CB_ERR_WAIT_FULL)) break;
       CB_PHASE(0);
       if (!wait_w(s_full, it, CB_ERR_WAIT_TMEM_FULL)) break;
       CB_PHASE(1);
       tc_fence_after();
-      uint32_t pk[2][16];
-      float pf[WIN ? 2 : 1][32];
+      uint32_t pk[NC][16];
+      float pf[WIN ? NC : 1][32];
       {
-        uint32_t s[2][32];
-        tmem_ld_32x32(t_s, s[0]);
-        tmem_ld_32x32(t_s + 32, s[1]);
+        uint32_t s[NC][32];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) tmem_ld_32x32(t_s + c * 32, s[c]);
         tmem_ld_wait();
         if (WIN && (ib + it == jb || (ib + it - jb) * 128 + 127 >= a.window)) {          // cut by the diagonal or by some query's window
           const int key = jb * 128 + r;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int at = (ib + it) * 128 + half * 64 + c * 32;
+          for (int c = 0; c < NC; ++c) {
+            const int at = (ib + it) * 128 + half * COLS + c * 32;
             const uint32_t see = ~low_bits(key - at) & (key < a.sinks ? 0xffffffffu : low_bits(key + a.window - at));
 #pragma unroll
             for (int k = 0; k < 32; ++k)
@@ -1768,12 +1818,12 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (!WIN && it == 0) {                         // the diagonal block: queries before my key see nothing of it
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
-            if (half * 64 + c < r) s[0][c] = 0xff800000u;                // -inf
-            if (half * 64 + 32 + c < r) s[1][c] = 0xff800000u;
+            if (half * COLS + c < r) s[0][c] = 0xff800000u;              // -inf
+            if (NC == 2 && half * COLS + 32 + c < r) s[NC - 1][c] = 0xff800000u;
           }
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < NC; ++c) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float4 l = lse4[c * 8 + k];
@@ -1805,7 +1855,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       tc_fence_after();
       if (WIN) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < NC; ++c) {
           uint32_t dp[32];
           tmem_ld_32x32(t_dp + c * 32, dp);
           tmem_ld_wait();
@@ -1821,12 +1871,12 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
         }
       } else {                                         // dS = P (dP - delta), over pk
-        uint32_t dp[2][32];
-        tmem_ld_32x32(t_dp, dp[0]);
-        tmem_ld_32x32(t_dp + 32, dp[1]);
+        uint32_t dp[NC][32];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) tmem_ld_32x32(t_dp + c * 32, dp[c]);
         tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < NC; ++c) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float4 d = dlt4[c * 8 + k];
@@ -1839,8 +1889,13 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       CB_PHASE(4);
       if (it > 0 && !wait_w(ds_free, it - 1, CB_ERR_WAIT_MISC)) break;
       CB_PHASE(5);
-      store_row_chunk32_packed(sdS, r, half * 2, pk[0]);
-      store_row_chunk32_packed(sdS, r, half * 2 + 1, pk[1]);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) store_row_chunk32_packed(sdS, r, half * NC + c, pk[c]);
+      if (L::WIDE) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) tmem_st_32x16(t_row + C_DS + (half * NC + c) * 16, pk[c]);
+        tmem_st_wait();
+      }
       tc_fence_before();
       fence_async_smem();
       arrive_w(ds_ready);
@@ -1850,13 +1905,16 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     // tiles, which nothing reads any more, and a TMA reduce-add each.
     if (ok && wait_w(ds_free, n_it - 1, CB_ERR_WAIT_MISC)) {
       tc_fence_after();
-      constexpr int NB = D / 64;                       // chunks of 32 columns of either that are this warp's
-      uint8_t* box = sQ + warp * 2 * NB * 4096;        // 8 warps x 2 NB boxes from the Q tiles on
+      // chunks of 32 columns that are this warp's: NB of dV and as many of dK; WIDE: one of either
+      constexpr int NB = L::WIDE ? 1 : D / 64, ALL = L::WIDE ? 1 : 2 * NB;
+      const int c0 = L::WIDE ? half & 1 : half * NB;
+      const auto of_dv = [&](int b) { return L::WIDE ? half < 2 : b < NB; };
+      uint8_t* box = sQ + warp * ALL * 4096;           // SW warps x ALL boxes from the Q tiles on
 #pragma unroll
-      for (int b = 0; b < 2 * NB; ++b) {
-        const int c = half * NB + b % NB;
+      for (int b = 0; b < ALL; ++b) {
+        const int c = c0 + b % NB;
         uint32_t v[32];
-        tmem_ld_32x32(t_row + (b < NB ? C_DV : C_DK) + c * 32, v);
+        tmem_ld_32x32(t_row + (of_dv(b) ? C_DV : C_DK) + c * 32, v);
         tmem_ld_wait();
         if (jb * 128 + r >= len) {                     // keys of the next document: nothing, whatever either holds
 #pragma unroll
@@ -1872,8 +1930,8 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int row0 = jb * 128 + q4 * 32;             // the warp's first key within the document
       if (row0 < len && elect_one()) {
 #pragma unroll
-        for (int b = 0; b < 2 * NB; ++b)
-          tma_reduce_add_2d(b < NB ? &tmdV : &tmdK, box + b * 4096, hkv * D + (half * NB + b % NB) * 32, start + row0);
+        for (int b = 0; b < ALL; ++b)
+          tma_reduce_add_2d(of_dv(b) ? &tmdV : &tmdK, box + b * 4096, hkv * D + (c0 + b % NB) * 32, start + row0);
         tma_store_commit();
         tma_store_wait_read<0>();                      // shared memory is released when the CTA exits
       }
@@ -2044,8 +2102,8 @@ template <int D, bool WIN>
 int launch_bwd3(dim3 grid, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mdo,
                 const CUtensorMap& mdq, const CUtensorMap& mdk, const CUtensorMap& mdv, const cb::AttnArgs& a) {
   static bool cfg = false;
-  if (!cfg) { const int e = set_smem(cb::attn_bwd3_kernel<D, WIN>, cb::Bwd3Smem<D>::TOTAL); if (e) return e; cfg = true; }
-  cb::attn_bwd3_kernel<D, WIN><<<grid, cb::BWD3_THREADS, cb::Bwd3Smem<D>::TOTAL, s>>>(mq, mk, mv, mdo, mdq, mdk, mdv, a);
+  if (!cfg) { const int e = set_smem(cb::attn_bwd3_kernel<D, WIN>, cb::Bwd3Smem<D, WIN>::TOTAL); if (e) return e; cfg = true; }
+  cb::attn_bwd3_kernel<D, WIN><<<grid, cb::Bwd3Smem<D, WIN>::THREADS, cb::Bwd3Smem<D, WIN>::TOTAL, s>>>(mq, mk, mv, mdo, mdq, mdk, mdv, a);
   return 0;
 }
 
@@ -2124,11 +2182,11 @@ int attn_bwd(const void* q, const void* k, const void* v, const void* o, const v
   // wins where the grid does not fill the SMs twice over (1 x 2048 tokens, 14 heads: 44 against 80 us; 4 x 512: 23 / 26)
   // or its loops are long (2 x 4096: 276 / 290; 4 x 2048, 32 heads: 403 / 350, so no earlier than 4096), unless the
   // documents are so short that a CTA is mostly set-up (20 x 100: 19 / 15).  Lengths as the average over the documents.
-  // With a window the loops are about as long for every document: only the grid decides (14 heads of 64: 2048 tokens, window 16
-  // and sinks 42 / 24 us, window 1024 47 / 40; 8192 tokens, window 128 / 1024 / 4096 79 / 87, 177 / 171, 364 / 362; 32 heads,
-  // 16,384 tokens, window 4096 1806 / 1895).
+  // With a window, where the pipelined one has twice the softmax warps, it wins from loops of 1024 tokens on (14 heads of 64, 8192
+  // tokens, window 128 / 1024 / 4096: phase by phase 62 / 176 / 353 us, pipelined 71 / 155 / 305; 4 x 2048, 32 heads, window 1024
+  // 274 / 270; 9 documents, 910 on average, window 1024 114 / 119; 27 x 300 69 / 83; 32 heads, 16,384 tokens, window 4096 1860 / 1594).
   const bool few = tile_heads <= 2LL * cbhost::num_sms() && (window > 0 || T >= 512LL * n_docs);
-  if (D == 64 && !few && (window > 0 || T < 4096LL * n_docs)) {
+  if (D == 64 && !few && (window > 0 ? std::min<long long>(window, T / n_docs) < 1024 : T < 4096LL * n_docs)) {
     e = window > 0 ? launch_bwd2<64, true>(grid, s, mq, mk, mv, mdo, mdq, a) : launch_bwd2<64, false>(grid, s, mq, mk, mv, mdo, mdq, a);
     if (e) return e;
   } else {
