@@ -1739,6 +1739,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           fence_async_smem();
           __syncwarp();
           if (elect_one()) {
+            CB_DEBUG_CHECK_ST(a.status, start + (ib + it) * 128 >= 0, CB_DBG_TMA_COORD, start + (ib + it) * 128);
             if ((ib + it) * 128 + q4 * 32 < len)
               tma_reduce_add_2d(&tmdQ, box + (c & 1) * 4096, h * D + c * 32, start + (ib + it) * 128 + q4 * 32);
             tma_store_commit();
