@@ -1423,7 +1423,7 @@ attn_bwd2_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 //   warp 13     TMA loads (Q two blocks deep, dO one) and the statistics of the query rows
 // TMEM: S^T [0, 128) with P^T over the first half of each 32 columns, dP^T [128, 256), dV, dK, and dQ over dP^T (D = 128)
 // or in columns of its own (D = 64, where dP need not wait for dQ to leave).
-// WIDE (windowed, D = 64): 16 softmax warps of 32 query columns each, three Q stages, and dS^T in the last 64 columns besides, from
+// WIDE (windowed, D = 64): 16 softmax warps of 32 query columns each (the others behind them), three Q stages, and dS^T in the last 64 columns besides, from
 // where dK takes it (dQ needs it the other way round, from shared memory): at this head size the softmax takes as long as the
 // products.  14 heads, 8192 tokens, window 4096: 357 us with 8 softmax warps and two stages, 315 with 16 and three, 307 with
 // dS^T in tensor memory besides (at D = 128 16 warps are slower: 80 registers a thread); some exponentials on the FMA pipe 313 to 320.
@@ -1479,7 +1479,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                  const __grid_constant__ CUtensorMap tmdQ, const __grid_constant__ CUtensorMap tmdK,
                  const __grid_constant__ CUtensorMap tmdV, const AttnArgs a) {
   using L = Bwd3Smem<D, WIN>;
-  using R = Bwd3Regs<L::WIDE>;
+  constexpr int REGS_SOFTMAX = Bwd3Regs<L::WIDE>::SOFTMAX, REGS_DQ = Bwd3Regs<L::WIDE>::DQ, REGS_ISSUE = Bwd3Regs<L::WIDE>::ISSUE;
   constexpr int PANELS = D / 64;
   constexpr uint32_t TMEM_COLS = 512;
   constexpr bool DQ_APART = D == 64;                   // columns are left for a dQ of its own
@@ -1567,7 +1567,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   };
 
   if (warp >= SW + 4) {
-    reg_dec<R::ISSUE>();        // the whole warpgroup at one place, before its warps part
+    reg_dec<REGS_ISSUE>();             // the whole warpgroup at one place, before its warps part
     if (warp == SW + 5) {
       // ------------------------------------------------------------------ loads
       const int u_start = __shfl_sync(0xffffffffu, start, 0);
@@ -1704,9 +1704,9 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       __syncwarp();
     }
-  } else if (warp >= SW) {
-    if constexpr (R::DQ >= R::LAUNCH) reg_inc<R::DQ>();
-    else reg_dec<R::DQ>();
+  } else if (warp >> 2 == SW / 4) {
+    if constexpr (L::WIDE) reg_dec<REGS_DQ>();
+    else reg_inc<REGS_DQ>();
     // ------------------------------------------------------------------ dQ: TMEM -> shared memory -> TMA reduce-add
     // Rows past the end of the document belong to the next one and get zeros; a box of nothing else stays here.
     const int q4 = warp - SW;
@@ -1782,7 +1782,7 @@ attn_bwd3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ P and dS: my key r, COLS query columns
-    reg_inc<R::SOFTMAX>();
+    reg_inc<REGS_SOFTMAX>();
     constexpr int NC = 16 / SW, COLS = NC * 32;          // chunks of 32 columns
     const int q4 = warp & 3, half = warp >> 2;
     const int r = q4 * 32 + lane;
