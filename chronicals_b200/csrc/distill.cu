@@ -305,14 +305,27 @@ kd_logits_grad_kernel(const T* __restrict__ logits, T* __restrict__ dlogits, lon
   }
 }
 
+// The factor c of d(logits) as 2^k times a rest in [1, 2).  Products of bf16 d(logits) are formed with 2^k and their results multiplied by
+// the rest in 32 bits: at a teacher's only word p - Q is close to -1 in every row, and c would be rounded the same way in all of them (by
+// up to 2^-8, which no sum averages out).
+__device__ __forceinline__ float kd_unit(float c, float& rest) {
+  int e;
+  const float m = frexpf(c, &e);
+  const bool whole = c != 0.f && isfinite(c);
+  rest = whole ? 2.f * m : 1.f;
+  return whole ? ldexpf(1.f, e - 1) : c;
+}
+
 // d(loss) / dz of fp32 logits as bf16, for the products that follow; with `lo` also what the rounding left out, in a second set of rows
 // (the products of few tokens have room for twice as many rows, and add the two in 32 bits).  Rows of both on 16-byte boundaries,
-// their pitches multiples of 8; a thread takes 8 values.  Blocks and words as in the kernel above.  1021 x 151,936, a fifth of the rows
+// their pitches multiples of 8; a thread takes 8 values.  Blocks and words as in the kernel above.  With `rest` the factor is a power of
+// two, and rest[0] what is left of it.  1021 x 151,936, a fifth of the rows
 // masked: 131 us, 6.2 TB/s.
 __global__ void __launch_bounds__(CE_THREADS)
 kd_logits_grad_split_kernel(const float* __restrict__ logits, bf16* __restrict__ hi, bf16* __restrict__ lo, long long ld, long long ldg,
                             int V, const KdTeacher t, float c2, const float2* __restrict__ stats, const float* __restrict__ q,
-                            const float* __restrict__ gout, const float* __restrict__ n_rows, const float* __restrict__ grows) {
+                            const float* __restrict__ gout, const float* __restrict__ n_rows, const float* __restrict__ grows,
+                            float* __restrict__ rest) {
   const long long row = blockIdx.x;
   const float* lp = logits + row * ld;
   bf16* hp = hi + row * ldg;
@@ -322,6 +335,11 @@ kd_logits_grad_split_kernel(const float* __restrict__ logits, bf16* __restrict__
   if (gout != nullptr) g += n_rows != nullptr ? gout[0] / fmaxf(n_rows[0], 1.f) : gout[0];
   if (grows != nullptr) g += grows[row];
   g *= t.tau;
+  if (rest != nullptr) {
+    float left;
+    g = kd_unit(g, left);
+    if (blockIdx.y == 0 && row == 0 && threadIdx.x == 0) rest[0] = left;
+  }
   const bool valid = !(st.y == -1.f);
   const float gs = valid ? st.y * g : 0.f;
   const auto put = [&](int i, float v) {
@@ -361,10 +379,9 @@ kd_logits_grad_split_kernel(const float* __restrict__ logits, bf16* __restrict__
   }
 }
 
-// loss = mean (or sum) of the rows' losses, n_rows = rows that take part; with gscale also the factor of each row's
-// d(logits), tau / n, tau or 0.  stats.y == -1 marks the rows that take no part.  One block, a fixed order.
+// loss = mean (or sum) of the rows' losses, n_rows = rows that take part; with gscale also 1 for each of them and 0 for the others.  stats.y == -1 marks the rows that take no part.  One block, a fixed order.
 __global__ void __launch_bounds__(1024)
-kd_finalize_kernel(const float* __restrict__ loss_rows, const float2* __restrict__ stats, long long rows, int mean, float tau,
+kd_finalize_kernel(const float* __restrict__ loss_rows, const float2* __restrict__ stats, long long rows, int mean,
                    float* __restrict__ loss, float* __restrict__ n_rows, float* __restrict__ gscale) {
   __shared__ float red[32];
   float sum = 0.f, cnt = 0.f;
@@ -375,13 +392,12 @@ kd_finalize_kernel(const float* __restrict__ loss_rows, const float2* __restrict
   }
   sum = kd_block_sum(sum, red);
   cnt = kd_block_sum(cnt, red);
-  const float n = mean ? fmaxf(cnt, 1.f) : 1.f;
   if (threadIdx.x == 0) {
-    loss[0] = sum / n;
+    loss[0] = mean ? sum / fmaxf(cnt, 1.f) : sum;
     n_rows[0] = cnt;
   }
   if (gscale != nullptr)
-    for (long long i = threadIdx.x; i < rows; i += blockDim.x) gscale[i] = stats[i].y == -1.f ? 0.f : tau / n;
+    for (long long i = threadIdx.x; i < rows; i += blockDim.x) gscale[i] = stats[i].y == -1.f ? 0.f : 1.f;
 }
 
 // ------------------------------------------------------------------ from hidden states and the output weight
@@ -492,6 +508,24 @@ kd_linear_rows_kernel(const bf16* __restrict__ hidden, long long ldh, const bf16
   }
 }
 
+// The factor of d(logits) from hidden states: unit[0] = its power of two, unit[1] = the rest.  One thread.
+__global__ void kd_unit_kernel(const float* __restrict__ gout, const float* __restrict__ n_rows, float tau, float* __restrict__ unit) {
+  float left;
+  unit[0] = kd_unit(tau * gout[0] / (n_rows != nullptr ? fmaxf(n_rows[0], 1.f) : 1.f), left);
+  unit[1] = left;
+}
+
+// out = bf16(x times the rest): d(hidden) summed in 32 bits; n8 times 8 values
+__global__ void __launch_bounds__(256)
+kd_cast_kernel(const float4* __restrict__ x, uint4* __restrict__ out, long long n8, const float* __restrict__ rest) {
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  if (i >= n8) return;
+  const float r = rest != nullptr ? rest[0] : 1.f;
+  const float4 a = x[2 * i], b = x[2 * i + 1];
+  const float w[8] = {a.x * r, a.y * r, a.z * r, a.w * r, b.x * r, b.y * r, b.z * r, b.w * r};
+  out[i] = pack8(w);
+}
+
 // G[row, i - c0] = gscale gout (p - q) for the teacher's words i in [c0, c0 + Vc), over the softmax's part that the product left.
 // words [M, K]: -1 for an absent entry.  A warp a row: every chunk looks at every entry, so the entries are read as plainly as can be
 // (8192 rows of 64 words, 19 chunks: 5 us each, as long as a launch).
@@ -558,7 +592,7 @@ int cb_kd_logits(const void* logits, long long rows, long long ld, int V, int is
                                 : cudaLaunchKernelEx(&cfg, cb::kd_logits_kernel<float>, static_cast<const float*>(logits), ld, V, t, c2,
                                                      st, q, loss_rows);
   if (e != cudaSuccess) return static_cast<int>(e);
-  cb::kd_finalize_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(loss_rows, st, rows, mean, tau, loss, n_rows, nullptr);
+  cb::kd_finalize_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(loss_rows, st, rows, mean, loss, n_rows, nullptr);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -584,11 +618,11 @@ int cb_kd_logits_grad(const void* logits, void* dlogits, long long rows, long lo
   return static_cast<int>(cudaGetLastError());
 }
 
-// fp32 logits -> their gradient as bf16 hi [rows, V], and (lo not null) what the rounding left out
+// fp32 logits -> their gradient as bf16 hi [rows, V], and (lo not null) what the rounding left out; rest [1] or null
 int cb_kd_logits_grad_split(const float* logits, void* hi, void* lo, long long rows, long long ld, long long ldg, int V, const void* idx,
                             long long ld_idx, int idx64, const void* lg, long long ld_lg, int lg_bf16, int K, const long long* labels,
                             long long ignore_index, float tau, const float* stats, const float* q, const float* gout,
-                            const float* n_rows, const float* grows, void* stream) {
+                            const float* n_rows, const float* grows, float* rest, void* stream) {
   cb::KdTeacher t;
   if (rows <= 0 || rows > 0x7fffffffLL || V <= 0 || ld % 8 != 0 || ldg % 8 != 0 ||
       ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(hi) | reinterpret_cast<uintptr_t>(lo)) & 15) != 0 ||
@@ -598,7 +632,7 @@ int cb_kd_logits_grad_split(const float* logits, void* hi, void* lo, long long r
   while (split < 64 && rows * split < 4LL * cbhost::num_sms() && V / (2 * split) >= 2048) split *= 2;
   cb::kd_logits_grad_split_kernel<<<dim3(static_cast<unsigned>(rows), split), cb::CE_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(
       logits, static_cast<cb::bf16*>(hi), static_cast<cb::bf16*>(lo), ld, ldg, V, t, kd_scale(tau), reinterpret_cast<const float2*>(stats), q,
-      gout, n_rows, grows);
+      gout, n_rows, grows, rest);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -631,7 +665,23 @@ int cb_kd_linear_rows(const void* hidden, long long ldh, const void* weight, lon
       static_cast<const cb::bf16*>(hidden), ldh, static_cast<const cb::bf16*>(weight), ldw, H, V, M, part_m, part_s, n_splits, t,
       kd_scale(tau), lse, st, coef, words, loss_rows);
   CB_CHECK_CUDA(cudaGetLastError());
-  cb::kd_finalize_kernel<<<1, 1024, 0, s>>>(loss_rows, st, M, mean, tau, loss, n_rows, gscale);
+  cb::kd_finalize_kernel<<<1, 1024, 0, s>>>(loss_rows, st, M, mean, loss, n_rows, gscale);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// unit [2] for the backward pass from hidden states; n_rows null: a sum
+int cb_kd_unit(const float* gout, const float* n_rows, float tau, float* unit, void* stream) {
+  cb::kd_unit_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(gout, n_rows, tau, unit);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// out [n] bf16 = x [n] fp32 times rest[0] (null: 1); n a multiple of 8
+int cb_kd_cast(const float* x, void* out, long long n, const float* rest, void* stream) {
+  if (n <= 0 || n % 8 != 0 || ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) != 0) return -1;
+  const long long blocks = (n / 8 + 255) / 256;
+  if (blocks > 0x7fffffffLL) return -1;
+  cb::kd_cast_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      reinterpret_cast<const float4*>(x), static_cast<uint4*>(out), n / 8, rest);
   return static_cast<int>(cudaGetLastError());
 }
 

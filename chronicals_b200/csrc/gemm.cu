@@ -84,6 +84,7 @@ struct GemmArgs {
   int kb_per_split;
   int slab_rows;                  // > 0: every K range has an output of its own, slab_rows rows further down in C, which it
   int slab_add;                   // ... is written to, or (1) added to: one sum an element and launch, in a fixed order
+  const float* alpha;             // both operands [K, .] (a weight's gradient): C = alpha[0] A^T B; null: 1
 };
 
 template <int BLOCK_N, int STAGES>
@@ -360,6 +361,11 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                   for (int j = 0; j < 32; ++j) v[j] = 0.f;
                 }
               } else {
+                if (A_MN && B_MN && g.alpha != nullptr) {
+                  const float by = *g.alpha;
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v[j] *= by;
+                }
                 if (g.bias != nullptr) {
 #pragma unroll
                   for (int j = 0; j < 32; ++j)
@@ -527,6 +533,11 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                   for (int j = 0; j < 32; ++j) v[j] = 0.f;
                 }
               } else {
+                if (A_MN && B_MN && g.alpha != nullptr) {
+                  const float by = *g.alpha;
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v[j] *= by;
+                }
                 if (g.bias != nullptr) {
 #pragma unroll
                   for (int j = 0; j < 32; ++j)
@@ -680,7 +691,8 @@ cce_combine_rows_kernel(const float* __restrict__ part_m, const float* __restric
 // threads share the slabs of four values (fold > 0: and of those `fold` elements further on, which are added): few values and many slabs are bound by the latency of the loads (120 x 256 values, 50
 // slabs: 8.6 us with a thread for all of them).
 __global__ void __launch_bounds__(256)
-slab_sum_kernel(const float* __restrict__ slabs, bf16* __restrict__ out, int n_slabs, long long slab, long long n4, long long fold) {
+slab_sum_kernel(const float* __restrict__ slabs, bf16* __restrict__ out, int n_slabs, long long slab, long long n4, long long fold,
+                const float* __restrict__ scale) {
   __shared__ float4 part[8][32];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const long long i = blockIdx.x * 32LL + x;
@@ -704,7 +716,8 @@ slab_sum_kernel(const float* __restrict__ slabs, bf16* __restrict__ out, int n_s
     const float4 b = part[s][x];
     a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
   }
-  reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+  const float by = scale != nullptr ? scale[0] : 1.f;
+  reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16x2(a.x * by, a.y * by), pack_bf16x2(a.z * by, a.w * by));
 }
 
 // Single block: deterministic sum of per-row losses and the valid count; writes
@@ -749,6 +762,8 @@ __global__ void cce_finalize_kernel(const float* __restrict__ loss_rows, const l
 
 // =========================================================================================== host side
 extern "C" int cb_gemm2sm_supported(const void* C, long long ldc, int out_fp32);
+extern "C" int cb_gemm2sm_bf16_times(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb,
+                                     long long ldc, const float* alpha, int* status, void* stream);
 extern "C" int cb_gemm2sm_cost_ns(int M, int N, int K, int a_mn, int b_mn, int out_bytes, int sms);
 extern "C" int cb_gemm2sm_bf16(const void* A, const void* B, void* C, const void* bias, const void* addend, int M, int N,
                                int K, long long lda, long long ldb, long long ldc, long long ld_add, int a_mn, int b_mn,
@@ -897,9 +912,9 @@ int cb_glu_bwd_fused_pays(int M, int I, int K, int sms) {
 // C[M,N] = A * B^T (+bias) (+addend) (+C).  a_mn / b_mn: 0 when the operand is stored [M|N, K]
 // (K contiguous), 1 when stored [K, M|N].  lda/ldb/ldc/ld_add are row pitches in elements.
 // Returns 0 on a successful launch; negative for rejected arguments; positive CUDA error otherwise.
-int cb_gemm_bf16(const void* A, const void* B, void* C, const void* bias, const void* addend, int M, int N, int K,
-                 long long lda, long long ldb, long long ldc, long long ld_add, int a_mn, int b_mn, int out_fp32,
-                 int accumulate, int force_block_n, int* status, void* stream) {
+static int gemm_bf16(const void* A, const void* B, void* C, const void* bias, const void* addend, int M, int N, int K,
+                     long long lda, long long ldb, long long ldc, long long ld_add, int a_mn, int b_mn, int out_fp32,
+                     int accumulate, int force_block_n, const float* alpha, int* status, void* stream) {
   if (M <= 0 || N <= 0 || K <= 0) return -1;
   // force_block_n: 0 = choose (CTA-pair kernel or 128 / 256 wide single-CTA tiles), 128 / 256 = single-CTA tile
   // of that width, 2 = CTA-pair kernel
@@ -908,6 +923,8 @@ int cb_gemm_bf16(const void* A, const void* B, void* C, const void* bias, const 
     force_block_n = choose_kernel(M, N, K, a_mn, b_mn, out_fp32 ? 4 : 2, pairs_possible, num_sms());
     if (force_block_n == 0) force_block_n = 2;
   }
+  if (force_block_n == 2 && pairs_possible && alpha != nullptr)
+    return cb_gemm2sm_bf16_times(A, B, C, M, N, K, lda, ldb, ldc, alpha, status, stream);
   if (force_block_n == 2 && pairs_possible)
     return cb_gemm2sm_bf16(A, B, C, bias, addend, M, N, K, lda, ldb, ldc, ld_add, a_mn, b_mn, out_fp32, accumulate,
                            status, stream);
@@ -926,11 +943,25 @@ int cb_gemm_bf16(const void* A, const void* B, void* C, const void* bias, const 
   g.bias = static_cast<const cb::bf16*>(bias);
   g.addend = static_cast<const cb::bf16*>(addend);
   g.ld_add = ld_add;
+  g.alpha = alpha;
   g.status = status;
   CUtensorMap tc;
   e = build_out_map(&tc, &g.tma_store, C, M, N, ldc, out_fp32);
   if (e) return e;
   return dispatch<cb::EPI_STORE>(bn, a_mn, b_mn, ta, tb, tc, g, static_cast<cudaStream_t>(stream));
+}
+
+int cb_gemm_bf16(const void* A, const void* B, void* C, const void* bias, const void* addend, int M, int N, int K,
+                 long long lda, long long ldb, long long ldc, long long ld_add, int a_mn, int b_mn, int out_fp32,
+                 int accumulate, int force_block_n, int* status, void* stream) {
+  return gemm_bf16(A, B, C, bias, addend, M, N, K, lda, ldb, ldc, ld_add, a_mn, b_mn, out_fp32, accumulate, force_block_n, nullptr, status,
+                   stream);
+}
+
+// A weight's gradient times a number on the device: C [M, N] bf16 = alpha[0] A^T B with A [K, M], B [K, N]
+int cb_gemm_bf16_times(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
+                       const float* alpha, int* status, void* stream) {
+  return gemm_bf16(A, B, C, nullptr, nullptr, M, N, K, lda, ldb, ldc, 0, 1, 1, 0, 0, 0, alpha, status, stream);
 }
 
 // Split-K GEMM for skinny outputs: C[M,N] (fp32, zeroed here) = A * B^T with the K range cut into pieces so
@@ -1083,13 +1114,13 @@ int cb_gemm_bf16_slabs(const void* A, const void* B, float* C, int M, int N, int
 }
 
 // out [M, N] bf16 without gaps = the sum of the slabs, whose rows (a multiple of 128) are those of the product; twice: a product of
-// 2 M rows, whose second M are added to the first
-int cb_slab_sum(const float* slabs, void* out, int M, int N, int n_slabs, int twice, void* stream) {
+// 2 M rows, whose second M are added to the first; times scale[0] (null: 1)
+int cb_slab_sum(const float* slabs, void* out, int M, int N, int n_slabs, int twice, const float* scale, void* stream) {
   if (M <= 0 || N <= 0 || N % 4 != 0 || n_slabs < 1) return -1;
   const long long n4 = static_cast<long long>(M) * N / 4, blocks = (n4 + 31) / 32, rows = (M * (twice ? 2LL : 1LL) + 127) / 128 * 128;
   if (blocks > 0x7fffffffLL) return -1;
   cb::slab_sum_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      slabs, static_cast<cb::bf16*>(out), n_slabs, rows * N, n4, twice ? static_cast<long long>(M) * N : 0);
+      slabs, static_cast<cb::bf16*>(out), n_slabs, rows * N, n4, twice ? static_cast<long long>(M) * N : 0, scale);
   return static_cast<int>(cudaGetLastError());
 }
 

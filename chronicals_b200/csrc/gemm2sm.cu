@@ -69,6 +69,7 @@ struct Args {
   long long ld_add;
   const float* row_scale;  // fp8 operands: C = (A_q B_q^T) * row_scale[m] * col_scale[n]; null for bf16 operands
   const float* col_scale;
+  const float* alpha;      // both operands [K, .] (a weight's gradient): C = alpha[0] A^T B; null: 1
   int* status;
   // ---- tensor-parallel fusion (TP = 1 instantiations only; same contract as cb_gemm_bf16_tp in gemm.cu)
   // all-gather -> GEMM: the rows of A arrive in panels of `panel_pairs` 256-row tiles, one panel per source rank,
@@ -370,6 +371,11 @@ gemm2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         const float rs = row_ok ? g.row_scale[row] : 0.f;
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= rs * (col0 + j < g.N ? g.col_scale[col0 + j] : 0.f);
+      }
+      if (A_MN && B_MN && KIND == 0 && g.alpha != nullptr) {
+        const float by = *g.alpha;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= by;
       }
       if (g.bias != nullptr) {
 #pragma unroll
@@ -891,9 +897,9 @@ int cb_gemm2sm_cost_ns(int M, int N, int K, int a_mn, int b_mn, int out_bytes, i
 // a_mn / b_mn = 0 for operands stored [rows, K], 1 for [K, rows]; pitches in elements.
 // flags: bit 0 = never split tiles along K, bit 1 = split whenever the last round is partial (default: only when
 // it pays), bits 8.. = forced tile width (256, 224, 192; 0 = choose).
-int cb_gemm2sm_bf16_ex(const void* A, const void* B, void* C, const void* bias, const void* addend, int M, int N, int K,
-                       long long lda, long long ldb, long long ldc, long long ld_add, int a_mn, int b_mn, int out_fp32,
-                       int accumulate, int flags, int* status, void* stream) {
+static int gemm2sm_bf16(const void* A, const void* B, void* C, const void* bias, const void* addend, int M, int N, int K,
+                        long long lda, long long ldb, long long ldc, long long ld_add, int a_mn, int b_mn, int out_fp32,
+                        int accumulate, int flags, const float* alpha, int* status, void* stream) {
   if (M <= 0 || N <= 0 || K <= 0) return -1;
   if (!cb_gemm2sm_supported(C, ldc, out_fp32)) return -2;
   int bn = flags >> 8;
@@ -922,6 +928,7 @@ int cb_gemm2sm_bf16_ex(const void* A, const void* B, void* C, const void* bias, 
   g.bias = static_cast<const cb::bf16*>(bias);
   g.addend = static_cast<const cb::bf16*>(addend);
   g.ld_add = ld_add;
+  g.alpha = alpha;
   g.status = status;
   int pairs = cbhost::num_sms() / 2;
   if (pairs > g.num_tiles) pairs = g.num_tiles;
@@ -938,6 +945,19 @@ int cb_gemm2sm_bf16_ex(const void* A, const void* B, void* C, const void* bias, 
   if (bn == 256) return dispatch_layout<256>(a_mn, b_mn, ta, tb, tc, tw, g, pairs, s);
   if (bn == 224) return dispatch_layout<224>(a_mn, b_mn, ta, tb, tc, tw, g, pairs, s);
   return dispatch_layout<192>(a_mn, b_mn, ta, tb, tc, tw, g, pairs, s);
+}
+
+int cb_gemm2sm_bf16_ex(const void* A, const void* B, void* C, const void* bias, const void* addend, int M, int N, int K,
+                       long long lda, long long ldb, long long ldc, long long ld_add, int a_mn, int b_mn, int out_fp32,
+                       int accumulate, int flags, int* status, void* stream) {
+  return gemm2sm_bf16(A, B, C, bias, addend, M, N, K, lda, ldb, ldc, ld_add, a_mn, b_mn, out_fp32, accumulate, flags, nullptr, status,
+                      stream);
+}
+
+// C [M, N] bf16 = alpha[0] A^T B with A [K, M], B [K, N]; alpha: device memory, or null for 1
+int cb_gemm2sm_bf16_times(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
+                          const float* alpha, int* status, void* stream) {
+  return gemm2sm_bf16(A, B, C, nullptr, nullptr, M, N, K, lda, ldb, ldc, 0, 1, 1, 0, 0, 0, alpha, status, stream);
 }
 
 // Gate | up projection with the gated activation in the epilogue:

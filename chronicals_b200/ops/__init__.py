@@ -1205,31 +1205,37 @@ class _LinearDistillFn(torch.autograd.Function):
         status = _ext.status_buffer(dev)
         stats = buf.data_ptr()
         lse, gscale, coef, words = stats + 12 * M, stats + 16 * M, stats + 20 * M, stats + (20 + 4 * N) * M
+        need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        rest = None                                    # the results' factor: d(logits) are formed with a power of two
         if reduction == "none":                        # the factor of every row's d(logits) comes with the rows' gradients
             scale = buf[4 * M:5 * M] * grad
-            gscale, g1 = scale.data_ptr(), torch.ones(1, dtype=torch.float32, device=dev)
+            gscale, unit = scale.data_ptr(), torch.full((1,), tau, dtype=torch.float32, device=dev)
         else:
-            g1 = grad if grad.dtype == torch.float32 else grad.float()
-        need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+            unit = torch.empty(2, dtype=torch.float32, device=dev)
+            rest = unit.data_ptr() + 4
+            grad = grad if grad.dtype == torch.float32 else grad.float()
+            code = L.cb_kd_unit(grad.data_ptr(), stats + 4 * (buf.numel() - 1) if reduction == "mean" else None, tau, unit.data_ptr(),
+                                _ext.stream_ptr())
+            _ext.check(code, "kd_unit")
         Vc = _cce_chunk(M, K, V, _sm_count(dev))
         G = torch.empty(M, Vc, dtype=torch.bfloat16, device=dev)
-        # Sums over several chunks stay in fp32; one chunk is rounded where it is computed.  Few tokens make few tiles of dH with the
-        # whole vocabulary to sum over: ranges of it go to slabs of their own, which are added up at the end.
+        # Sums stay in fp32.  Few tokens make few tiles of dH with the whole vocabulary to sum over: ranges of it go to slabs of their
+        # own, which are added up at the end.
         slabs = _ext.lib().cb_gemm_slabs(M, K, min(Vc, V), 0, 1, _sm_count(dev)) if need_dh else 1
         dh = parts = None
         if slabs > 1:
             parts = torch.empty(slabs, -(-M // 128) * 128, K, dtype=torch.float32, device=dev)
         elif need_dh:
-            dh = torch.empty(M, K, dtype=torch.float32 if Vc < V else hidden.dtype, device=dev)
+            parts = torch.empty(M, K, dtype=torch.float32, device=dev)
         dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_dw else None
         for c0 in range(0, V, Vc):
             vc = min(Vc, V - c0)
             wc = weight[c0:c0 + vc]
-            code = L.cb_cce_dlogits_t(hidden.data_ptr(), wc.data_ptr(), None, lse, gscale, g1.data_ptr(),
+            code = L.cb_cce_dlogits_t(hidden.data_ptr(), wc.data_ptr(), None, lse, gscale, unit.data_ptr(),
                                       G.data_ptr(), M, vc, K, hidden.stride(0), weight.stride(0), G.stride(0), c0, V, 0.0, 0.0,
                                       math.log2(math.e) / tau, idle.data_ptr(), status.data_ptr(), _ext.stream_ptr())
             _ext.check(code, "cce_dlogits_t")
-            code = L.cb_kd_place(G.data_ptr(), G.stride(0), c0, vc, M, N, words, coef, gscale, g1.data_ptr(), _ext.stream_ptr())
+            code = L.cb_kd_place(G.data_ptr(), G.stride(0), c0, vc, M, N, words, coef, gscale, unit.data_ptr(), _ext.stream_ptr())
             _ext.check(code, "kd_place")
             Gc = G[:, :vc]
             if slabs > 1:
@@ -1237,13 +1243,19 @@ class _LinearDistillFn(torch.autograd.Function):
                                             slabs, int(c0 > 0), status.data_ptr(), _ext.stream_ptr())
                 _ext.check(code, "gemm_bf16_slabs")
             elif need_dh:   # dH += G_c @ W_c
-                gemm(Gc, wc, b_mn=True, out=dh, accumulate=c0 > 0)
+                gemm(Gc, wc, b_mn=True, out=parts, accumulate=c0 > 0)
             if need_dw:   # dW_c = G_c^T @ H
-                gemm(Gc, hidden, a_mn=True, b_mn=True, out=dw[c0:c0 + vc])
-        if slabs > 1:
+                code = L.cb_gemm_bf16_times(Gc.data_ptr(), hidden.data_ptr(), dw.data_ptr() + 2 * c0 * K, vc, K, M, Gc.stride(0),
+                                            hidden.stride(0), K, rest, status.data_ptr(), _ext.stream_ptr())
+                _ext.check(code, "gemm_bf16_times")
+        if need_dh:
             dh = torch.empty(M, K, dtype=hidden.dtype, device=dev)
-            _ext.check(L.cb_slab_sum(parts.data_ptr(), dh.data_ptr(), M, K, slabs, 0, _ext.stream_ptr()), "slab_sum")
-        return dh.to(hidden.dtype) if need_dh else None, dw, None, None, None, None, None, None
+            if slabs > 1:
+                code = L.cb_slab_sum(parts.data_ptr(), dh.data_ptr(), M, K, slabs, 0, rest, _ext.stream_ptr())
+            else:
+                code = L.cb_kd_cast(parts.data_ptr(), dh.data_ptr(), M * K, rest, _ext.stream_ptr())
+            _ext.check(code, "slab_sum" if slabs > 1 else "kd_cast")
+        return dh, dw, None, None, None, None, None, None
 
 
 # Up to a gigabyte of them, the logits are kept (fp32) for the backward pass instead of formed again: a product less, and the loss's
@@ -1294,25 +1306,34 @@ class _LinearDistillHeldFn(torch.autograd.Function):
         two = M <= 64
         R = 2 * M if two else M
         G = torch.empty(R, ld, dtype=torch.bfloat16, device=dev)
+        need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        unit = None if each or two else torch.empty(1, dtype=torch.float32, device=dev)        # as in _LinearDistillFn
         code = L.cb_kd_logits_grad_split(z.data_ptr(), G.data_ptr(), G.data_ptr() + 2 * M * ld if two else None, M, ld, ld, V,
                                          *_teacher_ptrs(idx, lg), _ext.ptr(labels), ignore_index, tau, stats, q, None if each else g,
-                                         n if reduction == "mean" else None, g if each else None, _ext.stream_ptr())
+                                         n if reduction == "mean" else None, g if each else None, _ext.ptr(unit), _ext.stream_ptr())
         _ext.check(code, "kd_logits_grad_split")
         Gv = G[:, :V] if V < ld else G
         dh = dw = None
-        if ctx.needs_input_grad[0]:
+        if need_dh:
             slabs = L.cb_gemm_slabs(R, K, V, 0, 1, _sm_count(dev))
+            dh = torch.empty(M, K, dtype=hidden.dtype, device=dev)
             if slabs > 1 or two:
                 parts = torch.empty(slabs, -(-R // 128) * 128, K, dtype=torch.float32, device=dev)
                 code = L.cb_gemm_bf16_slabs(G.data_ptr(), weight.data_ptr(), parts.data_ptr(), R, K, V, ld, weight.stride(0), 0, 1, slabs, 0,
                                             _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr())
                 _ext.check(code, "gemm_bf16_slabs")
-                dh = torch.empty(M, K, dtype=hidden.dtype, device=dev)
-                _ext.check(L.cb_slab_sum(parts.data_ptr(), dh.data_ptr(), M, K, slabs, int(two), _ext.stream_ptr()), "slab_sum")
+                code = L.cb_slab_sum(parts.data_ptr(), dh.data_ptr(), M, K, slabs, int(two), _ext.ptr(unit), _ext.stream_ptr())
+                _ext.check(code, "slab_sum")
             else:
-                dh = gemm(Gv, weight, b_mn=True)
-        if ctx.needs_input_grad[1]:
-            dw = gemm(Gv, torch.cat((hidden, hidden)) if two else hidden, a_mn=True, b_mn=True)
+                parts = torch.empty(M, K, dtype=torch.float32, device=dev)
+                gemm(Gv, weight, b_mn=True, out=parts)
+                _ext.check(L.cb_kd_cast(parts.data_ptr(), dh.data_ptr(), M * K, _ext.ptr(unit), _ext.stream_ptr()), "kd_cast")
+        if need_dw:
+            dw = torch.empty(V, K, dtype=weight.dtype, device=dev)
+            h = torch.cat((hidden, hidden)) if two else hidden
+            code = L.cb_gemm_bf16_times(G.data_ptr(), h.data_ptr(), dw.data_ptr(), V, K, R, ld, h.stride(0), K, _ext.ptr(unit),
+                                        _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr())
+            _ext.check(code, "gemm_bf16_times")
         return dh, dw, None, None, None, None, None, None
 
 

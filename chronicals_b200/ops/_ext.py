@@ -56,8 +56,11 @@ _PROTOTYPES = {
     "cb_kd_idle": [P, L, I, P, L, I, I, P, L, F, I, I, P, P],
     "cb_gemm_slabs": [I, I, I, I, I, I],
     "cb_gemm_bf16_slabs": [P, P, P, I, I, I, L, L, I, I, I, I, P, P],
-    "cb_slab_sum": [P, P, I, I, I, I, P],
-    "cb_kd_logits_grad_split": [P, P, P, L, L, L, I, P, L, I, P, L, I, I, P, L, F, P, P, P, P, P, P],
+    "cb_slab_sum": [P, P, I, I, I, I, P, P],
+    "cb_gemm_bf16_times": [P, P, P, I, I, I, L, L, L, P, P, P],
+    "cb_kd_unit": [P, P, F, P, P],
+    "cb_kd_cast": [P, P, L, P, P],
+    "cb_kd_logits_grad_split": [P, P, P, L, L, L, I, P, L, I, P, L, I, I, P, L, F, P, P, P, P, P, P, P],
     "cb_kd_max_entries": [],
     "cb_kd_logits": [P, L, L, I, I, P, L, I, P, L, I, I, P, L, F, I, P, P, P, P, P, P],
     "cb_kd_logits_grad": [P, P, L, L, L, I, I, P, L, I, P, L, I, I, P, L, F, P, P, P, P, P, P],

@@ -310,7 +310,7 @@ def test_product_in_slabs(M, N, K, n):
         assert code == 0
         want += a[:, :k].double() @ b.double()
         size += a[:, :k].double().abs() @ b.double().abs()
-    assert L.cb_slab_sum(slabs.data_ptr(), out.data_ptr(), M, N, n, 0, _ext.stream_ptr()) == 0
+    assert L.cb_slab_sum(slabs.data_ptr(), out.data_ptr(), M, N, n, 0, None, _ext.stream_ptr()) == 0
     _ext.check_status()
     # the sums in 32 bits, a few roundings of the sum of sizes (n slabs of at least 64 products in one accumulator); then half a step
     assert _over(out.double() - want, torch.finfo(BF).eps / 2 * want.abs() + 2.0 ** -20 * size + 1e-12) == 0
@@ -326,7 +326,7 @@ def test_slabs_only_where_tiles_are_few():
             assert 1 <= n <= 96 and -(-(-(-K // 64)) // per) == n    # every slab of the first product is written
     assert L.cb_gemm_bf16_slabs(None, None, None, 0, 8, 8, 8, 8, 0, 1, 1, 0, None, None) == -1
     assert L.cb_gemm_bf16_slabs(None, None, None, 8, 6, 8, 8, 8, 0, 1, 1, 0, None, None) == -1
-    assert L.cb_slab_sum(None, None, 8, 6, 1, 0, None) == -1
+    assert L.cb_slab_sum(None, None, 8, 6, 1, 0, None, None) == -1
 
 
 @pytest.mark.usefixtures("form")
@@ -394,3 +394,32 @@ def test_gradients_of_few_tokens_are_rounded_once(T, V, reduction):
         if T <= 64:                                    # two bf16 numbers leave 2^-16 of d(logits), p and q are 2^-19 off
             assert _over(a.double() - b, torch.finfo(BF).eps / 2 * b.abs() + 2.0 ** -15 * c) == 0
         assert (a.double() - b).norm() <= 2.0 ** -7 * b.norm()
+
+
+@pytest.mark.usefixtures("form")
+@pytest.mark.parametrize("T,V,H", [(151, 20000, 64), (302, 5000, 256), (605, 20000, 128)])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_the_factor_of_the_gradient_is_not_rounded(T, V, H, reduction):
+    """One word a row: d(logits) is close to the same number in every row, and its rounding would scale the whole gradient.  121 rows
+    (or 242, 484) take part: 1 / 121 is 2^-8.4 of itself off in bf16."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    h = torch.randn(T, H, device=DEV, generator=g).to(BF).requires_grad_()
+    w = (torch.randn(V, H, device=DEV, generator=g) / (8 * math.sqrt(H))).to(BF).requires_grad_()
+    idx, lg = torch.randint(0, V, (T, 1), device=DEV, generator=g), torch.zeros(T, 1, device=DEV)
+    labels = torch.where(torch.arange(T, device=DEV) < T // 5, -100, 0)
+    n = int((labels != -100).sum())
+    assert n % 121 == 0
+    h64, w64 = h.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    rows, _ = definition(h64 @ w64.t(), idx, lg, 1.0, labels)
+    want = torch.autograd.grad(rows.sum() / n, (h64, w64))
+    loss = ops.linear_distillation(h, w, idx, lg, 1.0, labels, reduction=reduction)
+    got = torch.autograd.grad(loss if reduction == "mean" else loss * (1.0 / n), (h, w))
+    _ext.check_status()
+    p = torch.softmax(h64 @ w64.t(), 1).max().item()
+    for a, b in zip(got, want):
+        # 1 - p is rounded to 1 or to the number below it: p off, or half a step of 2^-8.  The results' roundings, d at most 2^-8 each, are
+        # as often up as down: the sum of b^2 d over that of b^2 has a deviation of at most 2^-8 sqrt(sum b^4) / sum b^2.  (Few values
+        # carry the weight's gradient: the rows of the words.)
+        off = abs(((a.double() * b).sum() / (b * b).sum()).item() - 1)
+        assert off <= min(p, 2.0 ** -9) + 6 * 2.0 ** -8 * (b ** 4).sum().sqrt().item() / (b * b).sum().item(), off
+        assert (a.double() - b).norm() <= 2.0 ** -8 * b.norm()
