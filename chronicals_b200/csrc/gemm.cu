@@ -911,7 +911,7 @@ int cb_glu_bwd_fused_pays(int M, int I, int K, int sms) {
 
 // C[M,N] = A * B^T (+bias) (+addend) (+C).  a_mn / b_mn: 0 when the operand is stored [M|N, K]
 // (K contiguous), 1 when stored [K, M|N].  lda/ldb/ldc/ld_add are row pitches in elements.
-// Returns 0 on a successful launch; negative for rejected arguments; positive CUDA error otherwise.
+// Returns 0 on a successful launch; negative for rejected arguments; positive CUDA error otherwise.  alpha: see cb_gemm_bf16_times.
 static int gemm_bf16(const void* A, const void* B, void* C, const void* bias, const void* addend, int M, int N, int K,
                      long long lda, long long ldb, long long ldc, long long ld_add, int a_mn, int b_mn, int out_fp32,
                      int accumulate, int force_block_n, const float* alpha, int* status, void* stream) {
