@@ -1221,7 +1221,7 @@ class _LinearDistillFn(torch.autograd.Function):
         G = torch.empty(M, Vc, dtype=torch.bfloat16, device=dev)
         # Sums stay in fp32.  Few tokens make few tiles of dH with the whole vocabulary to sum over: ranges of it go to slabs of their
         # own, which are added up at the end.
-        slabs = _ext.lib().cb_gemm_slabs(M, K, min(Vc, V), 0, 1, _sm_count(dev)) if need_dh else 1
+        slabs = L.cb_gemm_slabs(M, K, min(Vc, V), 0, 1, _sm_count(dev)) if need_dh else 1
         dh = parts = None
         if slabs > 1:
             parts = torch.empty(slabs, -(-M // 128) * 128, K, dtype=torch.float32, device=dev)
@@ -1277,7 +1277,10 @@ class _LinearDistillHeldFn(torch.autograd.Function):
         V = weight.shape[0]
         ld = -(-V // 8) * 8
         z = torch.empty(M, ld, dtype=torch.float32, device=hidden.device)
-        gemm(hidden, weight, out=z[:, :V] if V < ld else z)
+        code = _ext.lib().cb_gemm_bf16(hidden.data_ptr(), weight.data_ptr(), z.data_ptr(), None, None, M, V, K, hidden.stride(0),
+                                       weight.stride(0), ld, 0, 0, 0, 1, 0, 0, _ext.status_buffer(hidden.device).data_ptr(),
+                                       _ext.stream_ptr())
+        _ext.check(code, "gemm_bf16")
         each = reduction == "none"
         buf = torch.empty(M * (2 + idx.shape[1]) + 1 + (1 if each else M), dtype=torch.float32, device=hidden.device)
         loss = torch.empty((M,) if each else (), dtype=torch.float32, device=hidden.device)
