@@ -57,7 +57,8 @@ inline int ce_split(long long rows, int V) {
 // since rows that are masked leave the rest unevenly spread over one round of blocks; or rows so few that they leave half the
 // SMs without a block.  Measured, bf16, one / two / four blocks a row: 16 x 32,000 6.2 / 5.4 / 4.4 us, 200 x 50,257 (one: 11 and
 // more) 9.7 / 10.4, 400 x 16,384 6.3 / 8.1, 100 x 8192 3.5 / 4.4; 2047 x 151,936 fp32, a fifth of the rows masked, 173 / 145;
-// 1000 x 100,000 bf16, half of them, 47 / 31.
+// 1000 x 100,000 bf16, half of them, 47 / 31.  Not with rows
+// for more than one round: 4095 x 151,936 bf16, a fifth masked (distillation), 175 / 190 / 217.
 inline int ce_cluster(long long rows, int nvec) {
   int split = 1;
   while (split < 8 && ((rows * split < 4LL * num_sms() && nvec / (2 * split) >= 2048) ||

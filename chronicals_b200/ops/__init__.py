@@ -790,7 +790,8 @@ def attention_qkv_packed(qkv: torch.Tensor, cu_seqlens: torch.Tensor, num_q_head
     ``sinks`` tokens; time and gradients then grow with the window instead of with the document.  Documents do not reach each
     other, nor does padding reach them, whatever they hold.  Within a document masked scores are dropped whatever they are, but
     a masked key's V row is multiplied by an exact zero, so that V (and in the backward pass the output's gradient) has to be
-    finite.  The additions into dQ, dK and dV come in any order: their last bits of 32 differ from call to call."""
+    finite.  The additions into dQ, dK and dV come in any order: their last bits of 32 differ from call to call.
+    A call takes up to 65,535 blocks of 128 tokens and documents together (8 million tokens)."""
     from . import attention_cuda as _ac
     if window is not None or sinks:
         from .attention import window_band
