@@ -80,6 +80,17 @@ def test_long_documents(hq, hk, d, lens, window, sinks):
     _check(_run(qkv, do, cu, hq, hk, d, window, sinks), _truth(qkv, do, hq, hk, d, lens, window, sinks), hq, hk, d, sum(lens))
 
 
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("lens,window,sinks", [([57, 59, 30, 84] * 10, 2000, 1), ([120] * 18, 33, 4), ([2300], 20, 0), ([900], 300, 2)])
+def test_gradients_of_few_visible_keys(hq, hk, d, lens, window, sinks):
+    """The gradient's own rounding, and that of P or dS before the products, as large and independent of it: the square root of two
+    roundings together.  That of O, which the row sums would take in, is kept out where few keys are visible."""
+    qkv, do, cu = _inputs(hq, hk, d, lens, 0)
+    g64 = _truth(qkv, do, hq, hk, d, lens, window, sinks)[1]
+    g = _run(qkv, do, cu, hq, hk, d, window, sinks)[1]
+    assert (g.double() - g64).norm() <= 1.5 * (g64.to(BF).double() - g64).norm()
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_many_sinks_in_many_short_documents(d):
     """Every document's whole length is sinks: no more tiles than its own blocks ask for."""
