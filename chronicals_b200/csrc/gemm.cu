@@ -298,7 +298,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         lab = (l >= 0 && rel >= 0 && rel < g.N) ? static_cast<int>(rel) : -1;
         if (EPI == EPI_DLOGITS) {
           lse_r = g.lse[row];
-          gs = g.gscale[row] * g.gout[0];
+          gs = g.gscale[row];
+          if (gs != 0.f) gs *= g.gout[0];              // a row that takes no part: zero, also where gout overflowed
           coef = 1.f + 2.f * g.z_weight * lse_r;
         }
       }

@@ -1209,7 +1209,7 @@ class _LinearDistillFn(torch.autograd.Function):
         need_dh, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         rest = None                                    # the results' factor: d(logits) are formed with a power of two
         if reduction == "none":                        # the factor of every row's d(logits) comes with the rows' gradients
-            scale = buf[4 * M:5 * M] * grad
+            scale = torch.where(buf[4 * M:5 * M] != 0, grad, 0.0)     # of rows that take no part: zero, not 0 x whatever comes
             gscale, unit = scale.data_ptr(), torch.full((1,), tau, dtype=torch.float32, device=dev)
         else:
             unit = torch.empty(2, dtype=torch.float32, device=dev)
