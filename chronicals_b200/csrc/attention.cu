@@ -2024,8 +2024,8 @@ int set_smem(K kern, int bytes) {
 extern "C" {
 
 // q [T, hq, D] (row pitch ldq elements), k / v [T, hk, D]; cu: int32 [n_docs + 1] on the device.
-// o [T, hq, D] with pitch ldo; lse [hq, T] fp32.  Rows of o at or beyond cu[n_docs] (padding) are written as
-// zeros by the kernel, their lse entries are left untouched.  D is 64 or 128, hq a multiple of hk.
+// o [T, hq, D] with pitch ldo; lse [hq, T] fp32.  Rows of o before cu[0] and at or beyond cu[n_docs] (padding) are
+// written as zeros by the kernel, their lse entries are left untouched.  D is 64 or 128, hq a multiple of hk.
 int cb_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu, int n_docs, int T,
                 int hq, int hk, int D, long long ldq, long long ldk, long long ldv, long long ldo, float scale,
                 int* status, void* stream) {

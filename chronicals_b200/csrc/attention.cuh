@@ -127,16 +127,16 @@ __device__ __forceinline__ void window_query_blocks(const AttnArgs& a, int jb, i
   count = hi - lo;
 }
 
-// The grid holds at least ceil((T - cu[n_docs]) / 128) CTAs past the last tile (per head).  In the forward
-// kernels they write the zeros of the padding rows at or after cu[n_docs], 128 rows x D columns each, so the
-// caller need not clear the output first.
+// The grid of ceil(T / 128) + n_docs CTAs (per head) holds enough past the last tile for the rows of no document: where n rows lie
+// before cu[0] or at and after cu[n_docs] at least ceil(n / 128), since T - n tokens fill at most (T - n + 127 n_docs) / 128 tiles.  In the forward kernels they write
+// those rows' zeros, 128 rows x D columns each, so the caller need not clear the output first.
 template <int D>
 __device__ __forceinline__ void zero_padding_rows(const AttnArgs& a, int beyond, int h) {
-  const int valid = max(a.cu[a.n_docs], 0);
-  const long long row0 = static_cast<long long>(valid) + static_cast<long long>(beyond) * 128;
+  const int lead = min(max(a.cu[0], 0), a.T), valid = max(a.cu[a.n_docs], lead);
+  const long long row0 = static_cast<long long>(beyond) * 128;
   constexpr int CH = D / 8;                            // 16-byte chunks per row of one head
   for (int i = threadIdx.x; i < 128 * CH; i += blockDim.x) {
-    const long long t = row0 + i / CH;
+    const long long n = row0 + i / CH, t = n < lead ? n : n - lead + valid;
     if (t < a.T) reinterpret_cast<uint4*>(a.O + t * a.ldo + static_cast<long long>(h) * D)[i % CH] = make_uint4(0u, 0u, 0u, 0u);
   }
 }

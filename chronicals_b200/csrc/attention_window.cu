@@ -383,8 +383,8 @@ int launch(dim3 grid, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& 
 extern "C" {
 
 // q [T, hq, D] (row pitch ldq elements), k / v [T, hk, D]; cu: int32 [n_docs + 1] on the device; window >= 1, sinks >= 0.
-// o [T, hq, D] with pitch ldo; lse [hq, T] fp32.  Rows of o at or beyond cu[n_docs] (padding) are written as zeros, their
-// lse entries are left untouched.  o_lo (null: none), [T, hq, D] without gaps: what o's rounding left out, for the backward pass.
+// o [T, hq, D] with pitch ldo; lse [hq, T] fp32.  Rows of o before cu[0] and at or beyond cu[n_docs] (padding) are written as zeros,
+// their lse entries are left untouched.  o_lo (null: none), [T, hq, D] without gaps: what o's rounding left out, for the backward pass.
 // D is 64 or 128, hq a multiple of hk.
 int cb_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu, int n_docs, int T,
                        int hq, int hk, int D, long long ldq, long long ldk, long long ldv, long long ldo, float scale, int window,

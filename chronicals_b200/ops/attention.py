@@ -4,7 +4,8 @@ Replaces the reference's calls into flash-attn / SDPA
 (chronicals/kernels/flash_attention_optimizer.py:845-994, :1388-1462).
 Inputs are packed ``q [T, Hq, D]``, ``k/v [T, Hk, D]`` plus ``cu_seqlens``;
 the KV head of a query head is ``hq // (Hq // Hk)`` (no ``repeat_interleave``).
-Tokens at or after ``cu_seqlens[-1]`` are padding and produce zeros.
+Tokens before ``cu_seqlens[0]`` and at or after ``cu_seqlens[-1]`` are padding
+and produce zeros.
 """
 from __future__ import annotations
 

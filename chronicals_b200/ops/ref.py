@@ -193,11 +193,13 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, window: int, sinks: int,
                      scale: float) -> torch.Tensor:
     """:func:`attention_varlen` in which a query sees the last ``window`` tokens of its document, its own among them, and the
-    document's first ``sinks`` tokens.  A stretch of queries at a time, so that a long document never needs a square of scores."""
+    document's first ``sinks`` tokens.  A stretch of queries at a time, so that a long document never needs a square of scores.
+    Tokens before the first boundary and behind the last one belong to no document: zeros."""
     T, hq, d = q.shape
     rep = hq // k.shape[1]
     qf, kf, vf = ((t if t.dtype == torch.float64 else t.float()).transpose(0, 1) for t in (q, k, v))
-    out, bounds, stretch = [], cu_seqlens.tolist(), 512
+    bounds, stretch = cu_seqlens.tolist(), 512
+    out = [q.new_zeros(bounds[0], hq, d)]
     for a, b in zip(bounds[:-1], bounds[1:]):
         for r0 in range(a, b, stretch):
             r1 = min(b, r0 + stretch)
