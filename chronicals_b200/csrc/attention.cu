@@ -575,14 +575,15 @@ attn_delta_kernel(const bf16* __restrict__ dO, const bf16* __restrict__ O, long 
   if (in && sub == 0) delta[static_cast<long long>(h) * T + t] = s;
 }
 
-// The windowed form's: the same sum with what the rounding of O left out (o_lo, null: none), and the zeros of the accumulators
-// (zero: n4 vectors of 16 bytes), so that both pass memory at once.  14 / 2 heads of 64, 8253 tokens: 11.6 us, 14.9 apart.
-// delta is subtracted from dP, and with few visible keys the two are alike: with a window of two tokens the rounding of O alone
-// puts dQ 2.3 roundings off instead of 1.4.
+// The windowed form's: the same sum with what the rounding of O left out (o_lo, null: none; the rows that it has: LO_KEYS), and the
+// zeros of the accumulators (zero: n4 vectors of 16 bytes), so that both pass memory at once.  14 / 2 heads of 64, 8253 tokens: 11.6
+// us, 14.9 apart.  delta is subtracted from dP, and with few visible keys the two are alike: with a window of two tokens the rounding
+// of O alone puts dQ 2.3 roundings off instead of 1.4.
 template <int LANES>
 __global__ void __launch_bounds__(256)
 attn_window_delta_kernel(const bf16* __restrict__ dO, const bf16* __restrict__ O, const bf16* __restrict__ o_lo, long long ld_do,
-                         long long ld_o, int T, int hq, float* __restrict__ delta, uint4* __restrict__ zero, long long n4) {
+                         long long ld_o, int T, int hq, float* __restrict__ delta, uint4* __restrict__ zero, long long n4,
+                         const int* __restrict__ lo_index, int n_lo) {
   constexpr int D = LANES * 8;
   const long long gid = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x;
   const long long pair = gid / LANES;                       // (t, h) index, h fastest
@@ -591,16 +592,20 @@ attn_window_delta_kernel(const bf16* __restrict__ dO, const bf16* __restrict__ O
   float s = 0.f;
   long long t = 0;
   int h = 0;
+  int i_lo = -1;
   uint4 a, b, c = make_uint4(0u, 0u, 0u, 0u);
   if (in) {
     t = pair / hq;
     h = static_cast<int>(pair - t * hq);
+    i_lo = lo_index != nullptr ? lo_index[t] : static_cast<int>(t);
     const long long at = static_cast<long long>(h) * D + sub * 8;
     a = *reinterpret_cast<const uint4*>(dO + t * ld_do + at);
     b = *reinterpret_cast<const uint4*>(O + t * ld_o + at);
-    if (o_lo != nullptr) c = *reinterpret_cast<const uint4*>(o_lo + t * ld_o + at);
   }
   for (long long i = gid; i < n4; i += static_cast<long long>(gridDim.x) * blockDim.x) zero[i] = make_uint4(0u, 0u, 0u, 0u);
+  // (an index that is none of the rows: a token of no document)
+  if (in && o_lo != nullptr && (lo_index == nullptr || static_cast<unsigned>(i_lo) < static_cast<unsigned>(n_lo)))
+    c = *reinterpret_cast<const uint4*>(o_lo + i_lo * ld_o + static_cast<long long>(h) * D + sub * 8);
   if (in) {
     float x[8], y[8], z[8];
     unpack8(a, x);
@@ -2135,9 +2140,13 @@ int attn_bwd(const void* q, const void* k, const void* v, const void* o, const v
   if (window > 0) {
     if (!vec_ok || !joined || ldo != static_cast<long long>(hq) * D || (reinterpret_cast<uintptr_t>(o_lo) & 15) != 0) return -1;
     const unsigned blocks = static_cast<unsigned>((pairs * (D / 8) + 255) / 256);
+    const int n_lo = cb::lo_rows(T, n_docs, window);
+    const int* lo_index = o_lo != nullptr && !cb::lo_all(window)
+                              ? reinterpret_cast<const int*>(static_cast<const cb::bf16*>(o_lo) + n_lo * ldo) : nullptr;
     const auto kern = D == 64 ? cb::attn_window_delta_kernel<8> : cb::attn_window_delta_kernel<16>;
     kern<<<blocks, 256, 0, s>>>(static_cast<const cb::bf16*>(d_o), static_cast<const cb::bf16*>(o), static_cast<const cb::bf16*>(o_lo),
-                                ld_do, ldo, T, hq, delta, reinterpret_cast<uint4*>(dq_acc), static_cast<long long>((n_q + 2 * n_k) / 4));
+                                ld_do, ldo, T, hq, delta, reinterpret_cast<uint4*>(dq_acc), static_cast<long long>((n_q + 2 * n_k) / 4),
+                                lo_index, n_lo);
   } else if (vec_ok && D == 64) {
     cb::attn_delta_kernel<8><<<static_cast<unsigned>((pairs * 8 + 255) / 256), 256, 0, s>>>(
         static_cast<const cb::bf16*>(d_o), static_cast<const cb::bf16*>(o), ld_do, ldo, T, hq, delta);

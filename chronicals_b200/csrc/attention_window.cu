@@ -53,7 +53,8 @@ struct WinFwd {
 template <int D>
 __global__ void __launch_bounds__(WIN_THREADS, 2)
 attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const AttnArgs a) {
+                       const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const AttnArgs a,
+                       int* __restrict__ lo_index) {
   using L = WinFwd<D>;
   constexpr int NS = L::NS;
   constexpr int PANELS = D / 64;
@@ -61,9 +62,9 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   constexpr uint32_t IDESC_S = umma_idesc_bf16(128, 128, 0, 0);
   constexpr uint32_t IDESC_PV = umma_idesc_bf16(128, D, 0, 1);
 
-  int start, len, nblk, qb, run;
+  int start, len, nblk, qb, run, doc;
   int beyond = 0;
-  if (!locate_window_tile<false, D == 64>(a, blockIdx.y, start, len, nblk, qb, run, &beyond)) {
+  if (!locate_window_tile<false, D == 64>(a, blockIdx.y, start, len, nblk, qb, run, &beyond, &doc)) {
     zero_padding_rows<D>(a, beyond, blockIdx.x);
     return;
   }
@@ -304,6 +305,12 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       const long long t = start + (row_ok ? row : 0);
       CB_DEBUG_CHECK_ST(a.status, t >= 0 && t < a.T, CB_DBG_ATTN_ROW, t);
       uint4* op = reinterpret_cast<uint4*>(a.O + t * a.ldo + static_cast<long long>(h) * D);
+      int lo_at = a.o_lo != nullptr && row_ok ? static_cast<int>(t) : -1;
+      if (lo_index != nullptr) {
+        if (row >= LO_KEYS) lo_at = -1;
+        else if (a.T > static_cast<long long>(LO_KEYS) * a.n_docs && row_ok) lo_at = doc * LO_KEYS + row;
+        if (h == 0 && row_ok) lo_index[t] = lo_at;
+      }
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -312,8 +319,8 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         uint32_t w[16];
 #pragma unroll
         for (int q = 0; q < 16; ++q) w[q] = pack_bf16x2(__uint_as_float(o[2 * q]) * inv, __uint_as_float(o[2 * q + 1]) * inv);
-        if (a.o_lo != nullptr && row_ok) {
-          uint4* lo = reinterpret_cast<uint4*>(a.o_lo + (t * a.hq + h) * D + c * 32);
+        if (lo_at >= 0) {
+          uint4* lo = reinterpret_cast<uint4*>(a.o_lo + (static_cast<long long>(lo_at) * a.hq + h) * D + c * 32);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t v[4];
@@ -367,14 +374,14 @@ namespace {
 
 template <int D>
 int launch(dim3 grid, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mo,
-           const cb::AttnArgs& a) {
+           const cb::AttnArgs& a, int* lo_index) {
   constexpr int smem = cb::WinFwd<D>::TOTAL;
   static bool cfg = false;
   if (!cfg) {
     CB_CHECK_CUDA(cudaFuncSetAttribute(cb::attn_window_fwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cfg = true;
   }
-  cb::attn_window_fwd_kernel<D><<<grid, cb::WIN_THREADS, smem, s>>>(mq, mk, mv, mo, a);
+  cb::attn_window_fwd_kernel<D><<<grid, cb::WIN_THREADS, smem, s>>>(mq, mk, mv, mo, a, lo_index);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -382,10 +389,13 @@ int launch(dim3 grid, cudaStream_t s, const CUtensorMap& mq, const CUtensorMap& 
 
 extern "C" {
 
+// Rows of what the output's rounding left out; the buffer takes lo_rows * hq * D bf16 and T int32
+int cb_attn_window_lo_rows(int T, int n_docs, int window) { return cb::lo_rows(T, n_docs, window); }
+
 // q [T, hq, D] (row pitch ldq elements), k / v [T, hk, D]; cu: int32 [n_docs + 1] on the device; window >= 1, sinks >= 0.
 // o [T, hq, D] with pitch ldo; lse [hq, T] fp32.  Rows of o before cu[0] and at or beyond cu[n_docs] (padding) are written as zeros,
-// their lse entries are left untouched.  o_lo (null: none), [T, hq, D] without gaps: what o's rounding left out, for the backward pass.
-// D is 64 or 128, hq a multiple of hk.
+// their lse entries are left untouched.  o_lo (null: none; size: cb_attn_window_lo_rows): what o's rounding left out
+// where few keys are visible, for the backward pass.  D is 64 or 128, hq a multiple of hk.
 int cb_attn_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int* cu, int n_docs, int T,
                        int hq, int hk, int D, long long ldq, long long ldk, long long ldv, long long ldo, float scale, int window,
                        int sinks, void* o_lo, int* status, void* stream) {
@@ -402,12 +412,14 @@ int cb_attn_window_fwd(const void* q, const void* k, const void* v, void* o, flo
   a.T = T; a.hq = hq; a.hk = hk; a.n_docs = n_docs; a.cu = cu; a.scale = scale;
   a.O = static_cast<cb::bf16*>(o); a.ldo = ldo; a.lse = lse; a.status = status;
   a.o_lo = static_cast<cb::bf16*>(o_lo);
+  int* lo_index = o_lo != nullptr && !cb::lo_all(window)
+                      ? reinterpret_cast<int*>(a.o_lo + static_cast<long long>(cb::lo_rows(T, n_docs, window)) * hq * D) : nullptr;
   a.window = std::min(window, T); a.sinks = std::min(sinks, T); a.cap = (a.window + 126) / 128 + 1;
   a.o_tma = cbhost::make_tmap(&mo, o, static_cast<unsigned long long>(hq) * D, T, ldo, 64, 128) == 0 ? 1 : 0;
   if (!a.o_tma) mo = mq;                                // O is not TMA-addressable: every block stores row by row
   const dim3 grid(hq, static_cast<unsigned>(tiles));    // x: query head (fastest, the heads of a group share K / V in L2)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return D == 64 ? launch<64>(grid, s, mq, mk, mv, mo, a) : launch<128>(grid, s, mq, mk, mv, mo, a);
+  return D == 64 ? launch<64>(grid, s, mq, mk, mv, mo, a, lo_index) : launch<128>(grid, s, mq, mk, mv, mo, a, lo_index);
 }
 
 }  // extern "C"

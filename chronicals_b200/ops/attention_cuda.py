@@ -16,15 +16,6 @@ def _cu32(cu_seqlens: torch.Tensor) -> torch.Tensor:
     return cu.contiguous()
 
 
-# Windows of at most this many tokens keep what the rounding of O to bf16 left out for the backward pass (as much memory as O, 4 to 8 %
-# of the time): with few visible keys it shows in dQ and dK.  Error of the whole gradient against 64 bits, in roundings to bf16,
-# without / with it: window 2 1.70 / 1.41, 4 1.60 / 1.45, 8 1.52 / 1.44, 32 1.46 / 1.43.  So do documents as short on the average (40
-# in 2309 tokens 1.50 / 1.44) and batches of few tokens, whose documents may be.
-EXACT_DELTA_WINDOW = 32
-EXACT_DELTA_DOCUMENT = 128
-EXACT_DELTA_TOKENS = 1024
-
-
 class _AttnPackedFn(torch.autograd.Function):
     """Attention on a fused ``[T, (hq + 2 hk) * D]`` QKV buffer; the gradient comes back as one
     fused buffer too, so autograd never has to stitch three slice gradients together.
@@ -37,9 +28,10 @@ class _AttnPackedFn(torch.autograd.Function):
         o = torch.empty(T, nq, dtype=qkv.dtype, device=qkv.device)     # the kernel writes the zeros of the padding rows
         lse = torch.empty(hq, T, dtype=torch.float32, device=qkv.device)
         esz = qkv.element_size()
-        exact = (band and ctx.needs_input_grad[0] and
-                 (band[0] <= EXACT_DELTA_WINDOW or T <= EXACT_DELTA_TOKENS or T <= EXACT_DELTA_DOCUMENT * (cu.numel() - 1)))
-        o_lo = torch.empty_like(o) if exact else None
+        o_lo = None                                    # what the rounding of O leaves out, where few keys are visible
+        if band and ctx.needs_input_grad[0]:
+            rows = _ext.lib().cb_attn_window_lo_rows(T, cu.numel() - 1, band[0])
+            o_lo = torch.empty(2 * rows * nq + 4 * T, dtype=torch.uint8, device=qkv.device)
         fwd = _ext.lib().cb_attn_window_fwd if band else _ext.lib().cb_attn_fwd
         code = fwd(qkv.data_ptr(), qkv.data_ptr() + nq * esz, qkv.data_ptr() + (nq + nk) * esz,
                    o.data_ptr(), lse.data_ptr(), cu.data_ptr(), cu.numel() - 1, T, hq, hk, d,
