@@ -2113,12 +2113,28 @@ int launch_bwd3(dim3 grid, cudaStream_t s, const CUtensorMap& mq, const CUtensor
   return 0;
 }
 
+// Which kernel: the pipelined one, or (D = 64) the one that goes phase by phase.
+// D = 64 runs two CTAs of the phase-by-phase kernel on an SM where one of the pipelined kernel fits, so the pipelined one
+// wins where the grid does not fill the SMs twice over (1 x 2048 tokens, 14 heads: 44 against 80 us; 4 x 512: 23 / 26)
+// or its loops are long (2 x 4096: 276 / 290; 4 x 2048, 32 heads: 403 / 350, so no earlier than 4096), unless the
+// documents are so short that a CTA is mostly set-up (20 x 100: 19 / 15).  Lengths as the average over the documents.
+// With a window, where the pipelined one has twice the softmax warps, it wins from loops of 1024 tokens on (14 heads of 64, 8192
+// tokens, window 128 / 1024 / 4096: phase by phase 62 / 176 / 353 us, pipelined 71 / 155 / 305; 4 x 2048, 32 heads, window 1024
+// 274 / 270; 9 documents, 910 on average, window 1024 114 / 119; 27 x 300 69 / 83; 32 heads, 16,384 tokens, window 4096 1860 / 1594).
+// `documents` of the n_docs are not empty, as far as the caller knows: a list that was filled up says nothing about their length.
+bool bwd_pipelined(int T, int hq, int D, int n_docs, int window, int documents, int sms) {
+  if (D != 64) return true;
+  const bool few = static_cast<long long>(hq) * ((T + 127) / 128) <= 2LL * sms;
+  if (window > 0) return few || std::min(window, T / std::max(1, std::min(documents, n_docs))) >= 1024;
+  return (few && T >= 512LL * n_docs) || T >= 4096LL * n_docs;
+}
+
 // Both backward entry points; window = 0: none.
 int attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
                 const int* cu, int n_docs, int T, int hq, int hk, int D, long long ldq, long long ldk, long long ldv,
                 long long ldo, long long ld_do, float scale, float* delta, float* dq_acc, float* dk_part,
                 float* dv_part, void* dqkv, long long ld_dqkv, int* status, void* stream, int scratch_is_zero, int window, int sinks,
-                const void* o_lo) {
+                const void* o_lo, int documents) {
   if ((D != 64 && D != 128) || hq % hk != 0 || T <= 0 || n_docs <= 0) return -1;
   if ((reinterpret_cast<uintptr_t>(dqkv) & 7) != 0 || ld_dqkv % 4 != 0) return -1;       // the gradient is written 8 bytes at a time
   const bool wide = (reinterpret_cast<uintptr_t>(dqkv) & 15) == 0 && ld_dqkv % 8 == 0;   // or 16
@@ -2188,15 +2204,7 @@ int attn_bwd(const void* q, const void* k, const void* v, const void* o, const v
     if (rows() > 65535) return -1;
     grid.y = static_cast<unsigned>(rows());
   }
-  // D = 64 runs two CTAs of the phase-by-phase kernel on an SM where one of the pipelined kernel fits, so the pipelined one
-  // wins where the grid does not fill the SMs twice over (1 x 2048 tokens, 14 heads: 44 against 80 us; 4 x 512: 23 / 26)
-  // or its loops are long (2 x 4096: 276 / 290; 4 x 2048, 32 heads: 403 / 350, so no earlier than 4096), unless the
-  // documents are so short that a CTA is mostly set-up (20 x 100: 19 / 15).  Lengths as the average over the documents.
-  // With a window, where the pipelined one has twice the softmax warps, it wins from loops of 1024 tokens on (14 heads of 64, 8192
-  // tokens, window 128 / 1024 / 4096: phase by phase 62 / 176 / 353 us, pipelined 71 / 155 / 305; 4 x 2048, 32 heads, window 1024
-  // 274 / 270; 9 documents, 910 on average, window 1024 114 / 119; 27 x 300 69 / 83; 32 heads, 16,384 tokens, window 4096 1860 / 1594).
-  const bool few = tile_heads <= 2LL * cbhost::num_sms() && (window > 0 || T >= 512LL * n_docs);
-  if (D == 64 && !few && (window > 0 ? std::min<long long>(window, T / n_docs) < 1024 : T < 4096LL * n_docs)) {
+  if (!bwd_pipelined(T, hq, D, n_docs, window, documents, cbhost::num_sms())) {
     e = window > 0 ? launch_bwd2<64, true>(grid, s, mq, mk, mv, mdo, mdq, a) : launch_bwd2<64, false>(grid, s, mq, mk, mv, mdo, mdq, a);
     if (e) return e;
   } else {
@@ -2235,18 +2243,32 @@ int cb_attn_bwd(const void* q, const void* k, const void* v, const void* o, cons
                 long long ldo, long long ld_do, float scale, float* delta, float* dq_acc, float* dk_part,
                 float* dv_part, void* dqkv, long long ld_dqkv, int* status, void* stream, int scratch_is_zero) {
   return attn_bwd(q, k, v, o, d_o, lse, cu, n_docs, T, hq, hk, D, ldq, ldk, ldv, ldo, ld_do, scale, delta, dq_acc, dk_part, dv_part,
-                  dqkv, ld_dqkv, status, stream, scratch_is_zero, 0, 0, nullptr);
+                  dqkv, ld_dqkv, status, stream, scratch_is_zero, 0, 0, nullptr, n_docs);
 }
 
 // The same for cb_attn_window_fwd, with its window, sinks and o_lo (null: none); ldo = hq * D, d_o on 16-byte boundaries, and the
-// accumulators one behind the other.
+// accumulators one behind the other.  documents: how many of the n_docs are not empty, as a rule (for the choice of the kernel).
+int cb_attn_window_bwd_filled(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+                              const int* cu, int n_docs, int T, int hq, int hk, int D, long long ldq, long long ldk, long long ldv,
+                              long long ldo, long long ld_do, float scale, int window, int sinks, const void* o_lo, float* delta,
+                              float* dq_acc, float* dk_part, float* dv_part, void* dqkv, long long ld_dqkv, int documents, int* status,
+                              void* stream) {
+  if (window < 1 || sinks < 0 || hk <= 0) return -1;
+  return attn_bwd(q, k, v, o, d_o, lse, cu, n_docs, T, hq, hk, D, ldq, ldk, ldv, ldo, ld_do, scale, delta, dq_acc, dk_part, dv_part,
+                  dqkv, ld_dqkv, status, stream, 0, window, sinks, o_lo, documents);
+}
+
 int cb_attn_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
                        const int* cu, int n_docs, int T, int hq, int hk, int D, long long ldq, long long ldk, long long ldv,
                        long long ldo, long long ld_do, float scale, int window, int sinks, const void* o_lo, float* delta, float* dq_acc, float* dk_part,
                        float* dv_part, void* dqkv, long long ld_dqkv, int* status, void* stream) {
-  if (window < 1 || sinks < 0 || hk <= 0) return -1;
-  return attn_bwd(q, k, v, o, d_o, lse, cu, n_docs, T, hq, hk, D, ldq, ldk, ldv, ldo, ld_do, scale, delta, dq_acc, dk_part, dv_part,
-                  dqkv, ld_dqkv, status, stream, 0, window, sinks, o_lo);
+  return cb_attn_window_bwd_filled(q, k, v, o, d_o, lse, cu, n_docs, T, hq, hk, D, ldq, ldk, ldv, ldo, ld_do, scale, window, sinks, o_lo,
+                                   delta, dq_acc, dk_part, dv_part, dqkv, ld_dqkv, n_docs, status, stream);
+}
+
+// 1 where the backward pass takes the pipelined kernel, 0 where the one that goes phase by phase
+int cb_attn_window_bwd_pipelined(int T, int hq, int D, int n_docs, int window, int documents, int sms) {
+  return bwd_pipelined(T, hq, D, n_docs, window, documents, sms) ? 1 : 0;
 }
 
 #ifdef CB_ATTN_PHASE_TIMERS

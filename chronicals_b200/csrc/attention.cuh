@@ -62,7 +62,8 @@ __device__ __forceinline__ int lane_of_item(int& b, int mine) {
 // BY_WEIGHT (head size 64): two to 32 documents are handed out by weight, the blocks that a tile's loop visits, at most a.cap: first
 // all tiles of full weight, then those of every lower one, of which a document has at most one (14 / 2 heads of 64, 9 documents in 8192 tokens, window 1024,
 // backward: 124 us in the order of the documents, 114 so).  More of them go in their order: a search through more lengths than a
-// register holds, level by level, takes longer than it saves (40 documents: 74 and 94 us).  A single document's tiles are in that
+// register holds, level by level, takes longer than it saves (40 documents: 74 and 94 us); empty ones behind the 32nd, to which a
+// list may have been filled up, do not count.  A single document's tiles are in that
 // order already; with heads of 128, whose tiles take more rounds, the order of the documents is the faster one (16 documents, 28 / 4
 // heads, window 512: 248 and 260 us).
 template <bool BWD, bool BY_WEIGHT>
@@ -90,7 +91,7 @@ __device__ __forceinline__ bool locate_window_tile(const AttnArgs& a, int b, int
       nblk = (len + 127) >> 7;
       if (doc != nullptr) *doc = d0 + src;
     };
-    if (!BY_WEIGHT || a.n_docs == 1 || a.n_docs > 32) {
+    if (!BY_WEIGHT || a.n_docs == 1 || (a.n_docs > 32 && a.cu[32] < a.cu[a.n_docs])) {
       take(lane_of_item(b, own + in_runs));
       const int n_s = min(nblk, with_sinks), n_runs = n_s > 0 ? n_s * ((nblk + a.sink_run - 1) / a.sink_run) : 0;
       if (b < n_runs) {

@@ -791,7 +791,8 @@ def attention_qkv_packed(qkv: torch.Tensor, cu_seqlens: torch.Tensor, num_q_head
     other, nor does padding reach them, whatever they hold.  Within a document masked scores are dropped whatever they are, but
     a masked key's V row is multiplied by an exact zero, so that V (and in the backward pass the output's gradient) has to be
     finite.  The additions into dQ, dK and dV come in any order: their last bits of 32 differ from call to call.
-    A call takes up to 65,535 blocks of 128 tokens and documents together (8 million tokens)."""
+    A call takes up to 65,535 blocks of 128 tokens and documents together (8 million tokens).  Where ``cu_seqlens`` is filled up to a
+    fixed length with empty documents, ``seqlens_host`` without them lets the kernel be chosen by the others."""
     from . import attention_cuda as _ac
     if window is not None or sinks:
         from .attention import window_band
@@ -803,7 +804,7 @@ def attention_qkv_packed(qkv: torch.Tensor, cu_seqlens: torch.Tensor, num_q_head
         if _ac.kernel_supports(qkv, head_dim) and qkv.shape[0] and cu_seqlens.numel() > 1:
             if not _gemm_ok(qkv) or qkv.stride(0) < qkv.shape[1]:
                 qkv = qkv.clone(memory_format=torch.contiguous_format)
-            return _ac.attention_qkv_packed(qkv, cu_seqlens, num_q_heads, num_kv_heads, head_dim, None, band)
+            return _ac.attention_qkv_packed(qkv, cu_seqlens, num_q_heads, num_kv_heads, head_dim, None, band, seqlens_host)
         heads = (num_q_heads, num_kv_heads, num_kv_heads)
         q, k, v = (t.reshape(qkv.shape[0], n, head_dim) for t, n in zip(qkv.split([n * head_dim for n in heads], dim=1), heads))
         return ref.attention_window(q, k, v, cu_seqlens, *band, 1.0 / math.sqrt(head_dim)).reshape(qkv.shape[0], num_q_heads * head_dim)

@@ -71,6 +71,8 @@ _PROTOTYPES = {
     "cb_attn_window_lo_rows": [I, I, I],
     "cb_attn_window_fwd": [P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, F, I, I, P, P, P],
     "cb_attn_window_bwd": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, F, I, I, P, P, P, P, P, P, L, P, P],
+    "cb_attn_window_bwd_filled": [P, P, P, P, P, P, P, I, I, I, I, I, L, L, L, L, L, F, I, I, P, P, P, P, P, P, L, I, P, P],
+    "cb_attn_window_bwd_pipelined": [I, I, I, I, I, I, I],
     "cb_gemm2sm_bf16": [P, P, P, P, P, I, I, I, L, L, L, L, I, I, I, I, P, P],
     "cb_gemm2sm_supported": [P, L, I],
     "cb_gemm2sm_bf16_ex": [P, P, P, P, P, I, I, I, L, L, L, L, I, I, I, I, I, P, P],
@@ -166,7 +168,7 @@ def lib() -> ctypes.CDLL:
 
 # device kernels launched by one call of each entry point (0: host-only query)
 _KERNELS_PER_CALL = {"cb_gemm2sm_supported": 0, "cb_gemm2sm_cost_ns": 0, "cb_gemm_choice": 0, "cb_glu_bwd_fused_pays": 0, "cb_cce_chunk": 0, "cb_cce_num_splits": 0, "cb_rmsnorm_max_n": 0, "cb_rmsnorm_bwd_blocks": 0, "cb_opt_chunk": 0,
-                     "cb_embedding_rank_max": 0, "cb_embedding_part_rows": 0, "cb_embedding_bwd": 2, "cb_cce_combine": 2, "cb_rmsnorm_bwd": 2, "cb_grad_clip_coef": 2, "cb_attn_bwd": 3, "cb_attn_window_bwd": 3,
+                     "cb_embedding_rank_max": 0, "cb_embedding_part_rows": 0, "cb_embedding_bwd": 2, "cb_cce_combine": 2, "cb_rmsnorm_bwd": 2, "cb_grad_clip_coef": 2, "cb_attn_bwd": 3, "cb_attn_window_bwd": 3, "cb_attn_window_bwd_filled": 3, "cb_attn_window_bwd_pipelined": 0,
                      "cb_attn_window_lo_rows": 0, "cb_gemm_slabs": 0, "cb_kd_max_entries": 0, "cb_kd_logits": 2, "cb_kd_linear_rows": 2}
 LAUNCH_COUNT = [0]
 

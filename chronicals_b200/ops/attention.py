@@ -70,7 +70,7 @@ def window_band(op: str, window: Optional[int], sinks: int, causal: bool = True)
     return min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1)
 
 
-def _windowed(q, k, v, cu_seqlens, max_seqlen, scale, band):
+def _windowed(q, k, v, cu_seqlens, max_seqlen, scale, band, seqlens_host):
     T, hq, d = q.shape
     if k.shape != v.shape or k.dim() != 3 or k.shape[0] != T or k.shape[2] != d or k.shape[1] == 0 or hq % k.shape[1]:
         raise ValueError(f"attention_varlen: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit")
@@ -80,7 +80,7 @@ def _windowed(q, k, v, cu_seqlens, max_seqlen, scale, band):
     _same_device("attention_varlen", q, k, v, cu_seqlens)
     from .attention_cuda import attention_varlen_cuda, kernel_supports
     if T and cu_seqlens.numel() > 1 and all(kernel_supports(t, d) for t in (q, k, v)):
-        return attention_varlen_cuda(q, k, v, cu_seqlens, max_seqlen, scale, band)
+        return attention_varlen_cuda(q, k, v, cu_seqlens, max_seqlen, scale, band, seqlens_host)
     return ref.attention_window(q, k, v, cu_seqlens, *band, scale)
 
 
@@ -91,13 +91,14 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(d)
     band = window_band("attention_varlen", window, sinks, causal)
     if band:
-        return _windowed(q, k, v, cu_seqlens, max_seqlen, scale, band)
+        return _windowed(q, k, v, cu_seqlens, max_seqlen, scale, band, seqlens_host)
     if q.is_cuda and not _ext.reference_forced() and q.dtype == torch.bfloat16 and _ext.available() and _ext.has_symbol("cb_attn_fwd") \
             and d in (64, 128) and causal:
         from .attention_cuda import attention_varlen_cuda
         return attention_varlen_cuda(q, k, v, cu_seqlens, max_seqlen, scale)
     if q.is_cuda:
-        if seqlens_host is not None:
+        # lengths of another number of documents: those of a typical batch, where the boundaries were filled up with empty ones
+        if seqlens_host is not None and len(seqlens_host) == cu_seqlens.numel() - 1:
             bounds = [0]
             for l in seqlens_host:
                 bounds.append(bounds[-1] + int(l))

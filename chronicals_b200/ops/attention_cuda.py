@@ -19,10 +19,10 @@ def _cu32(cu_seqlens: torch.Tensor) -> torch.Tensor:
 class _AttnPackedFn(torch.autograd.Function):
     """Attention on a fused ``[T, (hq + 2 hk) * D]`` QKV buffer; the gradient comes back as one
     fused buffer too, so autograd never has to stitch three slice gradients together.
-    ``band``: () or (window, sinks)."""
+    ``band``: () or (window, sinks).  ``documents``: how many of the boundaries' documents are not empty, as a rule; 0: all."""
 
     @staticmethod
-    def forward(ctx, qkv, cu, hq, hk, d, scale, band=()):
+    def forward(ctx, qkv, cu, hq, hk, d, scale, band=(), documents=0):
         T, ld = qkv.shape[0], qkv.stride(0)
         nq, nk = hq * d, hk * d
         o = torch.empty(T, nq, dtype=qkv.dtype, device=qkv.device)     # the kernel writes the zeros of the padding rows
@@ -39,13 +39,13 @@ class _AttnPackedFn(torch.autograd.Function):
                    _ext.stream_ptr())
         _ext.check(code, "attn_window_fwd" if band else "attn_fwd")
         ctx.save_for_backward(qkv, o, lse, cu, *(() if o_lo is None else (o_lo,)))
-        ctx.cfg = (hq, hk, d, scale, band)
+        ctx.cfg = (hq, hk, d, scale, band, documents)
         return o
 
     @staticmethod
     def backward(ctx, do):
         qkv, o, lse, cu, *o_lo = ctx.saved_tensors
-        hq, hk, d, scale, band = ctx.cfg
+        hq, hk, d, scale, band, documents = ctx.cfg
         T, ld = qkv.shape[0], qkv.stride(0)
         nq, nk = hq * d, hk * d
         if not do.is_contiguous():
@@ -67,14 +67,16 @@ class _AttnPackedFn(torch.autograd.Function):
         dv_part = dk_part + 4 * T * nk
         dqkv = torch.empty(T, nq + 2 * nk, dtype=qkv.dtype, device=dev)
         esz = qkv.element_size()
-        bwd = _ext.lib().cb_attn_window_bwd if band else _ext.lib().cb_attn_bwd
+        lib = _ext.lib()
+        bwd = lib.cb_attn_window_bwd_filled if documents else lib.cb_attn_window_bwd if band else lib.cb_attn_bwd
         code = bwd(qkv.data_ptr(), qkv.data_ptr() + nq * esz, qkv.data_ptr() + (nq + nk) * esz,
                    o.data_ptr(), do.data_ptr(), lse.data_ptr(), cu.data_ptr(), cu.numel() - 1, T,
                    hq, hk, d, ld, ld, ld, nq, do.stride(0), scale, *((*band, _ext.ptr(o_lo[0]) if o_lo else None) if band else ()), delta,
                    dq_acc, dk_part, dv_part, dqkv.data_ptr(),
-                   dqkv.stride(0), _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr(), *(() if band else (0,)))
+                   dqkv.stride(0), *((documents,) if documents else ()), _ext.status_buffer(dev).data_ptr(), _ext.stream_ptr(),
+                   *(() if band else (0,)))
         _ext.check(code, "attn_window_bwd" if band else "attn_bwd")
-        return dqkv, None, None, None, None, None, None
+        return dqkv, None, None, None, None, None, None, None
 
 
 def kernel_supports(t: torch.Tensor, d: int) -> bool:
@@ -83,17 +85,22 @@ def kernel_supports(t: torch.Tensor, d: int) -> bool:
 
 
 def attention_qkv_packed(qkv: torch.Tensor, cu_seqlens: torch.Tensor, num_q_heads: int, num_kv_heads: int,
-                         head_dim: int, softmax_scale: Optional[float] = None, band: tuple = ()) -> torch.Tensor:
-    """Causal GQA attention over packed documents; ``qkv [T, (hq + 2 hk) * D]`` → ``[T, hq * D]``."""
+                         head_dim: int, softmax_scale: Optional[float] = None, band: tuple = (), seqlens_host=None) -> torch.Tensor:
+    """Causal GQA attention over packed documents; ``qkv [T, (hq + 2 hk) * D]`` → ``[T, hq * D]``.  With a window ``seqlens_host``
+    tells the documents that hold tokens from those that a list of boundaries was filled up with, for the choice of the kernel."""
     scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(head_dim)
     assert qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.stride(0) % 8 == 0
-    return _AttnPackedFn.apply(qkv, _cu32(cu_seqlens), num_q_heads, num_kv_heads, head_dim, scale, band)
+    documents = 0
+    if band and seqlens_host is not None:
+        documents = len(seqlens_host) - list(seqlens_host).count(0)
+        documents = documents if 0 < documents < cu_seqlens.numel() - 1 else 0
+    return _AttnPackedFn.apply(qkv, _cu32(cu_seqlens), num_q_heads, num_kv_heads, head_dim, scale, band, documents)
 
 
 def attention_varlen_cuda(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
-                          max_seqlen: Optional[int], scale: float, band: tuple = ()) -> torch.Tensor:
+                          max_seqlen: Optional[int], scale: float, band: tuple = (), seqlens_host=None) -> torch.Tensor:
     """Separate q / k / v tensors: packed into one buffer (a copy) and run through the fused-buffer path."""
     T, hq, d = q.shape
     hk = k.shape[1]
     qkv = torch.cat((q.reshape(T, hq * d), k.reshape(T, hk * d), v.reshape(T, hk * d)), dim=1)
-    return attention_qkv_packed(qkv, cu_seqlens, hq, hk, d, scale, band).view(T, hq, d)
+    return attention_qkv_packed(qkv, cu_seqlens, hq, hk, d, scale, band, seqlens_host).view(T, hq, d)

@@ -447,7 +447,10 @@ class ChronicalsTrainer:
             f = dict(f)
             f["cu_seqlens"] = torch.cat((cu, cu[-1:].expand(max_docs + 1 - cu.numel())))
             f["max_seqlen"] = int(self.args.max_seq_length)
-            f["seqlens_host"] = None
+            # the batch that is captured stands for the others where kernels are chosen by the documents that hold tokens; as many
+            # lengths as boundaries would be taken for those of every batch
+            lens = f.get("seqlens_host")
+            f["seqlens_host"] = lens if lens is not None and len(lens) < max_docs else None
         key = (tuple(ids.shape), tuple(f["cu_seqlens"].shape) if isinstance(f.get("cu_seqlens"), torch.Tensor) else None,
                f.get("max_seqlen"), tuple(f["seqlens_host"]) if f.get("seqlens_host") is not None and
                not isinstance(f.get("cu_seqlens"), torch.Tensor) else None,
