@@ -261,9 +261,7 @@ kd_logits_grad_kernel(const T* __restrict__ logits, T* __restrict__ dlogits, lon
     const float x = fmaf(v, c2, -st.x);
     return sizeof(T) == 2 ? ex2_approx(x) : exp2f(x);
   };
-  // source and destination rows may start at different distances from a 16-byte boundary: value by value then
-  const bool vec = ((reinterpret_cast<uintptr_t>(lp) ^ reinterpret_cast<uintptr_t>(dp)) & 15) == 0;
-  const int head = vec ? ce_head(lp, V) : V, nvec = (V - head) / N;
+  const int head = ce_head(lp, V), nvec = (V - head) / N;                 // the same of both rows
   const uint4* vp = reinterpret_cast<const uint4*>(lp + head);
   uint4* wp = reinterpret_cast<uint4*>(dp + head);
   // this block's stretch: vectors [v0, v1), with the values before the first vector and after the last at the ends
@@ -596,6 +594,7 @@ int cb_kd_logits(const void* logits, long long rows, long long ld, int V, int is
   return static_cast<int>(cudaGetLastError());
 }
 
+// Rows of dlogits start at the same distance from a 16-byte boundary as those of logits.
 // gout: gradient of the reduced loss (or null), over n_rows[0] for a mean (null: a sum); grows [rows]: of the rows' losses (or null)
 int cb_kd_logits_grad(const void* logits, void* dlogits, long long rows, long long ld, long long ldd, int V, int is_bf16,
                       const void* idx, long long ld_idx, int idx64, const void* lg, long long ld_lg, int lg_bf16, int K,
@@ -604,6 +603,8 @@ int cb_kd_logits_grad(const void* logits, void* dlogits, long long rows, long lo
   cb::KdTeacher t;
   if (rows <= 0 || rows > 0x7fffffffLL || V <= 0 || !kd_teacher(&t, idx, ld_idx, idx64, lg, ld_lg, lg_bf16, K, labels, ignore_index, tau))
     return -1;
+  const long long apart = (ldd - ld) * (is_bf16 ? 2 : 4);
+  if (((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15) != 0 || (rows > 1 && apart % 16 != 0)) return -1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(rows), cbhost::ce_split(rows, V));
   const int threads = cbhost::ce_threads(rows, V, is_bf16);

@@ -1117,8 +1117,13 @@ class _DistillLogitsFn(torch.autograd.Function):
         ignore_index, tau, reduction = ctx.cfg
         rows, V = logits.shape
         ld = logits.stride(0)
-        # rows as far apart as the logits', so that both start at the same distance from a 16-byte boundary
-        dl = torch.empty_strided((rows, V), (ld, 1) if V <= ld < 2 * V else (V, 1), dtype=logits.dtype, device=logits.device)
+        # every row at the same distance from a 16-byte boundary as the logits': 16-byte vectors on both sides
+        size = logits.element_size()
+        pitch, skip = ld if V <= ld < 2 * V else V + (ld - V) % (16 // size), logits.data_ptr() % 16 // size
+        if skip:
+            dl = torch.empty(skip + rows * pitch, dtype=logits.dtype, device=logits.device).as_strided((rows, V), (pitch, 1), skip)
+        else:
+            dl = torch.empty_strided((rows, V), (pitch, 1), dtype=logits.dtype, device=logits.device)
         grad = grad if grad.dtype == torch.float32 and grad.is_contiguous() else grad.float().contiguous()
         each = reduction == "none"
         stats, g = buf.data_ptr(), grad.data_ptr()
