@@ -454,7 +454,9 @@ class ChronicalsTrainer:
         key = (tuple(ids.shape), tuple(f["cu_seqlens"].shape) if isinstance(f.get("cu_seqlens"), torch.Tensor) else None,
                f.get("max_seqlen"), tuple(f["seqlens_host"]) if f.get("seqlens_host") is not None and
                not isinstance(f.get("cu_seqlens"), torch.Tensor) else None,
-               tuple(tuple(f[k].shape) for k in ("position_ids", *_TEACHER) if isinstance(f.get(k), torch.Tensor)))
+               # the static buffers keep their types, and the captured kernels the numbers they were given
+               tuple((k, tuple(f[k].shape), f[k].dtype) for k in ("position_ids", *_TEACHER) if isinstance(f.get(k), torch.Tensor)),
+               tuple(getattr(self.model, k, None) for k in ("distill_weight", "distill_temperature")))
         if self._graph is None or self._graph["key"] != key:
             self._capture_graph(f, key)
         g = self._graph
