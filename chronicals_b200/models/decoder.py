@@ -277,7 +277,8 @@ class CausalLM(nn.Module):
     for the token that follows each position) add a distillation loss:
     ``(1 - distill_weight) * cross-entropy + distill_weight * distillation``,
     over the positions whose label is not ignored; without ``labels`` the loss is
-    the distillation's alone.
+    the distillation's alone.  Logits come where there is nothing to compute a loss
+    from, or with ``return_logits``.
     """
 
     def __init__(self, cfg: ChronicalsConfig, dtype: Optional[torch.dtype] = None, device=None):
@@ -419,7 +420,7 @@ class CausalLM(nn.Module):
             kd = ops.linear_distillation(h, self.output_weight, teacher_indices.reshape(T, K), teacher_logits.reshape(T, K),
                                          float(self.distill_temperature), y)
             out.loss = kd if out.loss is None else (1.0 - share) * out.loss + share * kd
-        if return_logits or (labels is None and not output_hidden_states):
+        if return_logits or (out.loss is None and not output_hidden_states):
             out.logits = torch.nn.functional.linear(h, self.output_weight).view(B, S, -1)
         return out
 
