@@ -691,7 +691,8 @@ def qk_rope_axes_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
     ``position_ids [axes, T]`` (one to four axes); ``sections`` says how many of the ``head_dim / 2`` frequencies turn by which
     axis: blocks one behind the other, or (``cyclic``) dealt to the axes in turn, axis 0 taking what is left over.  ``cos`` and
     ``sin`` are the tables of :func:`ref.rope_cache`, one row a position; positions outside them use the first or last row.
-    ``inverse`` turns back.  In place on CUDA; returns the rotated buffer.  The backward pass turns the gradient back into a
+    ``inverse`` turns back.  Returns the rotated buffer: bf16 rows on CUDA that start and step by 16 bytes are rotated in place, of
+    anything else a rotated copy is returned.  The backward pass turns the gradient back into a
     buffer of its own."""
     sections = tuple(int(n) for n in sections)
     if qkv.dim() != 2 or qkv.shape[1] != (num_q_heads + 2 * num_kv_heads) * head_dim:
@@ -715,7 +716,9 @@ def qk_rope_axes_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
         cfg = (num_q_heads, num_kv_heads, head_dim, sections, bool(cyclic), bool(interleaved), bool(inverse))
         if torch.is_grad_enabled() and qkv.requires_grad:
             return _QKRopeAxesFn.apply(qkv, cos, sin, pos, cfg)
-        return _rope_axes_launch(qkv, qkv, cos, sin, pos, *cfg)
+        _rope_axes_launch(qkv, qkv, cos, sin, pos, *cfg)
+        torch.autograd.graph.increment_version(qkv)    # whoever kept it for a backward pass is told that it changed
+        return qkv
     T, nqk = qkv.shape[0], (num_q_heads + num_kv_heads) * head_dim
     c, s = ref.rope_axes_tables(cos, sin, position_ids, ref.rope_axis_map(sections, cyclic))
     y = ref.apply_rope(qkv[:, :nqk].reshape(T, -1, head_dim), c, s, None, interleaved, inverse)
