@@ -17,6 +17,7 @@ from torch.utils.data import DataLoader, Dataset, IterableDataset, Sampler
 
 from .sequence_packer import (IGNORE_INDEX, DataPrefetcher, FixedShapeSequencePacker, PackedBatch, PackedDataLoader,
                               PackedDataset)
+from .teacher import TEACHER_KEYS, join_teachers, teacher_of
 
 # ------------------------------------------------------------------------------------------- prompt templates
 PROMPT_TEMPLATES: Dict[str, Dict[str, str]] = {
@@ -84,7 +85,9 @@ class DataCollator:
             x = torch.as_tensor(s["input_ids"], dtype=torch.long)[:L]
             y = torch.as_tensor(s.get("labels", s["input_ids"]), dtype=torch.long)[:L]
             ids[i, :len(x)], lab[i, :len(y)], mask[i, :len(x)] = x, y, 1
-        return {"input_ids": ids, "labels": lab, "attention_mask": mask}
+        kept = [min(len(s["input_ids"]), L) for s in samples]
+        teacher = join_teachers([p for s, n in zip(samples, kept) for p in ((teacher_of(s), n), (None, L - n))])
+        return {"input_ids": ids, "labels": lab, "attention_mask": mask, **{k: v.view(len(samples), L, -1) for k, v in teacher.items()}}
 
 
 class DataCollatorWithFlattening:
@@ -107,7 +110,8 @@ class DataCollatorWithFlattening:
         cu = torch.zeros(len(lens) + 1, dtype=torch.int32)
         cu[1:] = torch.cumsum(torch.tensor(lens, dtype=torch.int32), 0)
         return {"input_ids": torch.cat(ids)[None], "labels": torch.cat(lab)[None], "position_ids": torch.cat(pos)[None],
-                "cu_seqlens": cu, "max_seqlen": max(lens) if lens else 0, "seqlens_host": lens}
+                "cu_seqlens": cu, "max_seqlen": max(lens) if lens else 0, "seqlens_host": lens,
+                **{k: v[None] for k, v in join_teachers([(teacher_of(s), n) for s, n in zip(samples, lens)]).items()}}
 
 
 class PackingDataCollator:
@@ -118,6 +122,10 @@ class PackingDataCollator:
 
     def __call__(self, samples: List[Dict[str, Any]]) -> List[PackedBatch]:
         return self.packer.pack_all_sequences(samples)
+
+
+def _row_teacher(row: PackedBatch):
+    return None if row.teacher_indices is None else tuple(getattr(row, k).flatten(0, -2) for k in TEACHER_KEYS)
 
 
 def stack_packed_rows(rows: Sequence[PackedBatch]) -> Dict[str, Any]:
@@ -137,7 +145,8 @@ def stack_packed_rows(rows: Sequence[PackedBatch]) -> Dict[str, Any]:
     cu = torch.zeros(len(lens) + 1, dtype=torch.int32)
     cu[1:] = torch.cumsum(torch.tensor(lens, dtype=torch.int32), 0)
     return {"input_ids": ids, "labels": lab, "position_ids": pos, "cu_seqlens": cu,
-            "max_seqlen": max(lens) if lens else L, "seqlens_host": lens}
+            "max_seqlen": max(lens) if lens else L, "seqlens_host": lens,
+            **{k: v[None] for k, v in join_teachers([(_row_teacher(r), r.input_ids.numel()) for r in rows]).items()}}
 
 
 # ------------------------------------------------------------------------------------------- datasets

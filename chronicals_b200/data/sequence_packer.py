@@ -19,6 +19,8 @@ from typing import Any, Dict, Iterable, Iterator, List, Optional, Sequence, Tupl
 
 import torch
 
+from .teacher import TEACHER_KEYS, join_teachers, teacher_of
+
 IGNORE_INDEX = -100
 
 
@@ -37,6 +39,8 @@ class PackedBatch:
     loss_mask: Optional[torch.Tensor] = None
     total_padding_tokens: int = 0
     packing_efficiency_cached: Optional[float] = None
+    teacher_indices: Optional[torch.Tensor] = None      # [rows, max_seq_length, K] where samples carry a teacher's top logits
+    teacher_logits: Optional[torch.Tensor] = None
 
     @property
     def use_varlen(self) -> bool:
@@ -63,7 +67,7 @@ class PackedBatch:
 
     def _map(self, fn) -> "PackedBatch":
         kw = dict(self.__dict__)
-        for k in ("input_ids", "position_ids", "labels", "attention_mask", "cu_seqlens", "loss_mask"):
+        for k in ("input_ids", "position_ids", "labels", "attention_mask", "cu_seqlens", "loss_mask", *TEACHER_KEYS):
             if kw[k] is not None:
                 kw[k] = fn(kw[k])
         return PackedBatch(**kw)
@@ -83,6 +87,8 @@ class PackedBatch:
             d["max_seqlen"] = self.max_seqlen
         if self.loss_mask is not None:
             d["loss_mask"] = self.loss_mask
+        if self.teacher_indices is not None:
+            d.update({k: getattr(self, k) for k in TEACHER_KEYS})
         d["seqlens_host"] = list(self.sequence_lengths)
         return d
 
@@ -275,7 +281,7 @@ class FixedShapeSequencePacker:
 
     # -- API -------------------------------------------------------------------------------------------
     def pack_all_sequences(self, sequences: Iterable[Seq]) -> List[PackedBatch]:
-        seqs = [_as_ids_labels(s) for s in sequences]
+        seqs = [(*_as_ids_labels(s), teacher_of(s)) for s in sequences]
         if not seqs:
             return [self._empty_batch()]
         lengths = [min(len(s[0]), self.max_seq_length) for s in seqs]
@@ -310,15 +316,17 @@ class FixedShapeSequencePacker:
             loss_mask=torch.zeros(1, L) if self.generate_loss_mask else None,
             total_padding_tokens=L, packing_efficiency_cached=0.0)
 
-    def _create_batch_from_bin(self, seqs: List[Tuple[List[int], Optional[List[int]]]]) -> PackedBatch:
+    def _create_batch_from_bin(self, seqs: List[Tuple]) -> PackedBatch:
+        """``seqs``: token ids, labels or None and, where there is one, the teacher (:func:`teacher_of`) of each document."""
         L = self.max_seq_length
         ids = torch.full((L,), self.pad_token_id, dtype=self.dtype)
         pos = torch.zeros(L, dtype=self.dtype)
         lab = torch.full((L,), self.ignore_index, dtype=self.dtype)
         lens: List[int] = []
         bounds: List[Tuple[int, int]] = []
+        teachers = []
         o = 0
-        for di, (tok, labels) in enumerate(seqs):
+        for di, (tok, labels, *teacher) in enumerate(seqs):
             n = min(len(tok), L - o)
             if n <= 0:
                 break
@@ -329,6 +337,7 @@ class FixedShapeSequencePacker:
                 lab[o] = self.ignore_index
             lens.append(n)
             bounds.append((o, o + n))
+            teachers.append((teacher[0] if teacher else None, n))
             o += n
         cu = torch.tensor([0] + [b for _, b in bounds], dtype=torch.int32)
         mask = None
@@ -338,7 +347,8 @@ class FixedShapeSequencePacker:
             input_ids=ids[None], position_ids=pos[None], labels=lab[None], attention_mask=mask,
             sequence_lengths=lens, num_sequences=len(lens), cu_seqlens=cu, max_seqlen=max(lens) if lens else 0,
             sequence_boundaries=bounds, loss_mask=(lab != self.ignore_index).float()[None] if self.generate_loss_mask else None,
-            total_padding_tokens=L - o, packing_efficiency_cached=o / L)
+            total_padding_tokens=L - o, packing_efficiency_cached=o / L,
+            **{k: v[None] for k, v in join_teachers([*teachers, (None, L - o)]).items()})
 
     @staticmethod
     def _create_block_causal_mask(bounds: List[Tuple[int, int]], L: int) -> torch.Tensor:

@@ -14,6 +14,7 @@ import torch
 
 from .sequence_packer import (IGNORE_INDEX, BinPackingAlgorithm, _as_ids_labels,
                               create_cu_seqlens_from_position_ids as compute_cu_seqlens_from_position_ids)
+from .teacher import TEACHER_KEYS, join_teachers, teacher_of
 
 
 @dataclass
@@ -30,6 +31,8 @@ class PackedBatchV2:
     num_sequences: int = 0
     sequence_lengths: List[int] = field(default_factory=list)
     num_padding_tokens: int = 0
+    teacher_indices: Optional[torch.Tensor] = None      # [tokens, K] where samples carry a teacher's top logits
+    teacher_logits: Optional[torch.Tensor] = None
 
     @property
     def total_tokens(self) -> int:
@@ -65,7 +68,8 @@ class PackedBatchV2:
         """Keyword arguments for ``CausalLM.forward`` / a trainer batch."""
         return {"input_ids": self.input_ids[None], "labels": self.labels[None], "position_ids": self.position_ids[None],
                 "cu_seqlens": self.cu_seqlens_q, "max_seqlen": self.max_seqlen_q,
-                "seqlens_host": list(self.sequence_lengths) + ([self.num_padding_tokens] if self.num_padding_tokens else [])}
+                "seqlens_host": list(self.sequence_lengths) + ([self.num_padding_tokens] if self.num_padding_tokens else []),
+                **({} if self.teacher_indices is None else {k: getattr(self, k)[None] for k in TEACHER_KEYS})}
 
     to_dict = to_model_inputs
 
@@ -116,16 +120,16 @@ class SequencePackerV2:
         return BinPackingAlgorithm.pack(lengths, self.max_seq_length, self.strategy)
 
     def pack(self, sequences: Iterable[Any]) -> List[PackedBatchV2]:
-        seqs = [_as_ids_labels(s) for s in sequences]
+        seqs = [(*_as_ids_labels(s), teacher_of(s)) for s in sequences]
         lengths = [min(len(s[0]), self.max_seq_length) for s in seqs]
         return [self._build([seqs[i] for i in b]) for b in self._bins(lengths)] if seqs else []
 
     pack_all_sequences = pack
 
     def _build(self, seqs) -> PackedBatchV2:
-        ids, labs, pos, sid, lens = [], [], [], [], []
+        ids, labs, pos, sid, lens, teachers = [], [], [], [], [], []
         room = self.max_seq_length
-        for di, (tok, labels) in enumerate(seqs):
+        for di, (tok, labels, *teacher) in enumerate(seqs):
             n = min(len(tok), room)
             if n <= 0:
                 break
@@ -138,6 +142,7 @@ class SequencePackerV2:
             pos.append(torch.arange(n, dtype=self.dtype))
             sid.append(torch.full((n,), di, dtype=self.dtype))
             lens.append(n)
+            teachers.append((teacher[0] if teacher else None, n))
             room -= n
         pad = room if self.fixed_output_shape else 0
         if pad:
@@ -152,7 +157,8 @@ class SequencePackerV2:
                              cu_seqlens_k=cu, max_seqlen_q=max(seg) if seg else 0, max_seqlen_k=max(seg) if seg else 0,
                              sequence_ids=torch.cat(sid) if self.generate_sequence_ids else None,
                              loss_mask=(labels != self.ignore_index).float() if self.generate_loss_mask else None,
-                             num_sequences=len(lens), sequence_lengths=lens, num_padding_tokens=pad)
+                             num_sequences=len(lens), sequence_lengths=lens, num_padding_tokens=pad,
+                             **join_teachers([*teachers, (None, pad)]))
 
 
 def create_block_causal_mask(cu_seqlens: torch.Tensor, total_tokens: Optional[int] = None) -> torch.Tensor:

@@ -35,6 +35,7 @@ import torch.nn as nn
 from ..checkpoint import io as ckpt_io
 from ..config.config import ChronicalsConfig, TrainingConfig
 from ..data.sequence_packer import PackedBatch
+from ..data.teacher import TEACHER_KEYS
 from ..optimizers.fused_adamw import FusedAdamW
 from ..optimizers.optimizers import ScheduleFreeAdamW, create_optimizer, create_scheduler
 
@@ -62,9 +63,6 @@ def print_chronicals_banner(num_gpus: int = 1, model_name: str = "", extra: Opti
     for k, v in (extra or {}).items():
         print(f"  {k}: {v}")
     print(line)
-
-
-_TEACHER = ("teacher_indices", "teacher_logits")      # a teacher's top logits [B, S, K], where a batch carries them
 
 
 def _batch_fields(batch: Any) -> Dict[str, Any]:
@@ -343,7 +341,7 @@ class ChronicalsTrainer:
         f = _batch_fields(batch)
         nb = bool(self.args.non_blocking_transfers)
         out: Dict[str, Any] = {}
-        for k in ("input_ids", "labels", "position_ids", "cu_seqlens", "attention_mask", *_TEACHER):
+        for k in ("input_ids", "labels", "position_ids", "cu_seqlens", "attention_mask", *TEACHER_KEYS):
             v = f.get(k)
             if isinstance(v, torch.Tensor):
                 out[k] = v.to(self.device, non_blocking=nb)
@@ -359,9 +357,9 @@ class ChronicalsTrainer:
             o = self.model(inp["input_ids"], position_ids=inp.get("position_ids"), labels=inp["labels"],
                            cu_seqlens=inp.get("cu_seqlens"), max_seqlen=inp.get("max_seqlen"),
                            seqlens_host=inp.get("seqlens_host"), shift_labels=bool(self._get("shift_labels", True)),
-                           **{k: inp[k] for k in _TEACHER if k in inp})
+                           **{k: inp[k] for k in TEACHER_KEYS if k in inp})
             return o.loss
-        if any(k in inp for k in _TEACHER):
+        if any(k in inp for k in TEACHER_KEYS):
             raise ValueError("a teacher's top logits in the batch: only this framework's own models have a distillation loss")
         kw = {"input_ids": inp["input_ids"], "labels": inp["labels"]}
         if inp.get("attention_mask") is not None and not self.args.use_sequence_packing:
@@ -411,7 +409,7 @@ class ChronicalsTrainer:
                                                cu_seqlens=inp.get("cu_seqlens"), max_seqlen=inp.get("max_seqlen"),
                                                seqlens_host=inp.get("seqlens_host"),
                                                shift_labels=bool(self._get("shift_labels", True)),
-                                               **{k: inp[k] for k in _TEACHER if k in inp})
+                                               **{k: inp[k] for k in TEACHER_KEYS if k in inp})
             self.optimizer.step()
             return loss
         if self._nvtx:
@@ -455,7 +453,7 @@ class ChronicalsTrainer:
                f.get("max_seqlen"), tuple(f["seqlens_host"]) if f.get("seqlens_host") is not None and
                not isinstance(f.get("cu_seqlens"), torch.Tensor) else None,
                # the static buffers keep their types, and the captured kernels the numbers they were given
-               tuple((k, tuple(f[k].shape), f[k].dtype) for k in ("position_ids", *_TEACHER) if isinstance(f.get(k), torch.Tensor)),
+               tuple((k, tuple(f[k].shape), f[k].dtype) for k in ("position_ids", *TEACHER_KEYS) if isinstance(f.get(k), torch.Tensor)),
                tuple(getattr(self.model, k, None) for k in ("distill_weight", "distill_temperature")))
         if self._graph is None or self._graph["key"] != key:
             self._capture_graph(f, key)
@@ -477,7 +475,7 @@ class ChronicalsTrainer:
         forward + backward + optimizer kernels of one micro-step into a CUDA graph."""
         a = self.args
         static: Dict[str, torch.Tensor] = {}
-        for k in ("input_ids", "labels", "position_ids", "cu_seqlens", *_TEACHER):
+        for k in ("input_ids", "labels", "position_ids", "cu_seqlens", *TEACHER_KEYS):
             v = f.get(k) if k != "labels" else f.get("labels", f["input_ids"])
             if isinstance(v, torch.Tensor):
                 static[k] = v.to(self.device).clone()
@@ -767,7 +765,7 @@ class ChronicalsTrainer:
                                                    position_ids=inp.get("position_ids"), cu_seqlens=inp.get("cu_seqlens"),
                                                    max_seqlen=inp.get("max_seqlen"),
                                                    shift_labels=bool(self._get("shift_labels", True)),
-                                                   **{k: inp[k] for k in _TEACHER if k in inp}).loss.float()
+                                                   **{k: inp[k] for k in TEACHER_KEYS if k in inp}).loss.float()
             else:
                 tot += self._forward_loss(inp).float()
             n += 1
