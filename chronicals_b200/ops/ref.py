@@ -356,13 +356,14 @@ def distillation_rows(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     """``(loss of every row, rows that take part)`` of ``logits [rows, V]`` against a teacher's top logits ``[rows, K]``:
     ``temperature**2 * KL(softmax(teacher / temperature) || softmax(logits / temperature))``, the teacher's distribution over the
     row's entries (those of one index add up), the student's over the vocabulary.  An entry whose index is outside the vocabulary or
-    whose logit is -inf is absent; a row without an entry, or with the ignored label, takes no part."""
+    whose logit is -inf is absent; a row without an entry, or with the ignored label, takes no part, and may hold anything."""
     z = (logits if logits.dtype == torch.float64 else logits.float()) / temperature
     t = teacher_logits.detach().to(z.dtype) / temperature
     on = (teacher_indices >= 0) & (teacher_indices < z.shape[1]) & (t != -math.inf)
     valid = on.any(1)
     if labels is not None:
         valid = valid & (labels != ignore_index)
+    z = z.masked_fill(~valid[:, None], 0.0)            # whatever they hold: 0 x NaN is NaN, in the gradient too
     q = torch.softmax(torch.where(valid[:, None], torch.where(on, t, -math.inf), 0.0), 1)
     at = torch.where(on, teacher_indices, 0).long()
     word = torch.zeros_like(z, requires_grad=False).scatter_add_(1, at, torch.where(on, q, 0.0)).gather(1, at)
