@@ -1359,8 +1359,9 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indi
                         reduction: str = "mean") -> torch.Tensor:
     """:func:`distillation_logits` of ``hidden @ weight.T`` without ever holding the ``[tokens, vocab]`` logits, as
     :func:`linear_cross_entropy` is :func:`cross_entropy_logits`, unless a gradient is wanted and all of them in fp32 take
-    no more than a gigabyte.  bf16 on CUDA runs on the kernels; the hidden states of rows that take no part have to be finite.  Like every product here it uses the device's one
-    workspace for split tiles: calls on two streams of a device must not overlap."""
+    no more than a gigabyte.  bf16 on CUDA runs on the kernels, of anything else a stretch of rows at a time is formed; the hidden
+    states of rows that take no part have to be finite.  Like every product here it uses the device's one workspace for split
+    tiles: calls on two streams of a device must not overlap."""
     lead = hidden.shape[:-1]
     if weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
         raise ValueError(f"linear_distillation: weight {tuple(weight.shape)} does not fit hidden states {tuple(hidden.shape)}")
@@ -1377,6 +1378,5 @@ def linear_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_indi
         fn = _LinearDistillHeldFn if grad and 4 * h.shape[0] * weight.shape[0] <= _HELD_LOGITS_BYTES else _LinearDistillFn
         loss = fn.apply(h, weight, idx, lg, y, ignore_index, float(temperature), reduction)
         return loss.view(lead) if reduction == "none" else loss
-    wide = torch.float64 if h.dtype == torch.float64 else torch.float32
-    rows, valid = ref.distillation_rows(h.to(wide) @ weight.to(wide).t(), idx, lg, float(temperature), y, ignore_index)
+    rows, valid = ref.linear_distillation_rows(h, weight, idx, lg, float(temperature), y, ignore_index)
     return ref.reduce_rows(rows.view(lead), valid, reduction)

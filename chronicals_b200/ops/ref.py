@@ -373,6 +373,28 @@ def distillation_rows(logits: torch.Tensor, teacher_indices: torch.Tensor, teach
     return temperature * temperature * terms.sum(1), valid
 
 
+LINEAR_DISTILL_VALUES = 1 << 26       # logits that are formed at a time
+
+
+def linear_distillation_rows(hidden: torch.Tensor, weight: torch.Tensor, teacher_indices: torch.Tensor, teacher_logits: torch.Tensor,
+                             temperature: float = 1.0, labels: Optional[torch.Tensor] = None, ignore_index: int = -100
+                             ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """:func:`distillation_rows` of ``hidden @ weight.T``, a stretch of rows at a time, whose logits are formed again for the gradient."""
+    wide = torch.float64 if hidden.dtype == torch.float64 else torch.float32
+    step = max(1, LINEAR_DISTILL_VALUES // weight.shape[0])
+
+    def stretch(h, w, idx, lg, y):
+        return distillation_rows(h.to(wide) @ w.to(wide).t(), idx, lg, temperature, y, ignore_index)
+
+    pieces = [(hidden[a:a + step], weight, teacher_indices[a:a + step], teacher_logits[a:a + step], None if labels is None else labels[a:a + step])
+              for a in range(0, max(1, hidden.shape[0]), step)]
+    if len(pieces) == 1:
+        return stretch(*pieces[0])
+    from torch.utils.checkpoint import checkpoint
+    rows, valid = zip(*(checkpoint(stretch, *p, use_reentrant=False, preserve_rng_state=False) for p in pieces))
+    return torch.cat(rows), torch.cat(valid)
+
+
 def reduce_rows(rows: torch.Tensor, valid: torch.Tensor, reduction: str) -> torch.Tensor:
     if reduction == "none":
         return rows

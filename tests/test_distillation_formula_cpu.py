@@ -1,10 +1,12 @@
-"""The formula's path of the distillation losses: rows that take no part are not read."""
+"""The formula's path of the distillation losses: rows that take no part are not read, and logits not all held at once."""
 import math
 
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from chronicals_b200 import ops
+from chronicals_b200.ops import ref
 from test_distillation_cpu import definition
 
 
@@ -26,6 +28,37 @@ def test_rows_that_take_no_part(value, reduction, dtype):
     want = {"none": rows, "sum": rows.sum(), "mean": rows.sum() / valid.sum()}[reduction]
     assert torch.allclose(loss.double(), want, rtol=1e-5)
     assert (grad[1:3] == 0).all()
-    (ref,) = torch.autograd.grad(rows[[0, 3]].sum() / (valid.sum() if reduction == "mean" else 1), z64)
+    (exact,) = torch.autograd.grad(rows[[0, 3]].sum() / (valid.sum() if reduction == "mean" else 1), z64)
     eps = torch.finfo(dtype).eps
-    assert (grad[[0, 3]].double() - ref[[0, 3]]).abs().max() <= eps / 2 * ref.abs().max() + 1e-6
+    assert (grad[[0, 3]].double() - exact[[0, 3]]).abs().max() <= eps / 2 * exact.abs().max() + 1e-6
+
+
+class _Largest(TorchDispatchMode):
+    values = 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        for t in out if isinstance(out, (tuple, list)) else (out,):
+            if isinstance(t, torch.Tensor):
+                self.values = max(self.values, t.numel())
+        return out
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_logits_are_formed_a_stretch_of_rows_at_a_time(monkeypatch, reduction, masked):
+    T, V, H, K = 37, 300, 8, 4
+    h, w = (torch.randn(n, H, dtype=torch.float64, requires_grad=True) for n in (T, V))
+    idx, lg = torch.randint(0, V, (T, K)), torch.randn(T, K)
+    labels = torch.arange(T).masked_fill(torch.arange(T) % 3 == 0, -100) if masked else None
+    up = torch.randn(T if reduction == "none" else ())
+    want = ops.linear_distillation(h, w, idx, lg, 1.5, labels, reduction=reduction)
+    dense = torch.autograd.grad(want, (h, w), up)
+    monkeypatch.setattr(ref, "LINEAR_DISTILL_VALUES", 5 * V)
+    with _Largest() as largest:
+        got = ops.linear_distillation(h, w, idx, lg, 1.5, labels, reduction=reduction)
+        grads = torch.autograd.grad(got, (h, w), up)
+    assert largest.values <= max(5 * V, V * H) < T * V
+    assert torch.allclose(got, want) and all(torch.allclose(a, b) for a, b in zip(grads, dense))
+    with torch.no_grad():
+        assert torch.equal(ops.linear_distillation(h, w, idx, lg, 1.5, labels, reduction=reduction), got)
