@@ -628,8 +628,7 @@ def qk_rope_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, position_i
     return torch.cat((q.reshape(T, nq), k.reshape(T, nk), qkv[:, nq + nk:]), dim=-1)
 
 
-def _whole(dtype: torch.dtype) -> bool:
-    return not (dtype.is_floating_point or dtype.is_complex or dtype == torch.bool)
+_WHOLE = frozenset((torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8, torch.uint16, torch.uint32, torch.uint64))
 
 
 def _same_device(op: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -704,7 +703,7 @@ def qk_rope_axes_(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
                          f"{num_q_heads}, {num_kv_heads}, {head_dim}")
     if not 1 <= len(sections) <= 4 or min(sections) < 0 or 2 * sum(sections) != head_dim:
         raise ValueError(f"qk_rope_axes_: sections {sections} must be one to four counts that sum up to head_dim / 2 = {head_dim / 2:g}")
-    if position_ids.shape != (len(sections), qkv.shape[0]) or not _whole(position_ids.dtype):
+    if position_ids.shape != (len(sections), qkv.shape[0]) or position_ids.dtype not in _WHOLE:
         raise ValueError(f"qk_rope_axes_: position_ids {tuple(position_ids.shape)} {position_ids.dtype}, wanted whole numbers of shape "
                          f"{(len(sections), qkv.shape[0])}")
     if cyclic and any(n and a + len(sections) * (n - 1) >= head_dim // 2 for a, n in enumerate(sections) if a):
@@ -1066,13 +1065,13 @@ def _distill_args(op, lead, V, idx, lg, temperature, labels, reduction, *others)
     K = idx.shape[-1] if idx.dim() else 0
     if idx.shape != (*lead, K) or lg.shape != idx.shape or K < 1:
         raise ValueError(f"{op}: teacher_indices {tuple(idx.shape)} and teacher_logits {tuple(lg.shape)}, wanted {(*lead, 'K')} with K >= 1")
-    if not _whole(idx.dtype):
+    if idx.dtype not in _WHOLE:
         raise ValueError(f"{op}: teacher_indices are {idx.dtype}, wanted whole numbers")
     if not lg.dtype.is_floating_point:
         raise ValueError(f"{op}: teacher_logits are {lg.dtype}, wanted floating-point numbers")
     if not (temperature > 0 and math.isfinite(temperature)):
         raise ValueError(f"{op}: temperature {temperature} must be positive and finite")
-    if labels is not None and (labels.shape != lead or not _whole(labels.dtype)):
+    if labels is not None and (labels.shape != lead or labels.dtype not in _WHOLE):
         raise ValueError(f"{op}: labels {tuple(labels.shape)} {labels.dtype}, wanted whole numbers of shape {tuple(lead)}")
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"{op}: reduction {reduction!r} is not 'mean', 'sum' or 'none'")
