@@ -25,7 +25,8 @@
 // pairs); 28 / 4 heads of 128, 8192 tokens, window 2048: 215 to 224 us (983 to 943).  On the GPU of the lower figures the form of attention.cu (64 keys a block, two score tiles) took 690 and 221 with
 // the same arithmetic, 822 and 232 with one score an instruction.  Tried besides: three and four CTAs an SM with one 64-key score
 // tile each 658 and 654 / -, two threads a row 650 / 234, P V in halves with P's half freed early 669 / 218, some exponentials on
-// the FMA pipe 618 (one pair in eight) to 690.
+// the FMA pipe 618 (one pair in eight) to 690.  The six warps' 168 registers (two CTAs an SM) are too few for the softmax warps: 144
+// bytes of spill stores and 384 of loads at head size 64, 84 and 220 at 128.
 //
 // P is rounded to bf16 (2^-9 on average) because the tensor core takes it so; sums, maxima and O stay in fp32.
 #include <algorithm>

@@ -104,7 +104,8 @@ __device__ __forceinline__ void kd_softmax(int K, const int* s_idx, float* s_lg,
   __syncthreads();
 }
 
-// the q of all entries with the index of entry k
+// the q of all entries with the index of entry k.  The square of the entries: 4096 rows of 32,000 words, bf16, with 64 / 256 / 1024 / 4096
+// entries each take 68 / 101 / 755 / 11,391 us for the loss on held logits (a row's entries are a few dozen as a rule).
 __device__ __forceinline__ float kd_merged(int K, const int* s_idx, const float* s_q, int k) {
   const int i = s_idx[k];
   float q = 0.f;
