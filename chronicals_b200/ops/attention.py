@@ -24,6 +24,9 @@ def _sdpa_docs(q, k, v, bounds: Sequence[int], causal: bool, scale: float) -> to
     """Library path: one SDPA call when all documents have equal length, else one per document."""
     T, hq, d = q.shape
     hk = k.shape[1]
+    if bounds[0] > 0:                                  # tokens before the first document
+        a = bounds[0]
+        return torch.cat((q.new_zeros(a, hq, d), _sdpa_docs(q[a:], k[a:], v[a:], [b - a for b in bounds], causal, scale)))
     lens = [b - a for a, b in zip(bounds[:-1], bounds[1:])]
     out = torch.zeros_like(q) if bounds[-1] < T else torch.empty_like(q)
     if lens and all(l == lens[0] for l in lens) and lens[0] > 0:

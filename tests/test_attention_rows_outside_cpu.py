@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from chronicals_b200 import ops
+from chronicals_b200.ops.attention import _sdpa_docs
 from test_attention_window_cpu import cu_of, dense
 
 
@@ -26,3 +27,16 @@ def test_rows_before_the_first_document(lens, lead, pad, window):
         assert torch.allclose(got, want, atol=1e-5)
         if got.requires_grad:
             assert torch.allclose(torch.autograd.grad(got, qkv, up, retain_graph=True)[0], ref, atol=1e-5)
+
+
+@pytest.mark.parametrize("lens,lead,pad", [([7], 3, 2), ([4, 0, 5], 1, 0), ([6, 6], 2, 1), ([6, 6], 0, 0)])
+def test_the_librarys_path(lens, lead, pad):
+    """Head sizes without a kernel, on the GPU."""
+    hq, hk, d, T = 4, 2, 8, lead + sum(lens) + pad
+    qkv = torch.randn(T, (hq + 2 * hk) * d, requires_grad=True)
+    q, k, v = (t.reshape(T, -1, d) for t in qkv.split((hq * d, hk * d, hk * d), 1))
+    got = _sdpa_docs(q, k, v, (lead + cu_of(lens)).tolist(), True, d ** -0.5).reshape(T, -1)
+    want = definition(qkv, lens, lead, hq, hk, d, T, 0)
+    up = torch.randn_like(want)
+    assert torch.allclose(got, want, atol=1e-5)
+    assert torch.allclose(torch.autograd.grad(got, qkv, up, retain_graph=True)[0], torch.autograd.grad(want, qkv, up)[0], atol=1e-5)
