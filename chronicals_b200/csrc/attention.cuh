@@ -62,7 +62,7 @@ __device__ __forceinline__ int lane_of_item(int& b, int mine) {
 // BY_WEIGHT (head size 64): two to 32 documents are handed out by weight, the blocks that a tile's loop visits, at most a.cap: first
 // all tiles of full weight, then those of every lower one, of which a document has at most one (14 / 2 heads of 64, 9 documents in 8192 tokens, window 1024,
 // backward: 124 us in the order of the documents, 114 so).  More of them go in their order: a search through more lengths than a
-// register holds, level by level, takes longer than it saves (40 documents: 74 and 94 us); empty ones behind the 32nd, to which a
+// register holds, level by level, takes longer than it saves (40 documents: 74 and 94 us); empty ones behind the 32nd, with which a
 // list may have been filled up, do not count.  A single document's tiles are in that
 // order already; with heads of 128, whose tiles take more rounds, the order of the documents is the faster one (16 documents, 28 / 4
 // heads, window 512: 248 and 260 us).
@@ -144,8 +144,8 @@ __device__ __forceinline__ void window_query_blocks(const AttnArgs& a, int jb, i
 }
 
 // The grid of ceil(T / 128) + n_docs CTAs (per head) holds enough past the last tile for the rows of no document: where n rows lie
-// before cu[0] or at and after cu[n_docs] at least ceil(n / 128), since T - n tokens fill at most (T - n + 127 n_docs) / 128 tiles.  In the forward kernels they write
-// those rows' zeros, 128 rows x D columns each, so the caller need not clear the output first.
+// before cu[0] or at and after cu[n_docs] at least ceil(n / 128), since T - n tokens fill at most (T - n + 127 n_docs) / 128 tiles.
+// In the forward kernels they write those rows' zeros, 128 rows x D columns each, so the caller need not clear the output first.
 template <int D>
 __device__ __forceinline__ void zero_padding_rows(const AttnArgs& a, int beyond, int h) {
   const int lead = min(max(a.cu[0], 0), a.T), valid = max(a.cu[a.n_docs], lead);

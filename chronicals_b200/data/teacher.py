@@ -31,7 +31,7 @@ def teacher_of(sample: Any) -> Optional[Pair]:
     n = torch.as_tensor(sample["input_ids"]).numel()
     if idx.dim() != 2 or idx.shape != lg.shape or idx.shape[0] != n or idx.shape[1] < 1:
         raise ValueError(f"teacher_indices {tuple(idx.shape)} and teacher_logits {tuple(lg.shape)} of a sample, wanted {(n, 'K')}")
-    if idx.dtype.is_floating_point or not lg.dtype.is_floating_point:
+    if idx.dtype.is_floating_point or idx.dtype.is_complex or idx.dtype == torch.bool or not lg.dtype.is_floating_point:
         raise ValueError(f"teacher_indices {idx.dtype} and teacher_logits {lg.dtype} of a sample, wanted whole and floating-point numbers")
     return idx.long(), lg
 

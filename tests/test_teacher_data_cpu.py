@@ -99,7 +99,7 @@ def test_loss_of_packed_documents():
 @pytest.mark.parametrize("change,what", [
     (dict(teacher_logits=None), "together"), (dict(teacher_indices=torch.zeros(6, 3, dtype=torch.long)), "wanted"),
     (dict(teacher_logits=torch.zeros(7, 2)), "wanted"), (dict(teacher_indices=torch.zeros(7, 3)), "whole"),
-    (dict(teacher_logits=torch.zeros(7, 3, dtype=torch.long)), "whole"), (dict(position_ids=torch.zeros(3, 7, dtype=torch.long)), "axes")])
+    (dict(teacher_indices=torch.ones(7, 3, dtype=torch.bool)), "whole"), (dict(teacher_logits=torch.zeros(7, 3, dtype=torch.long)), "whole"), (dict(position_ids=torch.zeros(3, 7, dtype=torch.long)), "axes")])
 @pytest.mark.parametrize("take", [lambda s: FixedShapeSequencePacker(12).pack_all_sequences(s), lambda s: SequencePackerV2(12).pack(s),
                                   lambda s: DataCollator()(s), lambda s: DataCollatorWithFlattening()(s)])
 def test_refusals(change, what, take):
